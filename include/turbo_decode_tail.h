@@ -48,7 +48,10 @@ enum {
     TURBO_ABI_SAMPLING_ROW = 2,   /* TurboSamplingRow */
     TURBO_ABI_STEP_INPUTS = 3,    /* TurboStepInputs */
     TURBO_ABI_ROW_REPORT = 4,     /* TurboRowReport */
-    TURBO_ABI_STEP_OUTPUTS = 5    /* TurboStepOutputs */
+    TURBO_ABI_STEP_OUTPUTS = 5,   /* TurboStepOutputs */
+    TURBO_ABI_KV_CACHE_DESC = 6,  /* TurboKvCacheDesc */
+    TURBO_ABI_ROTARY_DESC = 7,    /* TurboRotaryDesc */
+    TURBO_ABI_QKV_INPUTS = 8      /* TurboQkvInputs */
 };
 TURBO_DT_API uint32_t turbo_abi_version(void);
 /* sizeof of the struct TURBO_ABI_* names, as the library was built; 0 for an unknown id. */
@@ -316,6 +319,118 @@ TURBO_DT_API void turbo_int4_matrix_destroy(void* matrix);
  * turbo_int4_matvec on a head of the same matrix. */
 TURBO_DT_API int turbo_int4_matvec_grouped(void* const* matrices, int count, const float* const* x,
                                            float* const* out, void* hip_stream);
+
+/*
+ * ---- attention of the layer loop -----------------------------------------------------------
+ * What stands between the k/q/v projections (turbo_int4_matvec, turbo_int4_matvec_grouped) and the
+ * output projection: the norms of the query and key heads with the position rotation, a paged
+ * cache that holds keys and values in the tables' own affine format, and attention over it for a
+ * batch whose sequences share a prefix. They take the place of the reference's QKVEpilogue and
+ * Attention dispatches (shaders/QKVEpilogue.hlsl, shaders/Attention.hlsl).
+ *
+ * Common rules: head_dim is 64, 128, 256 or 512. Activations are FP32 or BF16 (TURBO_HIDDEN_*),
+ * [token][head][head_dim] with the heads of a token contiguous; a stride is the number of elements
+ * from one token to the next (0: heads * head_dim), so heads may be slices of a wider row. Buffers
+ * are 16-byte aligned and strides a multiple of 16 bytes. The work is enqueued on hip_stream and
+ * allocates nothing, so the calls may be captured into a HIP graph. A handle's calls are serialised
+ * by the caller; its destroy waits for the streams its calls were enqueued on (the whole device
+ * when more than four were used), which must still exist.
+ */
+
+/*
+ * Keys and values of one layer, quantised as they are written. The cache is `pages` pages of
+ * page_tokens tokens; slot s is token s % page_tokens of page s / page_tokens. Every 64 values of a
+ * (token, head) are one group: with L = 2^bits - 1, bias = the smallest value rounded down to BF16,
+ * scale = (the largest value - bias) / L rounded up to BF16 (at least 2^-126), and a value's code is
+ * (value - bias) / scale rounded to the nearest integer, ties to even, limited to 0..L. It reads back
+ * as code * scale + bias. A group that holds a value of magnitude 2^126 or more, or NaN, reads back as
+ * NaN. The layout in memory is the kernels' own.
+ */
+typedef struct {
+    uint32_t pages;        /* at least 1; pages * page_tokens at most 2^32 - 2 */
+    uint32_t page_tokens;  /* 32, 64, 128 or 256 */
+    uint32_t kv_heads;     /* 1 .. 1024 */
+    uint32_t head_dim;     /* 64, 128, 256 or 512 */
+    uint32_t bits;         /* 4 or 8 */
+    int device;            /* HIP device ordinal */
+} TurboKvCacheDesc;
+
+/* Marks a token that is not written (turbo_kv_cache_write, turbo_qk_norm_rope); like every slot past
+ * the cache it reads back as NaN. */
+#define TURBO_NO_SLOT 0xFFFFFFFFu
+
+/* 64-token pages, 8 key/value heads of 256 values, 8 bits, no pages yet. */
+TURBO_DT_API void turbo_kv_cache_desc_default(TurboKvCacheDesc* out);
+/* Allocates the cache: per token and head 2 * (head_dim * bits / 8 + head_dim / 16) bytes. The
+ * contents are undefined until they are written. NULL on failure. */
+TURBO_DT_API void* turbo_kv_cache_create(const TurboKvCacheDesc* desc);
+TURBO_DT_API void turbo_kv_cache_destroy(void* cache);
+/* Quantises k and v of `tokens` tokens ([token][kv_heads][head_dim]) into the device slots slots[i].
+ * A slot past the cache is skipped. The slots of one call differ: what a repeated one holds afterwards
+ * is undefined. */
+TURBO_DT_API int turbo_kv_cache_write(void* cache, const void* k, size_t k_stride, const void* v, size_t v_stride,
+                                      int dtype, const uint32_t* slots, int tokens, void* hip_stream);
+/* Reads `tokens` tokens back (dtype rounds once, to nearest even): out[i] = the token at slots[i], NaN
+ * for a slot past the cache. k or v may be NULL. */
+TURBO_DT_API int turbo_kv_cache_read(void* cache, const uint32_t* slots, int tokens, int dtype, void* k, size_t k_stride,
+                                     void* v, size_t v_stride, void* hip_stream);
+
+enum {
+    TURBO_ROPE_HALVES = 0, /* pair i is (x[i], x[i + rotary_dim / 2]); rotary_dim a multiple of 16 */
+    TURBO_ROPE_PAIRS = 1   /* pair i is (x[2 i], x[2 i + 1]) */
+};
+enum { TURBO_NORM_Q = 1u, TURBO_NORM_K = 2u, TURBO_NORM_V = 4u };
+
+/*
+ * The norms and the rotation of one layer's heads. A normed head is x / sqrt(mean(x^2) + eps), times
+ * the weight where there is one (plain w, as norm_weight of TurboLMHeadDesc; values have none). Then
+ * pair i < rotary_dim / 2 of a query or key at position p turns by p * theta^(-2 i / rotary_dim)
+ * radians, or p * inv_freq[i] where inv_freq is given (0 leaves a pair as it is); the other elements
+ * pass. The angle is exact to 2^-32 turns for every position below 2^32.
+ */
+typedef struct {
+    uint32_t head_dim;
+    uint32_t rotary_dim;         /* even, 0 .. head_dim */
+    int layout;                  /* TURBO_ROPE_* */
+    uint32_t norms;              /* TURBO_NORM_* */
+    float eps;
+    int weights_on_device;       /* of the two norm weights; inv_freq is host memory */
+    double theta;
+    const double* inv_freq;      /* [rotary_dim / 2], finite, or NULL */
+    const uint16_t* q_norm;      /* [head_dim] BF16 or NULL */
+    const uint16_t* k_norm;
+    int device;
+} TurboRotaryDesc;
+
+/* Heads of 256 that rotate whole in halves with theta 10000, queries and keys normed with eps 1e-6,
+ * no weights. */
+TURBO_DT_API void turbo_rotary_desc_default(TurboRotaryDesc* out);
+/* Copies the weights (device weights as the null stream has them) and lays out the frequencies. NULL on failure. */
+TURBO_DT_API void* turbo_rotary_create(const TurboRotaryDesc* desc);
+TURBO_DT_API void turbo_rotary_destroy(void* rotary);
+
+typedef struct {
+    int tokens;                  /* >= 0 */
+    int dtype;                   /* TURBO_HIDDEN_* of q, k, v, q_out and k_out */
+    int q_heads;
+    int kv_heads;
+    const void* q;               /* NULL: no queries */
+    const void* k;               /* NULL: no keys */
+    const void* v;               /* only for the cache, which needs k and v */
+    size_t q_stride, k_stride, v_stride;
+    const uint32_t* positions;   /* [tokens] */
+    /* where the turned heads go, rounded to dtype once: q (needed with q), k (NULL: only the cache takes
+     * them). An output may be its own input, with its stride, and may overlap nothing else. */
+    void* q_out;
+    void* k_out;
+    size_t q_out_stride, k_out_stride;
+    /* NULL, or the cache that takes the turned keys and the values, quantised from FP32; token i goes to
+     * slots[i] as in turbo_kv_cache_write */
+    void* cache;
+    const uint32_t* slots;
+} TurboQkvInputs;
+
+TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void* hip_stream);
 
 /*
  * Embedding lookup on the same tied table (shaders/EmbedLookup.hlsl:1-45; CPU

@@ -588,6 +588,9 @@ TURBO_DT_API size_t turbo_abi_struct_size(int which) {
         case TURBO_ABI_STEP_INPUTS: return sizeof(TurboStepInputs);
         case TURBO_ABI_ROW_REPORT: return sizeof(TurboRowReport);
         case TURBO_ABI_STEP_OUTPUTS: return sizeof(TurboStepOutputs);
+        case TURBO_ABI_KV_CACHE_DESC: return sizeof(TurboKvCacheDesc);
+        case TURBO_ABI_ROTARY_DESC: return sizeof(TurboRotaryDesc);
+        case TURBO_ABI_QKV_INPUTS: return sizeof(TurboQkvInputs);
         default: return 0;
     }
 }

@@ -23,6 +23,12 @@ TURBO_HIDDEN_BF16 = 1
 TURBO_STEP_NORMED = 1
 TURBO_STEP_APPEND_HISTORY = 2
 TURBO_STATUS_HISTORY_FULL = 1
+TURBO_NO_SLOT = 0xFFFFFFFF
+TURBO_ROPE_HALVES = 0
+TURBO_ROPE_PAIRS = 1
+TURBO_NORM_Q = 1
+TURBO_NORM_K = 2
+TURBO_NORM_V = 4
 
 # Every symbol include/turbo_decode_tail.h declares.
 EXPORTS = (
@@ -59,6 +65,15 @@ EXPORTS = (
     "turbo_int4_matrix_load",
     "turbo_int4_matrix_destroy",
     "turbo_int4_matvec_grouped",
+    "turbo_kv_cache_desc_default",
+    "turbo_kv_cache_create",
+    "turbo_kv_cache_destroy",
+    "turbo_kv_cache_write",
+    "turbo_kv_cache_read",
+    "turbo_rotary_desc_default",
+    "turbo_rotary_create",
+    "turbo_rotary_destroy",
+    "turbo_qk_norm_rope",
 )
 
 TURBO_NOALLOC_MAX_BATCH = 4
@@ -158,6 +173,55 @@ class TurboBundleTensor(C.Structure):
     ]
 
 
+class TurboKvCacheDesc(C.Structure):
+    _fields_ = [
+        ("pages", C.c_uint32),
+        ("page_tokens", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("bits", C.c_uint32),
+        ("device", C.c_int),
+    ]
+
+
+class TurboRotaryDesc(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_uint32),
+        ("rotary_dim", C.c_uint32),
+        ("layout", C.c_int),
+        ("norms", C.c_uint32),
+        ("eps", C.c_float),
+        ("weights_on_device", C.c_int),
+        ("theta", C.c_double),
+        ("inv_freq", C.c_void_p),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+        ("device", C.c_int),
+    ]
+
+
+class TurboQkvInputs(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int),
+        ("dtype", C.c_int),
+        ("q_heads", C.c_int),
+        ("kv_heads", C.c_int),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_stride", C.c_size_t),
+        ("k_stride", C.c_size_t),
+        ("v_stride", C.c_size_t),
+        ("positions", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p),
+        ("q_out_stride", C.c_size_t),
+        ("k_out_stride", C.c_size_t),
+        ("cache", C.c_void_p),
+        ("slots", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -208,6 +272,15 @@ def load(path: os.PathLike | str | None = None) -> C.CDLL:
         "turbo_int4_matrix_load": (i32, [vp, vp, vp, vp, i32, vp]),
         "turbo_int4_matrix_destroy": (None, [vp]),
         "turbo_int4_matvec_grouped": (i32, [vp, i32, vp, vp, vp]),
+        "turbo_kv_cache_desc_default": (None, [C.POINTER(TurboKvCacheDesc)]),
+        "turbo_kv_cache_create": (vp, [C.POINTER(TurboKvCacheDesc)]),
+        "turbo_kv_cache_destroy": (None, [vp]),
+        "turbo_kv_cache_write": (i32, [vp, vp, C.c_size_t, vp, C.c_size_t, i32, vp, i32, vp]),
+        "turbo_kv_cache_read": (i32, [vp, vp, i32, i32, vp, C.c_size_t, vp, C.c_size_t, vp]),
+        "turbo_rotary_desc_default": (None, [C.POINTER(TurboRotaryDesc)]),
+        "turbo_rotary_create": (vp, [C.POINTER(TurboRotaryDesc)]),
+        "turbo_rotary_destroy": (None, [vp]),
+        "turbo_qk_norm_rope": (i32, [vp, C.POINTER(TurboQkvInputs), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -443,6 +516,104 @@ def matvec_grouped(matrices, xs, outs, stream=None) -> None:
     n = len(matrices)
     mats, xp, op = array("Q", [m.h or 0 for m in matrices]), _ptrs(xs, n), _ptrs(outs, n)
     _ok(load().turbo_int4_matvec_grouped(mats.buffer_info()[0], n, xp.buffer_info()[0], op.buffer_info()[0], stream))
+
+
+def _stride(t) -> int:
+    """Elements from one token to the next of a [tokens][heads][head_dim] tensor (0, packed, for a raw address).
+    Heads of a token are contiguous; anything else cannot be passed."""
+    if t is None or not hasattr(t, "stride"):
+        return 0
+    if t.dim() == 3 and t.shape[0] and (t.stride(2) != 1 or t.stride(1) != t.shape[2]):
+        raise ValueError("the heads of a token must be contiguous")
+    return 0 if t.is_contiguous() else t.stride(0)
+
+
+class KvCache:
+    """One turbo_kv_cache handle: a layer's keys and values in pages, quantised to 4 or 8 bits.
+    Buffers are torch CUDA tensors [tokens][kv_heads][head_dim] or raw addresses (packed)."""
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, *, bits: int = 8, device: int = 0):
+        self.lib = load()
+        d = TurboKvCacheDesc(pages, page_tokens, kv_heads, head_dim, bits, device)
+        self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.bits = pages, page_tokens, kv_heads, head_dim, bits
+        self.h = self.lib.turbo_kv_cache_create(C.byref(d))
+        if not self.h:
+            raise TurboError(last_error())
+
+    def write(self, k, v, slots, tokens: int, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
+        """Quantises k and v of `tokens` tokens into slots (device ids; TURBO_NO_SLOT skips a token)."""
+        _ok(self.lib.turbo_kv_cache_write(self.h, _ptr(k), _stride(k), _ptr(v), _stride(v), dtype, _ptr(slots), tokens, stream))
+
+    def read(self, slots, tokens: int, k_out, v_out, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
+        """k_out, v_out (either may be None) = the tokens at slots; NaN for a slot past the cache."""
+        _ok(self.lib.turbo_kv_cache_read(self.h, _ptr(slots), tokens, dtype, _ptr(k_out), _stride(k_out), _ptr(v_out),
+                                         _stride(v_out), stream))
+
+    def close(self) -> None:
+        if getattr(self, "h", None):
+            self.lib.turbo_kv_cache_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Rotary:
+    """One turbo_rotary handle: the norms and the position rotation of a layer's heads. Weights: BF16 bits
+    as numpy uint16 (host) or torch CUDA bfloat16 tensors (device), both of a kind; inv_freq: host doubles."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, theta: float = 10000.0, inv_freq=None,
+                 layout: int = TURBO_ROPE_HALVES, norms: int = TURBO_NORM_Q | TURBO_NORM_K, eps: float = 1e-6, q_norm=None,
+                 k_norm=None, device: int = 0):
+        self.lib = load()
+        d = TurboRotaryDesc()
+        self.lib.turbo_rotary_desc_default(C.byref(d))
+        d.head_dim, d.rotary_dim = head_dim, head_dim if rotary_dim is None else rotary_dim
+        d.layout, d.norms, d.eps, d.theta, d.device = layout, norms, eps, theta, device
+        weights = [w for w in (q_norm, k_norm) if w is not None]
+        d.weights_on_device = 1 if weights and hasattr(weights[0], "data_ptr") else 0
+        if len({hasattr(w, "data_ptr") for w in weights}) > 1:
+            raise ValueError("q_norm and k_norm must both be host arrays or both device tensors")
+        for w in weights:
+            if len(w) != head_dim:
+                raise ValueError("a norm weight has head_dim values")
+        hp = (lambda w: None if w is None else w.data_ptr()) if d.weights_on_device else (
+            lambda w: None if w is None else w.ctypes.data)
+        d.q_norm, d.k_norm = hp(q_norm), hp(k_norm)
+        if inv_freq is not None:
+            freqs = (C.c_double * max(1, len(inv_freq)))(*[float(f) for f in inv_freq])
+            if len(inv_freq) != d.rotary_dim // 2:
+                raise ValueError("inv_freq has rotary_dim / 2 values")
+            d.inv_freq = C.addressof(freqs)
+        self.head_dim = head_dim
+        self.h = self.lib.turbo_rotary_create(C.byref(d))
+        if not self.h:
+            raise TurboError(last_error())
+
+    @staticmethod
+    def make_inputs(tokens: int, *, dtype: int = TURBO_HIDDEN_F32, q=None, k=None, v=None, q_heads: int = 0, kv_heads: int = 0,
+                    positions=None, q_out=None, k_out=None, cache: KvCache | None = None, slots=None) -> TurboQkvInputs:
+        inp = TurboQkvInputs(tokens, dtype, q_heads, kv_heads, _ptr(q), _ptr(k), _ptr(v), _stride(q), _stride(k), _stride(v),
+                             _ptr(positions), _ptr(q_out), _ptr(k_out), _stride(q_out), _stride(k_out),
+                             cache.h if cache is not None else None, _ptr(slots))
+        return inp
+
+    def apply(self, inp: TurboQkvInputs, stream=None) -> None:
+        _ok(self.lib.turbo_qk_norm_rope(self.h, C.byref(inp), stream))
+
+    def close(self) -> None:
+        if getattr(self, "h", None):
+            self.lib.turbo_rotary_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def sample_logits_noalloc(logits, vocab: int, inp: TurboStepInputs, tokens, report=None, *,
