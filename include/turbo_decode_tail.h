@@ -51,7 +51,8 @@ enum {
     TURBO_ABI_STEP_OUTPUTS = 5,   /* TurboStepOutputs */
     TURBO_ABI_KV_CACHE_DESC = 6,  /* TurboKvCacheDesc */
     TURBO_ABI_ROTARY_DESC = 7,    /* TurboRotaryDesc */
-    TURBO_ABI_QKV_INPUTS = 8      /* TurboQkvInputs */
+    TURBO_ABI_QKV_INPUTS = 8,     /* TurboQkvInputs */
+    TURBO_ABI_ATTENTION_INPUTS = 9 /* TurboAttentionInputs */
 };
 TURBO_DT_API uint32_t turbo_abi_version(void);
 /* sizeof of the struct TURBO_ABI_* names, as the library was built; 0 for an unknown id. */
@@ -431,6 +432,45 @@ typedef struct {
 } TurboQkvInputs;
 
 TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void* hip_stream);
+
+/*
+ * Attention of a batch over the cache. Sequence b holds kv_len[b] tokens: the first prefix_len are the
+ * shared prefix, token p of it on page prefix_pages[p / page_tokens], and token prefix_len + j is its
+ * own, on page pages[b * page_stride + j / page_tokens]. Its last q_len tokens are the queries, whose
+ * own keys are in the cache already: query t is at position kv_len[b] - q_len + t and sees every token
+ * up to its own, the last `window` of them where window is not 0.
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * over the tokens that it sees, query head h over key/value head h / (q_heads / kv_heads). A query at
+ * a negative position sees nothing and gives zeros (kv_len 0: a padded sequence). A query whose tokens
+ * pass its page table, or lie on a page past the cache, gives NaN.
+ * The prefix is read once for the whole batch: its products run over the rows of all sequences. Products
+ * accumulate in FP32; FP32 queries keep 22 bits in them, BF16 ones 11 bits of the softmax weights.
+ */
+typedef struct {
+    int batch;                   /* >= 0 */
+    int q_len;                   /* >= 1 */
+    int q_heads;                 /* a multiple of the cache's kv_heads */
+    int dtype;                   /* TURBO_HIDDEN_* of q and out */
+    const void* q;               /* [batch * q_len][q_heads][head_dim] */
+    void* out;                   /* the same shape; does not overlap q */
+    size_t q_stride, out_stride;
+    const uint32_t* kv_len;      /* [batch] */
+    uint32_t max_kv_len;         /* what kv_len may reach; sizes the launch, longer sequences are slower, not wrong */
+    uint32_t prefix_len;
+    const uint32_t* prefix_pages;
+    const uint32_t* pages;       /* [batch][page_stride]; NULL when page_stride is 0 */
+    uint32_t page_stride;
+    uint32_t window;
+    float scale;
+    /* device scratch of turbo_attention_workspace bytes, 16-byte aligned; calls that may overlap (two
+     * streams, two graphs) have one each */
+    void* workspace;
+    size_t workspace_bytes;
+} TurboAttentionInputs;
+
+/* The scratch a call with these sizes needs (0: none); pointers are not looked at. */
+TURBO_DT_API int turbo_attention_workspace(void* cache, const TurboAttentionInputs* in, size_t* bytes);
+TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs* in, void* hip_stream);
 
 /*
  * Embedding lookup on the same tied table (shaders/EmbedLookup.hlsl:1-45; CPU

@@ -29,7 +29,7 @@ def outward(x, up):
 def quantise(x, bits):
     """(codes, scale, bias) of the last axis's groups of 64, in the fp32 operations that define the format."""
     x = np.asarray(x, np.float32)
-    g = x.reshape(*x.shape[:-1], -1, 64)
+    g = x.reshape(*x.shape[:-1], x.shape[-1] // 64, 64)
     top = 2**bits - 1
     finite = (np.abs(g) < 2.0**126).all(axis=-1)
     safe = np.where(finite[..., None], g, np.float32(0))

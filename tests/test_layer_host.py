@@ -63,7 +63,7 @@ def test_every_value_has_its_place(tmp_path):
 
 def test_struct_sizes():
     lib = T.load()
-    for which, st in ((6, T.TurboKvCacheDesc), (7, T.TurboRotaryDesc), (8, T.TurboQkvInputs)):
+    for which, st in ((6, T.TurboKvCacheDesc), (7, T.TurboRotaryDesc), (8, T.TurboQkvInputs), (9, T.TurboAttentionInputs)):
         assert lib.turbo_abi_struct_size(which) == C.sizeof(st), st.__name__
 
 
@@ -106,6 +106,8 @@ def test_null_handles():
     assert lib.turbo_kv_cache_write(None, None, 0, None, 0, 0, None, 1, None) == 0 and "handle" in T.last_error()
     assert lib.turbo_kv_cache_read(None, None, 1, 0, None, 0, None, 0, None) == 0 and "handle" in T.last_error()
     assert lib.turbo_qk_norm_rope(None, None, None) == 0 and "handle" in T.last_error()
+    assert lib.turbo_prefix_attention(None, None, None) == 0 and "handle" in T.last_error()
+    assert lib.turbo_attention_workspace(None, None, None) == 0 and "handle" in T.last_error()
     assert not lib.turbo_kv_cache_create(None) and not lib.turbo_rotary_create(None)
 
 

@@ -591,6 +591,7 @@ TURBO_DT_API size_t turbo_abi_struct_size(int which) {
         case TURBO_ABI_KV_CACHE_DESC: return sizeof(TurboKvCacheDesc);
         case TURBO_ABI_ROTARY_DESC: return sizeof(TurboRotaryDesc);
         case TURBO_ABI_QKV_INPUTS: return sizeof(TurboQkvInputs);
+        case TURBO_ABI_ATTENTION_INPUTS: return sizeof(TurboAttentionInputs);
         default: return 0;
     }
 }

@@ -111,12 +111,12 @@ struct AttnArgs {
 struct AttnPlan {
     uint32_t prefix_tile_rows, own_tile_rows;  // 16 or 32 rows to a workgroup
     uint32_t prefix_tiles, prefix_splits, own_tiles, own_splits;
-    uint64_t items, rows;
+    uint64_t prefix_items, items, rows;
     uint32_t parts;
     uint64_t stats_bytes, bytes;
 };
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
-                        uint32_t prefix_len, uint32_t own_most, uint32_t cus);
+                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus);
 void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);
 
 }  // namespace tdt

@@ -103,6 +103,24 @@ size_t check_rows(const char* name, const void* p, size_t stride, size_t packed,
     return stride;
 }
 
+// The sizes of an attention call, checked, and how it is split.
+tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in) {
+    dtype_size(in.dtype);
+    if (in.batch < 0 || in.batch > (1 << 20)) fail("batch must be in 0..1048576");
+    if (in.q_len < 1 || in.q_len > (1 << 20)) fail("q_len must be in 1..1048576");
+    if (in.q_heads < 1 || in.q_heads > (int)kMaxQueryHeads || in.q_heads % (int)c.kv.heads != 0)
+        fail("q_heads must be a multiple of the cache's kv_heads, at most " + std::to_string(kMaxQueryHeads));
+    const uint64_t room = (uint64_t)in.page_stride * c.page_tokens;
+    if (in.prefix_len > 0x7FFFFF00u || room > 0x7FFFFF00u) fail("prefix_len and page_stride * page_tokens must be below 2^31 - 256");
+    const uint64_t beyond = in.max_kv_len > in.prefix_len ? in.max_kv_len - in.prefix_len : 0u;
+    const tdt::AttnPlan p =
+        tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype,
+                            in.prefix_len, (uint32_t)(room == 0u ? 0u : beyond == 0u ? 1u : beyond < room ? beyond : room),
+                            in.window, c.cus);
+    if (p.items > (1u << 24) - 1u || p.rows * (c.head_dim / 4u) > 0xFFFFFF00ull) fail("batch * q_len * q_heads is too large for one call");
+    return p;
+}
+
 }  // namespace
 
 #define ATT_TRY            \
@@ -364,6 +382,61 @@ TURBO_DT_API int turbo_qk_norm_rope(void* handle, const TurboQkvInputs* in, void
     r->streams.note(static_cast<hipStream_t>(hip_stream));
     if (c) c->streams.note(static_cast<hipStream_t>(hip_stream));
     tdt::launch_qkv(a, r->head_dim, in->dtype, static_cast<hipStream_t>(hip_stream));
+    return 1;
+    ATT_CATCH(0)
+}
+
+// ---- attention ---------------------------------------------------------------------------------------
+
+TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInputs* in, size_t* bytes) {
+    ATT_TRY
+    CacheBox* c = cbox(handle);
+    if (!in || !bytes) fail("in or bytes is NULL");
+    *bytes = (size_t)attention_plan(*c, *in).bytes;
+    return 1;
+    ATT_CATCH(0)
+}
+
+TURBO_DT_API int turbo_prefix_attention(void* handle, const TurboAttentionInputs* in, void* hip_stream) {
+    ATT_TRY
+    CacheBox* c = cbox(handle);
+    if (!in) fail("in is NULL");
+    const tdt::AttnPlan plan = attention_plan(*c, *in);
+    if (!std::isfinite(in->scale)) fail("scale must be finite");
+    if (in->batch == 0) return 1;
+    const size_t size = dtype_size(in->dtype), packed = (size_t)in->q_heads * c->head_dim;
+    tdt::AttnArgs a{};
+    a.q_stride = check_rows("q", in->q, in->q_stride, packed, size);
+    a.out_stride = check_rows("out", in->out, in->out_stride, packed, size);
+    if (in->q == in->out) fail("out is q");
+    if (!in->kv_len) fail("kv_len is NULL");
+    if (in->prefix_len && !in->prefix_pages) fail("prefix_pages is NULL");
+    if (in->page_stride && !in->pages) fail("pages is NULL");
+    if (plan.bytes) {
+        if (!in->workspace) fail("workspace is NULL");
+        if (reinterpret_cast<uintptr_t>(in->workspace) % 16u != 0u) fail("workspace must be 16-byte aligned");
+        if (in->workspace_bytes < plan.bytes)
+            fail("workspace holds " + std::to_string(in->workspace_bytes) + " bytes, the call needs " + std::to_string(plan.bytes));
+    }
+    a.kv = c->kv;
+    a.q = in->q;
+    a.out = in->out;
+    a.kv_len = in->kv_len;
+    a.prefix_pages = in->prefix_pages;
+    a.pages = in->pages;
+    a.prefix_len = in->prefix_len;
+    a.page_stride = in->page_stride;
+    a.batch = (uint32_t)in->batch;
+    a.q_len = (uint32_t)in->q_len;
+    a.q_heads = (uint32_t)in->q_heads;
+    a.group = a.q_heads / c->kv.heads;
+    a.window = in->window;
+    a.scale_log2e = (float)((double)in->scale * 1.4426950408889634);
+    a.stats = static_cast<float2*>(in->workspace);
+    a.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(in->workspace) + plan.stats_bytes);
+    tdt::DeviceGuard dg(c->device);
+    c->streams.note(static_cast<hipStream_t>(hip_stream));
+    tdt::launch_attention(a, plan, c->head_dim, in->dtype, static_cast<hipStream_t>(hip_stream));
     return 1;
     ATT_CATCH(0)
 }

@@ -74,6 +74,8 @@ EXPORTS = (
     "turbo_rotary_create",
     "turbo_rotary_destroy",
     "turbo_qk_norm_rope",
+    "turbo_attention_workspace",
+    "turbo_prefix_attention",
 )
 
 TURBO_NOALLOC_MAX_BATCH = 4
@@ -222,6 +224,29 @@ class TurboQkvInputs(C.Structure):
     ]
 
 
+class TurboAttentionInputs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("q_len", C.c_int),
+        ("q_heads", C.c_int),
+        ("dtype", C.c_int),
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_stride", C.c_size_t),
+        ("out_stride", C.c_size_t),
+        ("kv_len", C.c_void_p),
+        ("max_kv_len", C.c_uint32),
+        ("prefix_len", C.c_uint32),
+        ("prefix_pages", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("page_stride", C.c_uint32),
+        ("window", C.c_uint32),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -281,6 +306,8 @@ def load(path: os.PathLike | str | None = None) -> C.CDLL:
         "turbo_rotary_create": (vp, [C.POINTER(TurboRotaryDesc)]),
         "turbo_rotary_destroy": (None, [vp]),
         "turbo_qk_norm_rope": (i32, [vp, C.POINTER(TurboQkvInputs), vp]),
+        "turbo_attention_workspace": (i32, [vp, C.POINTER(TurboAttentionInputs), C.POINTER(C.c_size_t)]),
+        "turbo_prefix_attention": (i32, [vp, C.POINTER(TurboAttentionInputs), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -548,6 +575,25 @@ class KvCache:
         """k_out, v_out (either may be None) = the tokens at slots; NaN for a slot past the cache."""
         _ok(self.lib.turbo_kv_cache_read(self.h, _ptr(slots), tokens, dtype, _ptr(k_out), _stride(k_out), _ptr(v_out),
                                          _stride(v_out), stream))
+
+    @staticmethod
+    def make_attention_inputs(batch: int, *, dtype: int = TURBO_HIDDEN_F32, q, out, q_heads: int, q_len: int = 1, kv_len,
+                              max_kv_len: int, pages=None, prefix_len: int = 0, prefix_pages=None, window: int = 0, scale: float,
+                              workspace=None) -> TurboAttentionInputs:
+        """pages: [batch][page_stride] device ids. workspace: a uint8 tensor of attention_workspace(inputs) bytes."""
+        return TurboAttentionInputs(batch, q_len, q_heads, dtype, _ptr(q), _ptr(out), _stride(q), _stride(out), _ptr(kv_len),
+                                    max_kv_len, prefix_len, _ptr(prefix_pages) if prefix_len else None, _ptr(pages),
+                                    int(pages.shape[1]) if pages is not None else 0, window, scale, _ptr(workspace),
+                                    workspace.numel() if workspace is not None else 0)
+
+    def attention_workspace(self, inp: TurboAttentionInputs) -> int:
+        n = C.c_size_t()
+        _ok(self.lib.turbo_attention_workspace(self.h, C.byref(inp), C.byref(n)))
+        return n.value
+
+    def attend(self, inp: TurboAttentionInputs, stream=None) -> None:
+        """turbo_prefix_attention: out = softmax(scale q k) v over the shared prefix and each sequence's own keys."""
+        _ok(self.lib.turbo_prefix_attention(self.h, C.byref(inp), stream))
 
     def close(self) -> None:
         if getattr(self, "h", None):
