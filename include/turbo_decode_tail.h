@@ -344,7 +344,7 @@ TURBO_DT_API int turbo_int4_matvec_grouped(void* const* matrices, int count, con
  * (token, head) are one group: with L = 2^bits - 1, bias = the smallest value rounded down to BF16,
  * scale = (the largest value - bias) / L rounded up to BF16 (at least 2^-126), and a value's code is
  * (value - bias) / scale rounded to the nearest integer, ties to even, limited to 0..L. It reads back
- * as code * scale + bias. A group that holds a value of magnitude 2^126 or more, or NaN, reads back as
+ * as code * scale + bias. A group that holds a value of magnitude 2^103 or more, or NaN, reads back as
  * NaN. The layout in memory is the kernels' own.
  */
 typedef struct {
@@ -444,7 +444,9 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * a negative position sees nothing and gives zeros (kv_len 0: a padded sequence). A query whose tokens
  * pass its page table, or lie on a page past the cache, gives NaN.
  * The prefix is read once for the whole batch: its products run over the rows of all sequences. Products
- * accumulate in FP32; FP32 queries keep 22 bits in them, BF16 ones 11 bits of the softmax weights.
+ * accumulate in FP32; FP32 queries keep 22 bits of queries and softmax weights, BF16 ones 11 bits of the
+ * weights and, where more than 32 rows share keys, of keys and values (or 2^-25 of the largest of their
+ * 32 tokens).
  */
 typedef struct {
     int batch;                   /* >= 0 */

@@ -31,7 +31,7 @@ def quantise(x, bits):
     x = np.asarray(x, np.float32)
     g = x.reshape(*x.shape[:-1], x.shape[-1] // 64, 64)
     top = 2**bits - 1
-    finite = (np.abs(g) < 2.0**126).all(axis=-1)
+    finite = (np.abs(g) < 2.0**103).all(axis=-1)
     safe = np.where(finite[..., None], g, np.float32(0))
     lo, hi = safe.min(axis=-1), safe.max(axis=-1)
     bias = outward(lo, False)

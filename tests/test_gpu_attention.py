@@ -7,7 +7,9 @@ is off by at most scale * sum |q| K * (2^-22 + 80 * 2^-24): FP32 queries keep 22
 groups add in FP32 (BF16 queries are exact, the same bound holds); the factor and the exponential add
 (2 |s| + 2) 2^-23 to a weight's relative error. A weight is rounded to 2^-22 (FP32) or 2^-12 (BF16) of
 itself for the product with the values, which adds at most 32 + keys / 32 roundings, and the join and
-division 8 more. So |off| <= (2 e + w + (40 + keys / 32) 2^-24) sum p (|code * scale| + |bias|), and BF16 rounds
+division 8 more. Where more than 32 BF16 rows share keys, a key or value is rounded to fp16 twice (the
+middle code's value and the product's sum with it): 2^-11 K, or 2^-24 of the largest K of its 32 tokens.
+So |off| <= (2 e + w + (40 + keys / 32) 2^-24) sum p (|code * scale| + |bias|), and BF16 rounds
 the result by 2^-8 of it. Those are worst cases; the errors are independent, so the 2-norm must stay far
 below: under 4e-6 (FP32: 8 roundings' worth of a 64-term sum at the scores' size here) and 2.5e-3 (BF16:
 half a step is 2^-8 at most, 2^-9 / sqrt(3) * 1.4 on average over a binade)."""
@@ -101,9 +103,13 @@ def expect(s, q, b, q_len, kv_len, window, scale, dtype):
             w = np.exp(sc - sc.max())
             w /= w.sum()
             out[i, h] = w @ v[lo:hi, h // g]
-            e = scale * (kk[lo:hi, h // g] @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
-            rel = 2 * e.max() + (2.0**-22 if dtype == "f32" else 2.0**-12) + (40 + (hi - lo) / 32) * 2.0**-24
-            bound[i, h] = rel * (w @ vv[lo:hi, h // g])
+            ka, va = kk[lo:hi, h // g], vv[lo:hi, h // g]
+            e = scale * (ka @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
+            rel = (2.0**-22 if dtype == "f32" else 2.0**-12) + (40 + (hi - lo) / 32) * 2.0**-24
+            if dtype == "bf16":
+                e = e + scale * (ka @ np.abs(q[i, h]) * 2.0**-11 + np.nanmax(ka) * np.abs(q[i, h]).sum() * 2.0**-24)
+                rel += 2.0**-11
+            bound[i, h] = (2 * e.max() + rel) * (w @ va) + (np.nanmax(va) * 2.0**-24 if dtype == "bf16" else 0.0)
     if dtype == "bf16":
         bound += 2.0**-8 * (np.abs(out) + bound)
     return out, bound + 1e-37
@@ -167,6 +173,30 @@ def test_against_the_formula(dim, heads, group, page, bits, dtype, case):
     check(s, q, out, kv_len, q_len, window, dtype)
 
 
+MANY = {  # more than 32 rows over the same keys: prefix, own tokens, q_len, window
+    "batch": (333, [1, 40, 0, 77, 5] * 8, 1, 0),
+    "drafts": (100, [17, 60, 33] * 3, 17, 0),
+    "chunk": (0, [333], 300, 0),
+    "chunks": (64, [100, 0, 71], 71, 0),
+    "window": (500, [3, 90, 300] * 5, 3, 90),
+    "narrow": (40, [130], 130, 1),
+    "early": (0, [40], 70, 0),
+}
+
+
+@pytest.mark.parametrize("case", list(MANY))
+@pytest.mark.parametrize("dim,heads,group,page", [(64, 2, 3, 32), (128, 1, 8, 64), (256, 2, 2, 128), (512, 1, 5, 256)])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_over_the_same_keys(dim, heads, group, page, bits, dtype, case):
+    prefix, own, q_len, window = MANY[case]
+    rng = np.random.default_rng(dim + len(case))
+    s = Setup(rng, heads, dim, bits, page, prefix, own)
+    kv_len = [prefix + n if n else 0 for n in own]
+    q, out = run(s, rng, heads * group, kv_len, dtype=dtype, q_len=q_len, window=window)
+    check(s, q, out, kv_len, q_len, window, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_queries_before_the_first_token_and_sequences_inside_the_prefix(dtype):
     """More queries than tokens: those at negative positions give zeros. A sequence that has not reached the
@@ -200,18 +230,19 @@ def test_queries_past_their_pages_and_pages_past_the_cache_give_nan():
     assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all() and (out[2] == 0).all() and torch.isnan(out[3]).all()
 
 
-def test_values_that_are_not_finite_reach_only_the_rows_that_see_them():
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(dtype):
     rng = np.random.default_rng(3)
     s = Setup(rng, 2, 128, 8, 32, 64, [90, 90])
     s.v[64 + 50, 1, 70] = np.inf   # sequence 0's own token 50, head 1, second group
     s.k[64 + 90 + 10, 0, 3] = np.nan  # sequence 1's own token 10, head 0
     s.write(np.array([64 + 50, 64 + 90 + 10]))
-    q = queries(rng, 80, 4, 128, "f32")
+    q = queries(rng, 80, 4, 128, dtype)
     q[79, 3, 5] = np.nan
-    qt = tensor(q, "f32")
+    qt = tensor(q, dtype)
     out = torch.empty_like(qt)
-    s.cache.attend(inputs(s, qt, out, 4, [64 + 60, 64 + 40], dtype="f32", q_len=40))
-    got = out.cpu().numpy()
+    s.cache.attend(inputs(s, qt, out, 4, [64 + 60, 64 + 40], dtype=dtype, q_len=40))
+    got = out.float().cpu().numpy()
     nan = np.isnan(got)
     want = np.zeros_like(nan)
     want[30:40, 2:, 64:] = True   # queries at own positions 50 .. 59 of sequence 0, heads 2 and 3, that group
@@ -219,7 +250,7 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them():
     want[79, 3] = True
     assert np.array_equal(nan, want)
     for b, n in ((0, 124), (1, 104)):
-        w, bound = expect(s, np.nan_to_num(q[b * 40:b * 40 + 40]), b, 40, n, 0, 128**-0.5, "f32")
+        w, bound = expect(s, np.nan_to_num(q[b * 40:b * 40 + 40]), b, 40, n, 0, 128**-0.5, dtype)
         fine = ~want[b * 40:b * 40 + 40]
         assert np.all(np.abs(got[b * 40:b * 40 + 40][fine] - w[fine]) <= bound[fine])
 
@@ -247,6 +278,23 @@ def test_values_and_queries_of_any_size(bits, dtype):
         out = torch.empty_like(qt)
         s.cache.attend(inputs(s, qt, out, 2, [160, 196], dtype=dtype, scale=1 / 16 / size))
         check(s, q, out, [160, 196], 1, 0, dtype, scale=1 / 16 / size)
+
+
+@pytest.mark.parametrize("size", [1e-35, 1e-20, 1.0, 1e20, 1e36])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sizes_that_many_rows_share(size, dtype):
+    """Keys and values of any size, also growing and shrinking from record to record (by 2^40 in all; inside a
+    record a value of less than 2^-13 of the largest has fewer than 11 bits), 60 rows."""
+    rng = np.random.default_rng(13)
+    s = Setup(rng, 2, 128, 8, 64, 150, [100, 40, 1], k_size=size)
+    for by in (np.zeros(291), np.linspace(-20, 20, 291), np.linspace(20, -20, 291)):
+        s.v = (rng.standard_normal(s.v.shape) * (size if size < 1e30 else 1e30) * 2.0**by[:, None, None]).astype(np.float32)
+        s.write(np.arange(291))
+        q, out = run(s, rng, 20 * 2, [250, 190, 151], dtype=dtype, scale=128**-0.5 / size)
+        if size > 2.0**103:  # the cache refuses such keys: they are NaN
+            assert bool(torch.isnan(out).all())
+            continue
+        check(s, q, out, [250, 190, 151], 1, 0, dtype, scale=128**-0.5 / size, norm=not by.any())
 
 
 def test_sharp_and_flat_weights():

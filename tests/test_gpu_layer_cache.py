@@ -114,15 +114,15 @@ def test_values_at_the_ends_of_the_type(bits):
     rng = np.random.default_rng(4)
     x[0, 1] = -3.75
     x[0, 2] = rng.standard_normal(64) * 1e-40
-    x[0, 3] = rng.uniform(-8.5e37, 8.5e37, 64)  # 2^126 is the first that is refused
-    x[0, 3, 0, :2] = np.nextafter(np.float32(2.0**126), np.float32(0)), -np.nextafter(np.float32(2.0**126), np.float32(0))
+    x[0, 3] = rng.uniform(-1e31, 1e31, 64)  # 2^103 is the first that is refused
+    x[0, 3, 0, :2] = np.nextafter(np.float32(2.0**103), np.float32(0)), -np.nextafter(np.float32(2.0**103), np.float32(0))
     x[0, 4] = rng.standard_normal(64)
     x[0, 4, 0, 9] = np.nan
     x[0, 5] = rng.standard_normal(64)
     x[0, 5, 0, 63] = -np.inf
     x[0, 6] = 1000.0 + rng.uniform(0, 1e-3, 64)
     x[0, 7] = rng.standard_normal(64)
-    x[0, 8, 0, 1] = 2.0**126
+    x[0, 8, 0, 1] = 2.0**103
     cache = T.KvCache(1, 32, 1, 64, bits=bits)
     t, sl = tensor(x[0], "f32"), ids(np.arange(9))
     cache.write(t, t, sl, 9)

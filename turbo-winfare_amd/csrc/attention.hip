@@ -35,11 +35,18 @@ constexpr uint32_t kWaves = 4;
 constexpr uint32_t kXcds = 8;
 constexpr float kNegInf = -__builtin_inff();
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 union Frag {
     half8 h;
+    bf16x8 b;
     uint32_t u[4];
 };
 
+__device__ inline uint32_t out_bits(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x40u;
+    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
 // v over the lanes that hold the same row (lane, lane ^ 16, lane ^ 32, lane ^ 48)
 template <class Op>
 __device__ inline float rows_reduce(float v, Op op) {
@@ -180,29 +187,27 @@ __device__ inline void load_q8(const void* q, uint64_t at, float (&x)[8]) {
     }
 }
 
-__device__ inline uint32_t out_bits(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
-}
 template <bool F32>
 __device__ inline void store_out(void* out, uint64_t at, float4 v) {
     if constexpr (F32) *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(out_bits(v.x) | out_bits(v.y) << 16, out_bits(v.z) | out_bits(v.w) << 16);
 }
 
-template <int NG, int MT>
+template <int NG, bool F32, int MT>
 struct Shared {
     static constexpr uint32_t kRow = 68;  // floats of a row of 64, padded
     union {
-        uint32_t scales[kWaves][2 * NG * kKvBlock];
+        struct {
+            uint4 q[MT][NG][F32 ? 4 : 2][64];  // the queries as second operands: [.., chunk of 32 (and low parts)][lane]
+            uint32_t scales[kWaves][2 * NG * kKvBlock];
+        };
         float sums[kWaves][16 * MT][kRow];
     };
     float m[kWaves][16 * MT], l[kWaves][16 * MT];
 };
 
 template <int NG, uint32_t BITS, bool F32, int MT>
-__device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>& sh) {
+__device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32, MT>& sh) {
     constexpr int KU = BITS == 8u ? 2 : 1;       // 16-byte loads per group of keys or values
     constexpr int kUnit = F32 ? 0 : 24;          // codes are in units of 2^-kUnit
     constexpr uint32_t D = NG * 64u, PART = NG * 64u * kKvBlock * BITS / 8u, RECORD = 2u * PART + 2u * NG * kKvBlock * 4u;
@@ -234,44 +239,69 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
         s0 = min(b1, b0 + (int)it.split * per), s1 = min(b1, s0 + per);
     }
 
-    // ---- the queries, fp16 after a power of two that takes the row's largest to 2^14 .. 2^15
-    Frag qh[MT][NG][2], ql[F32 ? MT : 1][F32 ? NG : 1][2];
-    float qsum[MT][NG], factor[MT];
+    // ---- the queries, fp16 after a power of two that takes the row's largest to 2^14 .. 2^15, in LDS for
+    // all four waves; a negative scale is theirs, so that larger scores are larger weights
+    float factor[MT], qsum[F32 ? MT : 1][F32 ? NG : 1];
+    Frag qbias[MT];  // the groups' sums of q in three BF16 parts, part major, as the second operand against biases
+    const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        float x[NG][2][8], top = 0.0f;
+        const uint64_t at = row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + g * 16u;
+        float top = 0.0f;
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                load_q8<F32>(a.q, row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + n * 64u + g * 16u + c * 8u, x[n][c]);
+                float x[8];
+                load_q8<F32>(a.q, at + n * 64u + c * 8u, x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][c][i]));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
             }
         top = rows_max(top);
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        factor[mt] = ldexpf(a.scale_log2e, kUnit - shift);
+        factor[mt] = sign == 0.0f ? 1.0f : ldexpf(fabsf(a.scale_log2e), kUnit - shift);
+        qbias[mt].u[0] = qbias[mt].u[1] = qbias[mt].u[2] = qbias[mt].u[3] = 0u;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float v[8];
+                load_q8<F32>(a.q, at + n * 64u + c * 8u, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ldexpf(x[n][c][i], shift), sum += v[i];
+                for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], shift) * sign, sum += v[i];
+                Frag h, low;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = BITS == 8u ? 2 * i : i, k = j + (BITS == 8u ? 1 : 4);
-                    qh[mt][n][c].u[i] = pack_fp16(v[j], v[k]);
+                    h.u[i] = pack_fp16(v[j], v[k]);
                     if constexpr (F32) {
-                        const Pair h = unpack_fp16(qh[mt][n][c].u[i]);
-                        ql[mt][n][c].u[i] = pack_fp16(v[j] - h.lo, v[k] - h.hi);
+                        const Pair u = unpack_fp16(h.u[i]);
+                        low.u[i] = pack_fp16(v[j] - u.lo, v[k] - u.hi);
                     }
                 }
+                if ((n & 3) == (int)wave) {
+                    sh.q[mt][n][c][lane] = make_uint4(h.u[0], h.u[1], h.u[2], h.u[3]);
+                    if constexpr (F32) sh.q[mt][n][2 + c][lane] = make_uint4(low.u[0], low.u[1], low.u[2], low.u[3]);
+                }
             }
-            qsum[mt][n] = rows_sum(sum) * (F32 ? 1.0f : 0x1p-24f);
+            sum = rows_sum(sum);
+            if constexpr (F32) {
+                qsum[mt][n] = sum;
+            } else {
+                float rest = sum * 0x1p-24f;
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    const uint32_t w = out_bits(rest);  // BF16
+                    rest -= __uint_as_float(w << 16);
+                    const int slot = part * NG + n;
+                    if (g == (uint32_t)slot / 8u) qbias[mt].u[(slot % 8) / 2] |= w << (16 * (slot % 2));
+                }
+            }
         }
     }
+    // no wave reads the queries before all have written their part
+    __syncthreads();
 
     float4v o[MT][NG * 4];
     float obias[MT][NG], m[MT], l[MT];
@@ -293,6 +323,12 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
     };
     auto record_at = [&](int blk, uint32_t page) {
         return a.kv.base + kv_record_at(a.kv, page < a.kv.pages ? page : 0u, it.head, (uint32_t)blk & page_mask);
+    };
+    auto query = [&](int mt, int n, int c) {
+        Frag f;
+        const uint4 v = sh.q[mt][n][c][lane];
+        f.u[0] = v.x, f.u[1] = v.y, f.u[2] = v.z, f.u[3] = v.w;
+        return f;
     };
     uint4 kc[NG * KU];
     uint32_t sw[NG];
@@ -361,10 +397,26 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
         float s[MT][8];
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
+            if constexpr (F32) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[mt][tile * 4 + i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) s[mt][tile * 4 + i] = 0.0f;
+            } else {
+                // sum_n b_n sum(q_n): the biases are BF16 as they are; depth 8 g + i holds group i % NG
+                uint32_t w[NG];
+#pragma unroll
+                for (int n = 0; n < NG; ++n) w[n] = scales[n * kKvBlock + tile * 16u + (lane & 15u)];
+                Frag b;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b.u[i] = __builtin_amdgcn_perm(w[(2 * i + 1) % NG], w[(2 * i) % NG], 0x05040100u);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const float4v acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.b, qbias[mt].b, float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][tile * 4 + i] = acc[i];
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
                 const uint4 w4 = *reinterpret_cast<const uint4*>(scales + n * kKvBlock + tile * 16u + g * 4u);
@@ -380,16 +432,16 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, qh[mt][n][0].h, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, qh[mt][n][1].h, acc, 0, 0, 0);
-                    if constexpr (F32) {
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, ql[mt][n][0].h, acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, ql[mt][n][1].h, acc, 0, 0, 0);
+#pragma unroll
+                    for (int part = 0; part < (F32 ? 4 : 2); part += 2) {
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, query(mt, n, part).h, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, query(mt, n, part + 1).h, acc, 0, 0, 0);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float scale = scale_of<BITS, F32>(w[i]), bias = bias_of<BITS, F32>(w[i]);
-                        s[mt][tile * 4 + i] = fmaf(scale, acc[i], fmaf(bias, qsum[mt][n], s[mt][tile * 4 + i]));
+                        float& to = s[mt][tile * 4 + i];
+                        to = fmaf(scale_of<BITS, F32>(w[i]), acc[i], to);
+                        if constexpr (F32) to = fmaf(bias_of<BITS, F32>(w[i]), qsum[mt][n], to);
                     }
                 }
             }
@@ -409,11 +461,10 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
             float top = kNegInf;
             seen[mt] = 0xFFu;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                s[mt][j] *= factor[mt];
+            for (int j = 0; j < 8; ++j)
                 if (bad) s[mt][j] = __builtin_nanf("");
-            }
             if (masked) {
+                asm volatile("");  // a branch, not selects: few records are masked
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = base + (j >> 2) * 16 + (int)g * 4 + (j & 3);
@@ -422,7 +473,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, s[mt][j]);
-            top = fmaxf(m[mt], rows_max(top));
+            top = fmaxf(m[mt], rows_max(top) * factor[mt]);
             const float zero = top == kNegInf ? 0.0f : top;
             if (__any(top > m[mt])) {
                 const float alpha = __builtin_amdgcn_exp2f(m[mt] - zero);
@@ -435,7 +486,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[mt][j] = __builtin_amdgcn_exp2f(s[mt][j] - zero);
+                p[mt][j] = __builtin_amdgcn_exp2f(fmaf(s[mt][j], factor[mt], -zero));
                 l[mt] += p[mt][j];
             }
         }
@@ -446,15 +497,20 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
         for (int n = 0; n < NG; ++n) {
             const uint4 wa = *reinterpret_cast<const uint4*>(scales + (NG + n) * kKvBlock + g * 4u);
             const uint4 wb = *reinterpret_cast<const uint4*>(scales + (NG + n) * kKvBlock + 16u + g * 4u);
-            const uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
             Frag ph[MT], pl[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
+                uint32_t w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+                if (masked) {
+                    asm volatile("");
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (!((seen[mt] >> j) & 1u)) w[j] = 0u;  // what the slot holds may be anything, NaN too
+                }
                 float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float scale = scale_of<BITS, F32>(w[j]), bias = bias_of<BITS, F32>(w[j]);
-                    if (masked && !((seen[mt] >> j) & 1u)) scale = 0.0f, bias = 0.0f;  // what it holds may be anything
+                    const float scale = scale_of<BITS, F32>(w[j]), bias = bias_of<BITS, F32>(w[j]);
                     v[j] = p[mt][j] * unit * scale;
                     obias[mt][n] = fmaf(p[mt][j], bias, obias[mt][n]);
                 }
@@ -562,6 +618,374 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, MT>&
     }
 }
 
+// ---- many rows ------------------------------------------------------------------------------------
+// A tile of 64 MT rows of BF16 queries, 16 MT to a wave. The workgroup widens each record once, to fp16
+// values in LDS (key and value = (code - middle) * s' + b', one packed fused multiply-add per two codes, s'
+// and b' brought to the record's size by a power of two, so a value is rounded to 11 bits or to 2^-25 of
+// the record's largest), and every wave takes them from there as operands: the per-key scales, 144
+// instructions per 16 rows and record above, are paid once per workgroup. While a record is multiplied,
+// the next one is widened into the other half of LDS and the one after it is on its way to registers.
+template <int NG>
+struct Wide {
+    uint4 k[2][NG][2][2][64];   // [half][group][tile of 16 keys][chunk of 32 values][lane]
+    uint4 v[2][NG][4][64];      // [half][group][tile of 16 values][lane]
+    int range[kWaves][2];
+};
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+union Half2 {
+    uint32_t u;
+    half2v h;
+};
+__device__ inline uint32_t fma_fp16(uint32_t x, uint32_t s, uint32_t b) {
+    Half2 p, q, r;
+    p.u = x, q.u = s, r.u = b;
+    p.h = p.h * q.h + r.h;
+    return p.u;
+}
+
+template <int NG, uint32_t BITS, int MT>
+__device__ inline void attend_many(const AttnArgs& a, const Item& it, Wide<NG>& sh) {
+    constexpr int KU = BITS == 8u ? 2 : 1, UNITS = NG * KU, PER = (UNITS + 3) / 4;  // 16-byte loads of a wave, of keys and of values
+    constexpr uint32_t D = NG * 64u, PART = NG * 64u * kKvBlock * BITS / 8u;
+    constexpr float kMiddle = BITS == 8u ? 128.0f : 8.0f;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    Row row[MT];
+    bool live[MT];
+    int lo_min = 0x7FFFFFFF, lo_max = 0, hi_min = 0x7FFFFFFF, hi_max = 0;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        row[mt] = row_of(a, it, it.row0 + (wave * MT + mt) * 16u + (lane & 15u));
+        live[mt] = row[mt].exists && row[mt].lo < row[mt].hi;
+        if (live[mt]) {
+            lo_min = min(lo_min, row[mt].lo), lo_max = max(lo_max, row[mt].lo);
+            hi_min = min(hi_min, row[mt].hi), hi_max = max(hi_max, row[mt].hi);
+        } else {
+            row[mt].lo = 0, row[mt].hi = 0x7FFFFFFF;
+        }
+    }
+    auto least = [](int x, int y) { return min(x, y); };
+    auto most = [](int x, int y) { return max(x, y); };
+    lo_min = wave_reduce(lo_min, least), lo_max = wave_reduce(lo_max, most);
+    hi_min = wave_reduce(hi_min, least), hi_max = wave_reduce(hi_max, most);
+    if (lane == 0u) sh.range[wave][0] = lo_min, sh.range[wave][1] = hi_max;
+    __syncthreads();
+    int all_lo = 0x7FFFFFFF, all_hi = 0;  // keys that some row of the tile sees
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) all_lo = min(all_lo, sh.range[w][0]), all_hi = max(all_hi, sh.range[w][1]);
+    int s0 = 0, s1 = 0;
+    if (all_hi > 0) {
+        const int b0 = all_lo / (int)kKvBlock, b1 = (all_hi + (int)kKvBlock - 1) / (int)kKvBlock;
+        const int per = (b1 - b0 + (int)it.splits - 1) / (int)it.splits;
+        s0 = min(b1, b0 + (int)it.split * per), s1 = min(b1, s0 + per);
+    }
+
+    float factor[MT];
+    Frag q[MT][NG][2];
+    const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const uint64_t at = row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + g * 16u;
+        float top = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x[8];
+                load_q8<false>(a.q, at + n * 64u + c * 8u, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+            }
+        top = rows_max(top);
+        const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+        factor[mt] = sign == 0.0f ? 1.0f : ldexpf(fabsf(a.scale_log2e), -shift);
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float v[8];
+                load_q8<false>(a.q, at + n * 64u + c * 8u, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], shift) * sign;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = BITS == 8u ? 2 * i : i, k = j + (BITS == 8u ? 1 : 4);
+                    q[mt][n][c].u[i] = pack_fp16(v[j], v[k]);
+                }
+            }
+    }
+    float4v o[MT][NG * 4];
+    float m[MT], l[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        m[mt] = kNegInf, l[mt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG * 4; ++i) o[mt][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // ---- a record on its way: registers, then LDS
+    const uint32_t page_mask = (1u << a.kv.page_shift) / kKvBlock - 1u, block_shift = a.kv.page_shift - 5u;
+    auto page_at = [&](int blk) {
+        const uint32_t i = (uint32_t)blk >> block_shift;
+        return i < it.table ? it.pages[i] : 0xFFFFFFFFu;
+    };
+    auto record_at = [&](int blk, uint32_t page) {
+        return a.kv.base + kv_record_at(a.kv, page < a.kv.pages ? page : 0u, it.head, (uint32_t)blk & page_mask);
+    };
+    uint4 kr[PER], vr[PER];
+    uint32_t kw[PER * (BITS == 8u ? 1 : 2)], all[NG];
+    constexpr int VG = BITS == 8u ? (PER + 1) / 2 : PER;  // groups that a wave's value units belong to
+    uint4 vw[VG][2];
+    const uint32_t first = wave * PER;
+    auto load = [&](const uint8_t* rec) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(rec + 2u * PART);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) all[i] = words[lane * NG + i];
+        if (first < UNITS) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint32_t u = first + i;
+                kr[i] = *reinterpret_cast<const uint4*>(rec + u * 1024u + lane * 16u);
+                vr[i] = *reinterpret_cast<const uint4*>(rec + PART + u * 1024u + lane * 16u);
+                if constexpr (BITS == 8u) {
+                    kw[i] = words[(u >> 1) * kKvBlock + (u & 1u) * 16u + (lane & 15u)];
+                } else {
+                    kw[2 * i] = words[u * kKvBlock + (lane & 15u)];
+                    kw[2 * i + 1] = words[u * kKvBlock + 16u + (lane & 15u)];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VG; ++i) {
+                const uint32_t n = BITS == 8u ? (first + 2 * i) >> 1 : first + i;
+                vw[i][0] = *reinterpret_cast<const uint4*>(words + (NG + n) * kKvBlock + g * 4u);
+                vw[i][1] = *reinterpret_cast<const uint4*>(words + (NG + n) * kKvBlock + 16u + g * 4u);
+            }
+        }
+    };
+    // The powers of two of a record's keys and values: below 2^(e + 15) with a scale's largest code and its
+    // bias. Words of keys that no row sees are left out, and NaN. The values' is the largest so far.
+    int kexp = 0, vexp = -1000;
+    bool vnan = false;
+    auto sizes = [&](int base) {
+        uint32_t top = 0u;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int key = base + (int)((lane * NG + i) & 31u);
+            const bool in = key >= all_lo && key < all_hi;
+            const uint32_t s = all[i] >> 23, b = (all[i] >> 7) & 0xFFu;
+            if (in && s < 255u) top = max(top, max(s + BITS, b));
+            nan |= in && s >= 255u;
+        }
+        const uint32_t kt = wave_max_u(lane < 32u ? top : 0u), vt = wave_max_u(lane < 32u ? 0u : top);
+        kexp = min(max((int)kt - 140, -120), 113);
+        vexp = max(vexp, min(max((int)vt - 140, -120), 113));
+        vnan = __ballot(nan && lane >= 32u) != 0ull;
+    };
+    // s' and b' of a word; outside the visible keys, and (values) where it is NaN, both 0
+    auto scaled = [&](uint32_t w, int key, float unit, bool values) {
+        const bool in = key >= all_lo && key < all_hi && !(values && w >= 0x7F800000u);
+        const float s = __uint_as_float(w & 0xFFFF0000u) * unit, b = __uint_as_float(w << 16) * unit;
+        return Pair{in ? s : 0.0f, in ? fmaf(kMiddle, s, b) : 0.0f};
+    };
+    auto widen = [&](int half, int base) {
+        if (first >= UNITS) return;
+        const float kunit = __uint_as_float((uint32_t)(127 - kexp) << 23), vunit = __uint_as_float((uint32_t)(127 - vexp) << 23);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t u = first + i;
+#pragma unroll
+            for (int t = 0; t < (BITS == 8u ? 1 : 2); ++t) {
+                const uint32_t n = BITS == 8u ? u >> 1 : u, tile = BITS == 8u ? u & 1u : (uint32_t)t;
+                const Pair p = scaled(kw[BITS == 8u ? i : 2 * i + t], base + (int)(tile * 16u + (lane & 15u)), kunit, false);
+                const uint32_t s = pack_fp16(p.lo, p.lo), b = pack_fp16(p.hi, p.hi);
+                Frag f[2];
+                if constexpr (BITS == 8u) f[0] = widen_bytes<true>(kr[i].x, kr[i].y), f[1] = widen_bytes<true>(kr[i].z, kr[i].w);
+                else f[0] = widen_nibbles<true>(t ? kr[i].z : kr[i].x), f[1] = widen_nibbles<true>(t ? kr[i].w : kr[i].y);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[c].u[e] = fma_fp16(f[c].u[e], s, b);
+                    sh.k[half][n][tile][c][lane] = make_uint4(f[c].u[0], f[c].u[1], f[c].u[2], f[c].u[3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VG; ++i) {
+            const uint32_t w[8] = {vw[i][0].x, vw[i][0].y, vw[i][0].z, vw[i][0].w, vw[i][1].x, vw[i][1].y, vw[i][1].z, vw[i][1].w};
+            uint32_t s[4], b[4];  // in the order of the codes
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int x = BITS == 8u ? 2 * e : (e & 2) * 2 + (e & 1), y = x + (BITS == 8u ? 1 : 2);
+                const Pair p = scaled(w[x], base + (x >> 2) * 16 + (int)g * 4 + (x & 3), vunit, true);
+                const Pair r = scaled(w[y], base + (y >> 2) * 16 + (int)g * 4 + (y & 3), vunit, true);
+                s[e] = pack_fp16(p.lo, r.lo), b[e] = pack_fp16(p.hi, r.hi);
+            }
+#pragma unroll
+            for (int j = 0; j < (BITS == 8u ? 2 : 1); ++j) {
+                const int iu = BITS == 8u ? 2 * i + j : i;
+                if (iu >= PER) break;
+                const uint32_t u = first + iu;
+                const uint4 c = vr[iu];
+#pragma unroll
+                for (int d = 0; d < (BITS == 8u ? 2 : 4); ++d) {
+                    Frag f;
+                    if constexpr (BITS == 8u) f = d ? widen_bytes<true>(c.z, c.w) : widen_bytes<true>(c.x, c.y);
+                    else f = (d & 2) ? widen_halves<true>(c.z, c.w, (d & 1) * 4u) : widen_halves<true>(c.x, c.y, (d & 1) * 4u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f.u[e] = fma_fp16(f.u[e], s[e], b[e]);
+                    const uint32_t n = BITS == 8u ? u >> 1 : u, tile = BITS == 8u ? (u & 1u) * 2u + d : (uint32_t)d;
+                    sh.v[half][n][tile][lane] = make_uint4(f.u[0], f.u[1], f.u[2], f.u[3]);
+                }
+            }
+        }
+    };
+    auto operand = [&](const uint4& v) {
+        Frag f;
+        f.u[0] = v.x, f.u[1] = v.y, f.u[2] = v.z, f.u[3] = v.w;
+        return f;
+    };
+
+    uint32_t page = 0xFFFFFFFFu, next_page = 0xFFFFFFFFu;
+    int ov = -1000;  // the power of two that the sums are in
+    if (s0 < s1) {
+        page = page_at(s0);
+        load(record_at(s0, page));
+        sizes(s0 * (int)kKvBlock);
+        widen(0, s0 * (int)kKvBlock);
+        if (s0 + 1 < s1) {
+            next_page = page_at(s0 + 1);
+            load(record_at(s0 + 1, next_page));
+        }
+    }
+    for (int blk = s0; blk < s1; ++blk) {
+        __syncthreads();  // this record is in LDS, and nobody reads the other half any more
+        const int half = (blk - s0) & 1, base = blk * (int)kKvBlock, kx = kexp, vx = vexp;
+        const bool bad = page >= a.kv.pages, values_nan = vnan;
+        page = next_page;
+        if (blk + 1 < s1) {
+            sizes(base + (int)kKvBlock);
+            widen(half ^ 1, base + (int)kKvBlock);
+            if (blk + 2 < s1) {
+                next_page = page_at(blk + 2);
+                load(record_at(blk + 2, next_page));
+            }
+        }
+        if (base >= hi_max || base + (int)kKvBlock <= lo_min) continue;  // none of this wave's rows sees it
+        if (vx > ov) {
+            if (ov > -1000) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < NG * 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[mt][i][e] = ldexpf(o[mt][i][e], ov - vx);
+            }
+            ov = vx;
+        }
+        float4v s[MT][2];
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][tile] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const Frag k = operand(sh.k[half][n][tile][c][lane]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) s[mt][tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.h, q[mt][n][c].h, s[mt][tile], 0, 0, 0);
+                }
+        }
+        const bool masked = base < lo_max || base + (int)kKvBlock > hi_min;
+        Frag p[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float f = ldexpf(factor[mt], kx);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = s[mt][j >> 2][j & 3];
+            if (bad || masked) {
+                asm volatile("");
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = base + (j >> 2) * 16 + (int)g * 4 + (j & 3);
+                    x[j] = key < row[mt].lo || key >= row[mt].hi ? kNegInf : bad ? __builtin_nanf("") : x[j];
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            // weights are up to 2^14: small ones stay normal numbers in fp16
+            top = fmaxf(m[mt], fmaf(rows_max(top), f, -14.0f));
+            const float zero = top == kNegInf ? 0.0f : top;
+            if (__any(top > m[mt])) {
+                const float alpha = __builtin_amdgcn_exp2f(m[mt] - zero);
+                l[mt] *= alpha;
+#pragma unroll
+                for (int i = 0; i < NG * 4; ++i) o[mt][i] *= alpha;
+                m[mt] = top;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], f, -zero));
+                l[mt] += x[j];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = BITS == 8u ? 2 * e : (e & 2) * 2 + (e & 1), j = i + (BITS == 8u ? 1 : 2);
+                p[mt].u[e] = pack_fp16(x[i], x[j]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const Frag v = operand(sh.v[half][n][d][lane]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][n * 4 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.h, p[mt].h, o[mt][n * 4 + d], 0, 0, 0);
+            }
+        if (values_nan) {  // rows that see a group of NaN: they were taken as 0
+            const uint32_t pg = page_at(blk);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(record_at(blk, pg) + 2u * PART);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {
+                    float hit = 0.0f;
+                    for (int j = 0; j < 8; ++j) {
+                        const int t = (j >> 2) * 16 + (int)g * 4 + (j & 3), key = base + t;
+                        if (key >= row[mt].lo && key < row[mt].hi && words[(NG + n) * kKvBlock + t] >= 0x7F800000u) hit = 1.0f;
+                    }
+                    if (rows_max(hit) != 0.0f)
+#pragma unroll
+                        for (int i = n * 4; i < n * 4 + 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[mt][i][e] = __builtin_nanf("");
+                }
+        }
+    }
+
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        float total = rows_sum(l[mt]);
+        if (!live[mt]) m[mt] = kNegInf, total = 0.0f;
+        if (row[mt].over) m[mt] = 0.0f, total = __builtin_nanf("");
+        if (!row[mt].exists) continue;
+        const uint64_t r = (uint64_t)row[mt].token * a.q_heads + row[mt].head;
+        const float by = a.parts > 1u ? 1.0f : total != 0.0f ? 1.0f / total : 0.0f;
+        if (a.parts > 1u && g == 0u) a.stats[r * a.parts + it.part] = make_float2(m[mt], total);
+#pragma unroll
+        for (int i = 0; i < NG * 4; ++i) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = total != 0.0f && live[mt] ? ldexpf(o[mt][i][e], ov) * by : total;
+            const float4 x = make_float4(v[0], v[1], v[2], v[3]);
+            if (a.parts > 1u) *reinterpret_cast<float4*>(a.sums + (r * a.parts + it.part) * D + i * 16u + g * 4u) = x;
+            else store_out<false>(a.out, row[mt].token * a.out_stride + (uint64_t)row[mt].head * D + i * 16u + g * 4u, x);
+        }
+    }
+}
+
 // Workgroups are dealt out to the eight dies in turn. Tiles that read the same keys are neighbours in
 // `index`; this takes neighbours to one die, whose L2 then holds the keys for all of them.
 __device__ inline uint32_t same_die(uint32_t id, uint32_t n) {
@@ -569,11 +993,29 @@ __device__ inline uint32_t same_die(uint32_t id, uint32_t n) {
     return die * per + min(die, rest) + id / kXcds;
 }
 
+// MTP and MTO: rows of a prefix's and an own tile, as the multiple of 16 that a wave holds; kMany and
+// more is attend_many, with MT = that - kMany.
+constexpr int kMany = 8;
+constexpr uint32_t tile_rows(int mt) { return mt > kMany ? 64u * (mt - kMany) : 16u * mt; }
+template <int NG, uint32_t BITS, bool F32, int MT>
+struct Body {
+    typedef Shared<NG, F32, MT> Lds;
+    static __device__ void run(const AttnArgs& a, const Item& it, Lds& sh) { attend<NG, BITS, F32, MT>(a, it, sh); }
+};
+template <int NG, uint32_t BITS, int MT>
+    requires(MT > kMany)
+struct Body<NG, BITS, false, MT> {
+    typedef Wide<NG> Lds;
+    static __device__ void run(const AttnArgs& a, const Item& it, Lds& sh) { attend_many<NG, BITS, MT - kMany>(a, it, sh); }
+};
+
 template <int NG, uint32_t BITS, bool F32, int MTP, int MTO>
-__global__ __launch_bounds__(kThreads) void k_attend(const AttnArgs a) {
+__global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const AttnArgs a) {
+    typedef Body<NG, BITS, F32, MTP> Prefix;
+    typedef Body<NG, BITS, F32, MTO> Own;
     __shared__ union {
-        Shared<NG, MTP> p;
-        Shared<NG, MTO> o;
+        typename Prefix::Lds p;
+        typename Own::Lds o;
     } sh;
     Item it;
     uint32_t id = blockIdx.x;
@@ -583,7 +1025,7 @@ __global__ __launch_bounds__(kThreads) void k_attend(const AttnArgs a) {
         const uint32_t tile = id % a.prefix_tiles, rest = id / a.prefix_tiles;
         it.split = rest % a.prefix_splits, it.splits = a.prefix_splits, it.part = it.split;
         it.head = rest / a.prefix_splits;
-        it.seq = 0u, it.row0 = tile * 16u * MTP, it.rows = a.batch * a.q_len * a.group;
+        it.seq = 0u, it.row0 = tile * tile_rows(MTP), it.rows = a.batch * a.q_len * a.group;
         it.pages = a.prefix_pages, it.table = (a.prefix_len + (1u << a.kv.page_shift) - 1u) >> a.kv.page_shift;
     } else {
         id -= a.prefix_items;
@@ -593,14 +1035,14 @@ __global__ __launch_bounds__(kThreads) void k_attend(const AttnArgs a) {
         it.split = rest % a.own_splits, it.splits = a.own_splits, it.part = a.prefix_splits + it.split;
         rest /= a.own_splits;
         it.head = rest % a.kv.heads, it.seq = rest / a.kv.heads;
-        it.row0 = tile * 16u * MTO, it.rows = a.q_len * a.group;
+        it.row0 = tile * tile_rows(MTO), it.rows = a.q_len * a.group;
         it.pages = a.pages + (uint64_t)it.seq * a.page_stride, it.table = a.page_stride;
     }
     if constexpr (MTP == MTO) {
-        attend<NG, BITS, F32, MTP>(a, it, sh.p);
+        Prefix::run(a, it, sh.p);
     } else {
-        if (it.prefix) attend<NG, BITS, F32, MTP>(a, it, sh.p);
-        else attend<NG, BITS, F32, MTO>(a, it, sh.o);
+        if (it.prefix) Prefix::run(a, it, sh.p);
+        else Own::run(a, it, sh.o);
     }
 }
 
@@ -627,20 +1069,42 @@ __global__ __launch_bounds__(kThreads) void k_join(const AttnArgs a, uint32_t he
     store_out<F32>(a.out, token * a.out_stride + (uint64_t)head * head_dim + col, make_float4(v.x * r1, v.y * r1, v.z * r1, v.w * r1));
 }
 
+// Rows of a tile: one row of 16 to a wave up to 16 rows, two (where registers hold them: head_dim up to 128)
+// up to kFewRows, the many-row body beyond.
+template <int NG, bool F32>
+struct Tiles {
+    static constexpr int kFew = NG <= 2 ? 2 : 1, kLarge = F32 ? kFew : kMany + (NG <= 2 ? 2 : 1);
+};
+constexpr uint32_t kFewRows = 32;
+
+template <int NG, uint32_t BITS, bool F32, int MTP, int MTO>
+void launch_tiles(const AttnArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attend<NG, BITS, F32, MTP, MTO>), dim3(a.items), dim3(kThreads), 0, st, a);
+}
+
 template <int NG, uint32_t BITS, bool F32>
 void launch_typed(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
-    const dim3 grid((uint32_t)plan.items), block(kThreads);
-    if constexpr (NG <= (F32 ? 2 : 4)) {
-        if (plan.prefix_tile_rows == 32u && plan.own_tile_rows == 32u) {
-            hipLaunchKernelGGL((k_attend<NG, BITS, F32, 2, 2>), grid, block, 0, st, a);
-            return;
-        }
-        if (plan.prefix_tile_rows == 32u) {
-            hipLaunchKernelGGL((k_attend<NG, BITS, F32, 2, 1>), grid, block, 0, st, a);
-            return;
+    typedef Tiles<NG, F32> X;
+    const uint32_t p = plan.prefix_tile_rows, o = plan.own_tile_rows;
+    if constexpr (!F32) {
+        if (o == tile_rows(X::kLarge)) return launch_tiles<NG, BITS, F32, X::kLarge, X::kLarge>(a, st);
+        if (p == tile_rows(X::kLarge)) {
+            if (X::kFew > 1 && o == tile_rows(X::kFew)) return launch_tiles<NG, BITS, F32, X::kLarge, X::kFew>(a, st);
+            return launch_tiles<NG, BITS, F32, X::kLarge, 1>(a, st);
         }
     }
-    hipLaunchKernelGGL((k_attend<NG, BITS, F32, 1, 1>), grid, block, 0, st, a);
+    if constexpr (X::kFew > 1) {
+        if (o == tile_rows(X::kFew)) return launch_tiles<NG, BITS, F32, X::kFew, X::kFew>(a, st);
+        if (p == tile_rows(X::kFew)) return launch_tiles<NG, BITS, F32, X::kFew, 1>(a, st);
+    }
+    launch_tiles<NG, BITS, F32, 1, 1>(a, st);
+}
+
+uint32_t tile_for(uint64_t rows, uint32_t head_dim, int dtype) {
+    if (rows <= 16u) return 16u;
+    const uint32_t few = head_dim <= 128u ? 32u : 16u;
+    if (rows <= kFewRows || dtype == TURBO_HIDDEN_F32) return few;
+    return head_dim <= 128u ? 128u : 64u;
 }
 
 template <bool F32>
@@ -663,10 +1127,8 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
     AttnPlan p{};
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
-    const bool can32 = head_dim <= (dtype == TURBO_HIDDEN_F32 ? 128u : 256u);
-    p.prefix_tile_rows = can32 && all_rows > 16u ? 32u : 16u;
-    p.own_tile_rows = can32 && own_rows > 16u ? 32u : 16u;
-    if (!prefix_len) p.prefix_tile_rows = p.own_tile_rows;
+    p.own_tile_rows = tile_for(own_rows, head_dim, dtype);
+    p.prefix_tile_rows = prefix_len ? std::max(tile_for(all_rows, head_dim, dtype), p.own_tile_rows) : p.own_tile_rows;
     auto records = [&](uint64_t keys, uint64_t spread) {
         if (window) keys = std::min<uint64_t>(keys, (uint64_t)window + spread);
         return (keys + kKvBlock - 1u) / kKvBlock;

@@ -102,7 +102,8 @@ __device__ inline float bf16_outward(float x, bool up) {
 }
 
 // The codes of a lane's E values and the group's word of scale and bias. N lanes share a group. A group
-// with a value of 2^126 or more, infinite or NaN is NaN: below that no difference or product overflows.
+// with a value of 2^103 or more, infinite or NaN is NaN: below that a score's sum over 512 products with
+// queries of 2^15 stays in FP32.
 template <int E, int N>
 __device__ inline uint32_t quantise(const float (&x)[E], uint32_t top, uint32_t (&code)[E]) {
     float lo = x[0], hi = x[0];
@@ -114,7 +115,7 @@ __device__ inline uint32_t quantise(const float (&x)[E], uint32_t top, uint32_t 
         mag = max(mag, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     }
     const uint32_t lane = threadIdx.x & 63u;
-    const unsigned long long odd = __ballot(mag >= 0x7E800000u) >> (lane & ~(uint32_t)(N - 1));
+    const unsigned long long odd = __ballot(mag >= 0x73000000u) >> (lane & ~(uint32_t)(N - 1));
     const bool finite = (odd & ((1ull << N) - 1ull)) == 0ull;
     lo = lanes_reduce<N>(lo, [](float a, float b) { return fminf(a, b); });
     hi = lanes_reduce<N>(hi, [](float a, float b) { return fmaxf(a, b); });
