@@ -444,9 +444,8 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * a negative position sees nothing and gives zeros (kv_len 0: a padded sequence). A query whose tokens
  * pass its page table, or lie on a page past the cache, gives NaN.
  * The prefix is read once for the whole batch: its products run over the rows of all sequences. Products
- * accumulate in FP32; FP32 queries keep 22 bits of queries and softmax weights, BF16 ones 11 bits of the
- * weights and, where more than 32 rows share keys, of keys and values (or 2^-25 of the largest of their
- * 32 tokens).
+ * accumulate in FP32; for FP32 queries, queries and softmax weights keep 22 bits; for BF16 ones weights,
+ * keys and values keep 11 (or 2^-24 of the largest of their 32 tokens, 2^-20 at 4 bits).
  */
 typedef struct {
     int batch;                   /* >= 0 */

@@ -7,9 +7,9 @@ is off by at most scale * sum |q| K * (2^-22 + 80 * 2^-24): FP32 queries keep 22
 groups add in FP32 (BF16 queries are exact, the same bound holds); the factor and the exponential add
 (2 |s| + 2) 2^-23 to a weight's relative error. A weight is rounded to 2^-22 (FP32) or 2^-12 (BF16) of
 itself for the product with the values, which adds at most 32 + keys / 32 roundings, and the join and
-division 8 more. Where more than 32 BF16 rows share keys, a key or value is rounded to fp16 twice (the
-middle code's value and the product's sum with it): 2^-11 K, or 2^-24 of the largest K of its 32 tokens.
-So |off| <= (2 e + w + (40 + keys / 32) 2^-24) sum p (|code * scale| + |bias|), and BF16 rounds
+division 8 more. For BF16 queries a key or value is rounded to fp16: 2^-12 K, or half of fp16's smallest
+step, which is 2^-24 of the largest K of its 32 tokens (4 bits: 2^-20; scale and bias as well, once more
+each). So |off| <= (2 e + w + (40 + keys / 32) 2^-24) sum p (|code * scale| + |bias|), and BF16 rounds
 the result by 2^-8 of it. Those are worst cases; the errors are independent, so the 2-norm must stay far
 below: under 4e-6 (FP32: 8 roundings' worth of a 64-term sum at the scores' size here) and 2.5e-3 (BF16:
 half a step is 2^-8 at most, 2^-9 / sqrt(3) * 1.4 on average over a binade)."""
@@ -93,6 +93,7 @@ def expect(s, q, b, q_len, kv_len, window, scale, dtype):
     q = q.astype(np.float64)
     g = q.shape[1] // s.heads
     out, bound = np.zeros_like(q), np.zeros_like(q)
+    least = 2.0**-24 if s.bits == 8 else 2.0**-20
     for i in range(q_len):
         p = kv_len - q_len + i
         lo, hi = (max(0, p - window + 1) if window else 0), p + 1
@@ -107,9 +108,9 @@ def expect(s, q, b, q_len, kv_len, window, scale, dtype):
             e = scale * (ka @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
             rel = (2.0**-22 if dtype == "f32" else 2.0**-12) + (40 + (hi - lo) / 32) * 2.0**-24
             if dtype == "bf16":
-                e = e + scale * (ka @ np.abs(q[i, h]) * 2.0**-11 + np.nanmax(ka) * np.abs(q[i, h]).sum() * 2.0**-24)
+                e = e + scale * (ka @ np.abs(q[i, h]) * 2.0**-11 + np.nanmax(ka) * np.abs(q[i, h]).sum() * least)
                 rel += 2.0**-11
-            bound[i, h] = (2 * e.max() + rel) * (w @ va) + (np.nanmax(va) * 2.0**-24 if dtype == "bf16" else 0.0)
+            bound[i, h] = (2 * e.max() + rel) * (w @ va) + (np.nanmax(va) * least if dtype == "bf16" else 0.0)
     if dtype == "bf16":
         bound += 2.0**-8 * (np.abs(out) + bound)
     return out, bound + 1e-37
