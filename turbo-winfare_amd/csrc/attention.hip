@@ -151,6 +151,9 @@ __device__ inline Pair unpack_fp16(uint32_t w) {
     return Pair{(float)x.h[0], (float)x.h[1]};
 }
 
+// n / d for n below 2^31, by the multiplier that divider() made of d
+__device__ inline uint32_t quotient(uint32_t n, Divider d) { return d.factor ? __umulhi(n, d.factor) >> d.shift : n; }
+
 struct Item {
     bool prefix;
     uint32_t head, row0, rows;     // key/value head, first row of the tile, rows of the segment
@@ -170,11 +173,10 @@ __device__ inline Row row_of(const AttnArgs& a, const Item& it, uint32_t r) {
     Row w;
     w.exists = r < it.rows;
     if (!w.exists) r = it.rows - 1u;
-    const uint32_t per = a.q_len * a.group;
-    const uint32_t b = it.prefix ? r / per : it.seq, in = it.prefix ? r % per : r;
-    const uint32_t t = in / a.group;
+    const uint32_t b = it.prefix ? quotient(r, a.by_rows) : it.seq, in = it.prefix ? r - b * (a.q_len * a.group) : r;
+    const uint32_t t = quotient(in, a.by_group);
     w.token = b * a.q_len + t;
-    w.head = it.head * a.group + in % a.group;
+    w.head = it.head * a.group + in - t * a.group;
     const long long pos = (long long)a.kv_len[b] - (long long)a.q_len + t;
     const long long room = (long long)a.prefix_len + ((long long)a.page_stride << a.kv.page_shift);
     w.over = pos >= room;
@@ -233,7 +235,8 @@ struct Shared {
         };
         float sums[kWaves][16 * MT][kRow];
     };
-    float m[kWaves][16 * MT], l[kWaves][16 * MT];
+    float m[kWaves][16 * MT], l[kWaves][16 * MT], factor[16 * MT];
+    float qsum[F32 ? 16 * MT : 1][NG + 1];  // of a row's groups, fp32 queries
 };
 
 template <int NG, uint32_t BITS, bool F32, int MT>
@@ -274,35 +277,35 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     }
 
     // ---- the queries, fp16 after a power of two that takes the row's largest to 2^14 .. 2^15, in LDS for
-    // all four waves; a negative scale is theirs, so that larger scores are larger weights
-    float factor[MT], qsum[F32 ? MT : 1][F32 ? NG : 1];
+    // all four waves, which divide the tiles among them and then a tile's groups; a negative scale is
+    // theirs, so that larger scores are larger weights
     const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+    constexpr int kSharers = (int)kWaves / MT;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
+        if (mt != (int)wave % MT) continue;
         const uint64_t at = row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + g * 16u;
-        float top = 0.0f;
+        float x[NG][2][8], top = 0.0f;
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float x[8];
-                load_q8<F32>(a.q, at + n * 64u + c * 8u, x);
+                load_q8<F32>(a.q, at + n * 64u + c * 8u, x[n][c]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][c][i]));
             }
         top = rows_max(top);
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        factor[mt] = sign == 0.0f ? 1.0f : ldexpf(fabsf(a.scale_log2e), -shift);
+        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = sign == 0.0f ? 1.0f : ldexpf(fabsf(a.scale_log2e), -shift);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            if (!F32 && (n & 3) != (int)wave) continue;
+            if (n % kSharers != (int)wave / MT) continue;
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float v[8];
-                load_q8<F32>(a.q, at + n * 64u + c * 8u, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ldexpf(v[i], shift) * sign, sum += v[i];
+                for (int i = 0; i < 8; ++i) v[i] = ldexpf(x[n][c][i], shift) * sign, sum += v[i];
                 Frag h, low;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -313,16 +316,24 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                         low.u[i] = pack_fp16(v[j] - u.lo, v[k] - u.hi);
                     }
                 }
-                if ((n & 3) == (int)wave) {
-                    sh.q[mt][n][c][lane] = make_uint4(h.u[0], h.u[1], h.u[2], h.u[3]);
-                    if constexpr (F32) sh.q[mt][n][2 + c][lane] = make_uint4(low.u[0], low.u[1], low.u[2], low.u[3]);
-                }
+                sh.q[mt][n][c][lane] = make_uint4(h.u[0], h.u[1], h.u[2], h.u[3]);
+                if constexpr (F32) sh.q[mt][n][2 + c][lane] = make_uint4(low.u[0], low.u[1], low.u[2], low.u[3]);
             }
-            if constexpr (F32) qsum[mt][n] = rows_sum(sum);
+            if constexpr (F32) {
+                sum = rows_sum(sum);
+                if (g == 0u) sh.qsum[mt * 16 + lane][n] = sum;
+            }
         }
     }
-    // no wave reads the queries before all have written their part
     __syncthreads();
+    float factor[MT], qsum[F32 ? MT : 1][F32 ? NG : 1];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        factor[mt] = sh.factor[mt * 16 + (lane & 15u)];
+        if constexpr (F32)
+#pragma unroll
+            for (int n = 0; n < NG; ++n) qsum[mt][n] = sh.qsum[mt * 16 + (lane & 15u)][n];
+    }
 
     float4v o[MT][NG * 4];
     float obias[F32 ? MT : 1][F32 ? NG : 1], m[MT], l[MT];
@@ -753,37 +764,65 @@ __global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const Attn
     }
 }
 
-// Joins the partial results of a row: its largest maximum, then the weighted sums. head_dim / 4 threads
-// to a row.
+// Joins the partial results of a row. kThreads / (head_dim / 4) groups of threads; a group takes four values
+// to a thread of every per_row-th part of a row, and the groups of a row add up through LDS: with few
+// rows the parts' loads run side by side.
 template <bool F32>
-__global__ __launch_bounds__(kThreads) void k_join(const AttnArgs a, uint32_t head_dim, uint32_t rows) {
-    const uint32_t per = head_dim / 4u, r = blockIdx.x * (kThreads / per) + threadIdx.x / per, col = (threadIdx.x % per) * 4u;
-    if (r >= rows) return;
-    const float2* st = a.stats + (uint64_t)r * a.parts;
+__global__ __launch_bounds__(kThreads) void k_join(const AttnArgs a, uint32_t head_dim, uint32_t rows, uint32_t per_row) {
+    __shared__ float4 sum[kThreads];
+    __shared__ float part_total[kThreads];
+    const uint32_t width = head_dim / 4u, group = threadIdx.x / width, col = (threadIdx.x % width) * 4u;
+    const uint32_t r = blockIdx.x * (kThreads / width / per_row) + group / per_row, first = group % per_row;
+    const bool exists = r < rows;
+    const float2* st = a.stats + (uint64_t)(exists ? r : 0u) * a.parts;
     float top = kNegInf;
+#pragma unroll 4
     for (uint32_t i = 0; i < a.parts; ++i) top = fmaxf(top, st[i].x);
     float total = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t i = 0; i < a.parts; ++i) {
-        if (st[i].y == 0.0f) continue;  // its sums were not written
-        const float w = __builtin_amdgcn_exp2f(st[i].x - top);
-        total += w * st[i].y;
-        const float4 x = *reinterpret_cast<const float4*>(a.sums + ((uint64_t)r * a.parts + i) * head_dim + col);
-        v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+    const float* from = a.sums + (uint64_t)(exists ? r : 0u) * a.parts * head_dim + col;
+#pragma unroll 4
+    for (uint32_t i = first; i < a.parts; i += per_row) {
+        const float2 s = st[i];
+        const bool there = s.y != 0.0f;  // otherwise its sums were not written
+        const float w = there ? __builtin_amdgcn_exp2f(s.x - top) : 0.0f;
+        const float4 x = *reinterpret_cast<const float4*>(from + (uint64_t)i * head_dim);
+        if (there) {
+            total += w * s.y;
+            v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+        }
     }
+    if (per_row > 1u) {
+        sum[threadIdx.x] = v;
+        part_total[threadIdx.x] = total;
+        __syncthreads();
+        if (first != 0u) return;
+        for (uint32_t i = 1; i < per_row; ++i) {
+            const float4 x = sum[threadIdx.x + i * width];
+            total += part_total[threadIdx.x + i * width];
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+    }
+    if (!exists) return;
     const float r1 = total != 0.0f ? 1.0f / total : 0.0f;
     const uint32_t token = r / a.q_heads, head = r % a.q_heads;
     store_out<F32>(a.out, token * a.out_stride + (uint64_t)head * head_dim + col, make_float4(v.x * r1, v.y * r1, v.z * r1, v.w * r1));
 }
 
-// 16-row tiles of a workgroup at most: what the registers of two waves per SIMD hold.
-constexpr int most_tiles(uint32_t head_dim, bool f32) {
-    return head_dim == 64u ? (f32 ? 2 : 4) : head_dim == 128u ? (f32 ? 2 : 4) : head_dim == 256u ? (f32 ? 1 : 2) : 1;
-}
-uint32_t tiles_for(uint64_t rows, uint32_t head_dim, bool f32) {
+// 16-row tiles of a workgroup at most: what the registers of two waves per SIMD hold. Four at a head_dim of
+// 128 or less spill a little and measured 25.2 -> 30.2 us (32 sequences behind 8,000 tokens), 124 -> 129 us
+// (a chunk of 512 tokens); one in place of two 120 -> 139 us (head_dim 256, 64 sequences behind 32,768).
+constexpr int most_tiles(uint32_t head_dim, bool f32) { return head_dim <= (f32 ? 128u : 256u) ? 2 : 1; }
+uint32_t tiles_for(uint64_t rows, uint32_t most) {
     uint32_t mt = 1u;
-    while (mt < (uint32_t)most_tiles(head_dim, f32) && rows > 16u * mt) mt *= 2u;
+    while (mt < most && rows > 16u * mt) mt *= 2u;
     return mt;
+}
+Divider divider(uint32_t d) {  // ceil(2^(31 + L) / d) with 2^(L - 1) < d <= 2^L: exact for dividends below 2^31
+    uint32_t bits = 0u;
+    while (bits < 31u && (1u << bits) < d) ++bits;
+    if (bits == 0u) return Divider{0u, 0u};
+    return Divider{(uint32_t)(((1ull << (31u + bits)) + d - 1u) / d), bits - 1u};
 }
 
 template <int NG, uint32_t BITS, bool F32, int MTP, int MTO>
@@ -794,8 +833,6 @@ void launch_tiles(const AttnArgs& a, hipStream_t st) {
 template <int NG, uint32_t BITS, bool F32, int MTP>
 void launch_own(const AttnArgs& a, uint32_t mto, hipStream_t st) {
     if (mto == MTP) return launch_tiles<NG, BITS, F32, MTP, MTP>(a, st);
-    if constexpr (MTP == 4)
-        if (mto == 2u) return launch_tiles<NG, BITS, F32, 4, 2>(a, st);
     if constexpr (MTP > 1) launch_tiles<NG, BITS, F32, MTP, 1>(a, st);
 }
 
@@ -803,8 +840,6 @@ template <int NG, uint32_t BITS, bool F32>
 void launch_typed(const AttnArgs& a, const AttnPlan& plan, hipStream_t st) {
     constexpr int most = most_tiles(NG * 64u, F32);
     const uint32_t p = plan.prefix_tile_rows / 16u, o = plan.own_tile_rows / 16u;
-    if constexpr (most >= 4)
-        if (p == 4u) return launch_own<NG, BITS, F32, 4>(a, o, st);
     if constexpr (most >= 2)
         if (p == 2u) return launch_own<NG, BITS, F32, 2>(a, o, st);
     launch_own<NG, BITS, F32, 1>(a, o, st);
@@ -823,32 +858,34 @@ void launch_dtype(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, hi
 
 }  // namespace
 
-// Rows of 32 to a workgroup halve the widening of codes per row where registers hold them (head_dim up to
-// 256, FP32 up to 128). Keys are split until about two workgroups per compute unit have work, but not
-// below 8 records (two to a wave): then a workgroup's start and end weigh more than its keys.
+// More rows to a workgroup share the widening of codes, but a short call needs the workgroups: the tile is
+// the largest that leaves three workgroups to two compute units. Keys are split until they do, but
+// not below 8 records (two to a wave), where a workgroup's start and end weigh more than its keys.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
-    AttnPlan p{};
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
-    const bool f32 = dtype == TURBO_HIDDEN_F32;
-    p.own_tile_rows = 16u * tiles_for(own_rows, head_dim, f32);
-    p.prefix_tile_rows = prefix_len ? 16u * tiles_for(all_rows, head_dim, f32) : p.own_tile_rows;
     auto records = [&](uint64_t keys, uint64_t spread) {
         if (window) keys = std::min<uint64_t>(keys, (uint64_t)window + spread);
         return (keys + kKvBlock - 1u) / kKvBlock;
     };
     const uint64_t pr = prefix_len ? records(prefix_len, prefix_len / 4u) : 0u, orr = own_most ? records(own_most, q_len) : 0u;
-    const uint64_t pt = prefix_len ? (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows : 0u;
-    const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
-    const uint64_t work = kv_heads * (pt * pr + batch * ot * orr);
-    const uint64_t per = std::max<uint64_t>(8u, (work + 2u * cus - 1u) / (2u * cus));
-    p.prefix_tiles = (uint32_t)pt;
-    p.prefix_splits = prefix_len ? (uint32_t)((pr + per - 1u) / per) : 0u;
-    p.own_tiles = (uint32_t)ot;
-    p.own_splits = own_most ? (uint32_t)((orr + per - 1u) / per) : 0u;
-    if (!prefix_len && !own_most) p.own_splits = 1u;  // still writes zeros, or NaN past the tables
-    p.prefix_items = kv_heads * pt * p.prefix_splits;
-    p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
+    AttnPlan p{};
+    for (uint32_t most = most_tiles(head_dim, dtype == TURBO_HIDDEN_F32);; most /= 2u) {
+        p.own_tile_rows = 16u * tiles_for(own_rows, most);
+        p.prefix_tile_rows = prefix_len ? 16u * tiles_for(all_rows, most) : p.own_tile_rows;
+        const uint64_t pt = prefix_len ? (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows : 0u;
+        const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
+        const uint64_t work = kv_heads * (pt * pr + batch * ot * orr);
+        const uint64_t per = std::max<uint64_t>(8u, (work + 2u * cus - 1u) / (2u * cus));
+        p.prefix_tiles = (uint32_t)pt;
+        p.prefix_splits = prefix_len ? (uint32_t)((pr + per - 1u) / per) : 0u;
+        p.own_tiles = (uint32_t)ot;
+        p.own_splits = own_most ? (uint32_t)((orr + per - 1u) / per) : 0u;
+        if (!prefix_len && !own_most) p.own_splits = 1u;  // still writes zeros, or NaN past the tables
+        p.prefix_items = kv_heads * pt * p.prefix_splits;
+        p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
+        if (most == 1u || 2u * p.items >= 3u * cus) break;
+    }
     p.parts = p.prefix_splits + p.own_splits;
     p.rows = (uint64_t)batch * q_len * q_heads;
     if (p.parts > 1u) {
@@ -863,14 +900,18 @@ void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int 
     a.own_tiles = plan.own_tiles, a.own_splits = plan.own_splits;
     a.prefix_items = (uint32_t)plan.prefix_items, a.items = (uint32_t)plan.items;
     a.parts = plan.parts;
+    a.by_rows = divider(a.q_len * a.group), a.by_group = divider(a.group);
     if (dtype == TURBO_HIDDEN_F32) launch_dtype<true>(a, plan, head_dim, st);
     else launch_dtype<false>(a, plan, head_dim, st);
     check_hip(hipGetLastError(), "attention");
     if (plan.parts > 1u) {
-        const uint32_t per_group = kThreads / (head_dim / 4u), rows = (uint32_t)plan.rows;
-        const dim3 grid((rows + per_group - 1u) / per_group), block(kThreads);
-        if (dtype == TURBO_HIDDEN_F32) hipLaunchKernelGGL((k_join<true>), grid, block, 0, st, a, head_dim, rows);
-        else hipLaunchKernelGGL((k_join<false>), grid, block, 0, st, a, head_dim, rows);
+        const uint32_t groups = kThreads / (head_dim / 4u), rows = (uint32_t)plan.rows;
+        uint32_t per_row = 1u;  // more groups to a row while there are parts for them and the card has room
+        while (per_row < groups && per_row * 2u <= plan.parts && (uint64_t)rows * per_row < 4096u) per_row *= 2u;
+        const uint32_t per_block = groups / per_row;
+        const dim3 grid((rows + per_block - 1u) / per_block), block(kThreads);
+        if (dtype == TURBO_HIDDEN_F32) hipLaunchKernelGGL((k_join<true>), grid, block, 0, st, a, head_dim, rows, per_row);
+        else hipLaunchKernelGGL((k_join<false>), grid, block, 0, st, a, head_dim, rows, per_row);
         check_hip(hipGetLastError(), "attention");
     }
 }

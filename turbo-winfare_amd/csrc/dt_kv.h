@@ -88,6 +88,9 @@ struct KvReadArgs {
 void launch_kv_read(const KvReadArgs& a, uint32_t head_dim, int dtype, hipStream_t st);
 
 // attention.hip
+struct Divider {
+    uint32_t factor, shift;  // factor 0: by one
+};
 struct AttnArgs {
     KvView kv;
     const void* q;
@@ -104,12 +107,13 @@ struct AttnArgs {
     uint32_t prefix_tiles, prefix_splits;    // row tiles and key splits of the prefix, per key/value head
     uint32_t own_tiles, own_splits;          // of one sequence's own keys
     uint32_t prefix_items, items;            // workgroups
+    Divider by_rows, by_group;               // by q_len * group, by group
     uint32_t parts;                          // partial results per row (1: written to out directly)
     float2* stats;                           // [rows][parts] (running maximum, sum)
     float* sums;                             // [rows][parts][head_dim]
 };
 struct AttnPlan {
-    uint32_t prefix_tile_rows, own_tile_rows;  // 16 or 32 rows to a workgroup
+    uint32_t prefix_tile_rows, own_tile_rows;  // rows to a workgroup: 16 or 32
     uint32_t prefix_tiles, prefix_splits, own_tiles, own_splits;
     uint64_t prefix_items, items, rows;
     uint32_t parts;
