@@ -36,6 +36,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kXcds = 8;
+constexpr uint32_t kJoinStats = 1024;
 constexpr float kNegInf = -__builtin_inff();
 
 union Frag {
@@ -771,27 +772,44 @@ template <bool F32>
 __global__ __launch_bounds__(kThreads) void k_join(const AttnArgs a, uint32_t head_dim, uint32_t rows, uint32_t per_row) {
     __shared__ float4 sum[kThreads];
     __shared__ float part_total[kThreads];
+    __shared__ float2 stats[kJoinStats];
     const uint32_t width = head_dim / 4u, group = threadIdx.x / width, col = (threadIdx.x % width) * 4u;
-    const uint32_t r = blockIdx.x * (kThreads / width / per_row) + group / per_row, first = group % per_row;
+    const uint32_t per_block = kThreads / width / per_row, r0 = blockIdx.x * per_block;
+    const uint32_t r = r0 + group / per_row, first = group % per_row;
     const bool exists = r < rows;
-    const float2* st = a.stats + (uint64_t)(exists ? r : 0u) * a.parts;
+    // the rows' statistics through LDS where they fit: one load each, side by side
+    const bool held = per_block * a.parts <= kJoinStats;
+    const float2* st = a.stats + (uint64_t)(exists ? r : r0) * a.parts;
+    if (held) {
+        const uint32_t n = min(per_block, rows - r0) * a.parts;
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) stats[i] = a.stats[(uint64_t)r0 * a.parts + i];
+        __syncthreads();
+    }
+    const float2* mine = stats + (exists ? r - r0 : 0u) * a.parts;
+    auto stat = [&](uint32_t i) { return held ? mine[i] : st[i]; };
     float top = kNegInf;
-#pragma unroll 4
-    for (uint32_t i = 0; i < a.parts; ++i) top = fmaxf(top, st[i].x);
+#pragma unroll 8
+    for (uint32_t i = 0; i < a.parts; ++i) top = fmaxf(top, stat(i).x);
     float total = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float* from = a.sums + (uint64_t)(exists ? r : 0u) * a.parts * head_dim + col;
-#pragma unroll 4
-    for (uint32_t i = first; i < a.parts; i += per_row) {
-        const float2 s = st[i];
-        const bool there = s.y != 0.0f;  // otherwise its sums were not written
-        const float w = there ? __builtin_amdgcn_exp2f(s.x - top) : 0.0f;
-        const float4 x = *reinterpret_cast<const float4*>(from + (uint64_t)i * head_dim);
-        if (there) {
-            total += w * s.y;
-            v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
-        }
+    const float* from = a.sums + (uint64_t)(exists ? r : r0) * a.parts * head_dim + col;
+    auto take = [&](uint32_t i, float4 x) {
+        const float2 s = stat(i);
+        if (s.y == 0.0f) return;  // its sums were not written
+        const float w = __builtin_amdgcn_exp2f(s.x - top);
+        total += w * s.y;
+        v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+    };
+    auto load = [&](uint32_t i) { return *reinterpret_cast<const float4*>(from + (uint64_t)i * head_dim); };
+    uint32_t i = first;
+    for (; i + 7u * per_row < a.parts; i += 8u * per_row) {
+        float4 x[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) x[j] = load(i + j * per_row);
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) take(i + j * per_row, x[j]);
     }
+    for (; i < a.parts; i += per_row) take(i, load(i));
     if (per_row > 1u) {
         sum[threadIdx.x] = v;
         part_total[threadIdx.x] = total;
@@ -858,9 +876,11 @@ void launch_dtype(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, hi
 
 }  // namespace
 
-// More rows to a workgroup share the widening of codes, but a short call needs the workgroups: the tile is
-// the largest that leaves three workgroups to two compute units. Keys are split until they do, but
-// not below 8 records (two to a wave), where a workgroup's start and end weigh more than its keys.
+// Keys are split until every compute unit has as many workgroups as its registers hold (two; one at a
+// head_dim of 512), but not below 8 records, where a workgroup's start and end and its partial results
+// weigh more than its keys, or 4 where the rows are few: one sequence of 2,000 tokens 14.2 -> 12.7 us, but
+// 8 behind 2,000 13.9 -> 15.3. Two tiles of rows to a workgroup share the widening of codes, one makes more workgroups: where
+// two left fewer than 16 records to each, 7 x 8 drafts measured 19 -> 16 us with one.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -870,13 +890,15 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
     };
     const uint64_t pr = prefix_len ? records(prefix_len, prefix_len / 4u) : 0u, orr = own_most ? records(own_most, q_len) : 0u;
     AttnPlan p{};
+    p.rows = (uint64_t)batch * q_len * q_heads;
+    const uint64_t least = p.rows <= 64u ? 4u : 8u;
     for (uint32_t most = most_tiles(head_dim, dtype == TURBO_HIDDEN_F32);; most /= 2u) {
         p.own_tile_rows = 16u * tiles_for(own_rows, most);
         p.prefix_tile_rows = prefix_len ? 16u * tiles_for(all_rows, most) : p.own_tile_rows;
         const uint64_t pt = prefix_len ? (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows : 0u;
         const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
         const uint64_t work = kv_heads * (pt * pr + batch * ot * orr);
-        const uint64_t per = std::max<uint64_t>(8u, (work + 2u * cus - 1u) / (2u * cus));
+        const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(least, (work + groups - 1u) / groups);
         p.prefix_tiles = (uint32_t)pt;
         p.prefix_splits = prefix_len ? (uint32_t)((pr + per - 1u) / per) : 0u;
         p.own_tiles = (uint32_t)ot;
@@ -884,10 +906,9 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         if (!prefix_len && !own_most) p.own_splits = 1u;  // still writes zeros, or NaN past the tables
         p.prefix_items = kv_heads * pt * p.prefix_splits;
         p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
-        if (most == 1u || 2u * p.items >= 3u * cus) break;
+        if (most == 1u || per >= 16u) break;
     }
     p.parts = p.prefix_splits + p.own_splits;
-    p.rows = (uint64_t)batch * q_len * q_heads;
     if (p.parts > 1u) {
         p.stats_bytes = (p.rows * p.parts * sizeof(float2) + 15u) / 16u * 16u;
         p.bytes = p.stats_bytes + p.rows * p.parts * head_dim * sizeof(float);
