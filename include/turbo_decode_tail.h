@@ -443,7 +443,8 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * over the tokens that it sees, query head h over key/value head h / (q_heads / kv_heads). A query at
  * a negative position sees nothing and gives zeros (kv_len 0: a padded sequence). A query whose tokens
  * pass its page table, or lie on a page past the cache, gives NaN.
- * The prefix is read once for the whole batch: its products run over the rows of all sequences. Products
+ * The prefix is read once for the whole batch: its products run over the rows of all sequences (a
+ * sequence that fills the products' tiles by itself takes it along with its own tokens). Products
  * accumulate in FP32; for FP32 queries, queries and softmax weights keep 22 bits; for BF16 ones weights,
  * keys and values keep 11 (or 2^-24 of the largest of their 32 tokens, 2^-20 at 4 bits).
  */

@@ -406,12 +406,12 @@ def test_two_graphs_with_a_workspace_each_on_two_streams():
 
 def test_refusals():
     rng = np.random.default_rng(11)
-    s = Setup(rng, 2, 64, 8, 32, 40, [40])
+    s = Setup(rng, 2, 64, 8, 32, 400, [40])
     q = torch.zeros((1, 4, 64), device="cuda")
     out = torch.zeros_like(q)
 
     def refuse(word, **kw):
-        inp = inputs(s, q, out, 4, [80], dtype="f32")
+        inp = inputs(s, q, out, 4, [440], dtype="f32")
         for k, v in kw.items():
             setattr(inp, k, v)
         with pytest.raises(T.TurboError, match=word):
@@ -425,7 +425,7 @@ def test_refusals():
     refuse("2\\^31", prefix_len=2**31), refuse("2\\^31", page_stride=2**26)
     refuse("too large", batch=2**20, q_len=2**20)
     refuse("workspace is NULL", workspace=None), refuse("workspace holds", workspace_bytes=16)
-    inp = inputs(s, q, out, 4, [80], dtype="f32")
+    inp = inputs(s, q, out, 4, [440], dtype="f32")
     inp.workspace += 4
     with pytest.raises(T.TurboError, match="workspace must be"):
         s.cache.attend(inp)

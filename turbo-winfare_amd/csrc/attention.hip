@@ -155,18 +155,19 @@ __device__ inline Pair unpack_fp16(uint32_t w) {
 // n / d for n below 2^31, by the multiplier that divider() made of d
 __device__ inline uint32_t quotient(uint32_t n, Divider d) { return d.factor ? __umulhi(n, d.factor) >> d.shift : n; }
 
+// A sequence's records in order: the prefix's, whose last one may hold fewer than 32 of its tokens, then its own.
 struct Item {
-    bool prefix;
-    uint32_t head, row0, rows;     // key/value head, first row of the tile, rows of the segment
-    uint32_t seq;                  // own keys: the sequence
+    bool shared;                   // rows of every sequence, over the prefix alone
+    uint32_t head, row0, rows;     // key/value head, first row of the tile, rows there are
+    uint32_t seq;                  // otherwise: the sequence
     uint32_t split, splits, part;
-    const uint32_t* pages;
-    uint32_t table;                // entries of pages
+    int begin, end;                // positions of the keys
+    const uint32_t* pages;         // of the sequence's own tokens
 };
 
 struct Row {
     uint32_t token, head;          // of q and out
-    int lo, hi;                    // visible keys of the segment
+    int lo, hi;                    // positions it sees, of the item's
     bool exists, over;             // over: passes its page table
 };
 
@@ -174,18 +175,15 @@ __device__ inline Row row_of(const AttnArgs& a, const Item& it, uint32_t r) {
     Row w;
     w.exists = r < it.rows;
     if (!w.exists) r = it.rows - 1u;
-    const uint32_t b = it.prefix ? quotient(r, a.by_rows) : it.seq, in = it.prefix ? r - b * (a.q_len * a.group) : r;
+    const uint32_t b = it.shared ? quotient(r, a.by_rows) : it.seq, in = it.shared ? r - b * (a.q_len * a.group) : r;
     const uint32_t t = quotient(in, a.by_group);
     w.token = b * a.q_len + t;
     w.head = it.head * a.group + in - t * a.group;
     const long long pos = (long long)a.kv_len[b] - (long long)a.q_len + t;
-    const long long room = (long long)a.prefix_len + ((long long)a.page_stride << a.kv.page_shift);
-    w.over = pos >= room;
-    long long lo = a.window ? pos - (long long)a.window + 1 : 0, hi = pos + 1;
-    if (it.prefix) hi = hi < (long long)a.prefix_len ? hi : (long long)a.prefix_len;
-    else lo -= a.prefix_len, hi -= a.prefix_len;
-    w.lo = (int)(lo > 0 ? (lo < 0x7FFFFFFF ? lo : 0x7FFFFFFF) : 0);
-    w.hi = w.over ? 0 : (int)(hi > 0 ? hi : 0);
+    w.over = pos >= (long long)a.prefix_len + ((long long)a.page_stride << a.kv.page_shift);
+    const long long lo = a.window ? pos - (long long)a.window + 1 : 0;
+    w.lo = max(it.begin, (int)(lo > 0 ? (lo < 0x7FFFFFFF ? lo : 0x7FFFFFFF) : 0));
+    w.hi = w.over ? 0 : min(it.end, (int)(pos >= 0 ? pos + 1 : 0));
     return w;
 }
 
@@ -270,9 +268,14 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     auto most = [](int x, int y) { return max(x, y); };
     lo_min = uniform(wave_reduce(lo_min, least)), lo_max = uniform(wave_reduce(lo_max, most));
     hi_min = uniform(wave_reduce(hi_min, least)), hi_max = uniform(wave_reduce(hi_max, most));
+    // records: of the prefix up to prefix_records, then of the sequence's own tokens
+    const int prefix_len = (int)a.prefix_len, prefix_records = (prefix_len + (int)kKvBlock - 1) / (int)kKvBlock;
+    auto record_of = [&](int pos) {
+        return pos < prefix_len ? pos / (int)kKvBlock : prefix_records + (pos - prefix_len) / (int)kKvBlock;
+    };
     int s0 = 0, s1 = 0;  // this split's records
     if (hi_max > 0) {
-        const int b0 = lo_min / (int)kKvBlock, b1 = (hi_max + (int)kKvBlock - 1) / (int)kKvBlock;
+        const int b0 = record_of(lo_min), b1 = record_of(hi_max - 1) + 1;
         const int per = (b1 - b0 + (int)it.splits - 1) / (int)it.splits;
         s0 = min(b1, b0 + (int)it.split * per), s1 = min(b1, s0 + per);
     }
@@ -349,12 +352,16 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     }
 
     const uint32_t page_mask = (1u << a.kv.page_shift) / kKvBlock - 1u, block_shift = a.kv.page_shift - 5u;
-    auto page_at = [&](int blk) {  // the page of a record; past the table or the cache: none
-        const uint32_t i = (uint32_t)uniform(blk) >> block_shift;
-        return i < it.table ? table_word(it.pages, i) : 0xFFFFFFFFu;
+    const uint32_t prefix_table = (a.prefix_len + (1u << a.kv.page_shift) - 1u) >> a.kv.page_shift;
+    auto page_at = [&](int rec) {  // the page of a record; past the table or the cache: none
+        const int r = uniform(rec);
+        const bool own = r >= prefix_records;
+        const uint32_t i = (uint32_t)(own ? r - prefix_records : r) >> block_shift;
+        return i < (own ? a.page_stride : prefix_table) ? table_word(own ? it.pages : a.prefix_pages, i) : 0xFFFFFFFFu;
     };
-    auto record_at = [&](int blk, uint32_t page) {
-        return a.kv.base + kv_record_at(a.kv, page < a.kv.pages ? page : 0u, it.head, (uint32_t)blk & page_mask);
+    auto record_at = [&](int rec, uint32_t page) {
+        const uint32_t r = (uint32_t)(rec >= prefix_records ? rec - prefix_records : rec);
+        return a.kv.base + kv_record_at(a.kv, page < a.kv.pages ? page : 0u, it.head, r & page_mask);
     };
     const uint32_t at16 = lane * 16u, at_words = lane * (NG * 4u);
     uint4 kc[NG * KU], vc[NG * KU];
@@ -387,13 +394,14 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     int kexp = 0, vexp = -1000;
     bool vnan = false;
     auto size_of = [](uint32_t w) { return F32 ? w >> 16 : max((w >> 16) + (8u << 7), w & 0x7FFFu); };  // BF16 bits
-    auto prepare = [&](int base) {
-        if (base < lo_min || base + (int)kKvBlock > hi_max) {
+    auto prepare = [&](int base, int end) {
+        end = min(end, hi_max);
+        if (base < lo_min || base + (int)kKvBlock > end) {
             asm volatile("");  // a branch, not selects: few records are not seen whole
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const int key = base + (int)((lane * NG + i) & 31u);
-                if (key < lo_min || key >= hi_max) sw[i] = 0u;
+                if (key < lo_min || key >= end) sw[i] = 0u;
             }
         }
         uint32_t top = 0u;
@@ -454,11 +462,15 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         load_keys(rec);
     }
     while (blk < s1) {
-        const int next = blk + (int)kWaves, base = blk * (int)kKvBlock;
+        // position of the record's first token, and of the end of the tokens of its kind
+        const bool own_keys = blk >= prefix_records;
+        const int next = blk + (int)kWaves;
+        const int base = own_keys ? prefix_len + (blk - prefix_records) * (int)kKvBlock : blk * (int)kKvBlock;
+        const int end = own_keys ? 0x7FFFFFFF : prefix_len;
         const bool bad = page >= a.kv.pages;
         if constexpr (kEarly) load_values(rec);
         const uint32_t next_page = next < s1 ? page_at(next) : 0xFFFFFFFFu;
-        prepare(base);
+        prepare(base, end);
 
         // ---- scores of the rows against 32 keys
         float4v s[MT][2];
@@ -515,7 +527,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         }
 
         // ---- weights
-        const bool masked = base < lo_max || base + (int)kKvBlock > hi_min;
+        const bool masked = base < lo_max || base + (int)kKvBlock > min(hi_min, end);
         float p[MT][8];
         uint32_t seen[MT];
         Frag pw[MT];
@@ -530,7 +542,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = base + (j >> 2) * 16 + (int)g * 4 + (j & 3);
-                    if (key < row[mt].lo || key >= row[mt].hi) p[mt][j] = kNegInf, seen[mt] &= ~(1u << j);
+                    if (key < row[mt].lo || key >= min(row[mt].hi, end)) p[mt][j] = kNegInf, seen[mt] &= ~(1u << j);
                     else if (bad) p[mt][j] = __builtin_nanf("");
                 }
             }
@@ -738,14 +750,15 @@ __global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const Attn
     } sh;
     Item it;
     uint32_t id = blockIdx.x;
-    it.prefix = id < a.prefix_items;
-    if (it.prefix) {
+    it.shared = id < a.prefix_items;
+    if (it.shared) {
         id = same_die(id, a.prefix_items);
         const uint32_t tile = id % a.prefix_tiles, rest = id / a.prefix_tiles;
         it.split = rest % a.prefix_splits, it.splits = a.prefix_splits, it.part = it.split;
         it.head = rest / a.prefix_splits;
         it.seq = 0u, it.row0 = tile * 16u * MTP, it.rows = a.batch * a.q_len * a.group;
-        it.pages = a.prefix_pages, it.table = (a.prefix_len + (1u << a.kv.page_shift) - 1u) >> a.kv.page_shift;
+        it.begin = 0, it.end = (int)a.prefix_len;
+        it.pages = nullptr;
     } else {
         id -= a.prefix_items;
         if (a.own_tiles > 1u) id = same_die(id, a.items - a.prefix_items);
@@ -755,12 +768,13 @@ __global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const Attn
         rest /= a.own_splits;
         it.head = rest % a.kv.heads, it.seq = rest / a.kv.heads;
         it.row0 = tile * 16u * MTO, it.rows = a.q_len * a.group;
-        it.pages = a.pages + (uint64_t)it.seq * a.page_stride, it.table = a.page_stride;
+        it.begin = a.prefix_splits ? (int)a.prefix_len : 0, it.end = 0x7FFFFFFF;
+        it.pages = a.pages + (uint64_t)it.seq * a.page_stride;
     }
     if constexpr (MTP == MTO) {
         attend<NG, BITS, F32, MTP>(a, it, sh.p);
     } else {
-        if (it.prefix) attend<NG, BITS, F32, MTP>(a, it, sh.p);
+        if (it.shared) attend<NG, BITS, F32, MTP>(a, it, sh.p);
         else attend<NG, BITS, F32, MTO>(a, it, sh.o);
     }
 }
@@ -879,8 +893,11 @@ void launch_dtype(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, hi
 // Keys are split until every compute unit has as many workgroups as its registers hold (two; one at a
 // head_dim of 512), but not below 8 records, where a workgroup's start and end and its partial results
 // weigh more than its keys, or 4 where the rows are few: one sequence of 2,000 tokens 14.2 -> 12.7 us, but
-// 8 behind 2,000 13.9 -> 15.3. Two tiles of rows to a workgroup share the widening of codes, one makes more workgroups: where
-// two left fewer than 16 records to each, 7 x 8 drafts measured 19 -> 16 us with one.
+// 8 behind 2,000 13.9 -> 15.3. The prefix is taken apart from the sequences' own keys where that leaves
+// fewer tiles: with as many rows in a sequence as in a tile, a tile goes on from the prefix to its own
+// keys, without partial results to join. Two tiles of rows to a workgroup share the widening of codes,
+// one makes more workgroups: where two left fewer than 16 records to each, 7 x 8 drafts measured
+// 19 -> 16 us with one.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -894,16 +911,20 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
     const uint64_t least = p.rows <= 64u ? 4u : 8u;
     for (uint32_t most = most_tiles(head_dim, dtype == TURBO_HIDDEN_F32);; most /= 2u) {
         p.own_tile_rows = 16u * tiles_for(own_rows, most);
-        p.prefix_tile_rows = prefix_len ? 16u * tiles_for(all_rows, most) : p.own_tile_rows;
-        const uint64_t pt = prefix_len ? (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows : 0u;
         const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
-        const uint64_t work = kv_heads * (pt * pr + batch * ot * orr);
+        p.prefix_tile_rows = 16u * tiles_for(all_rows, most);
+        uint64_t pt = (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows;
+        const bool shared = pr && 2u * batch * ot > 3u * pt;
+        if (!shared) p.prefix_tile_rows = p.own_tile_rows, pt = 0u;
+        const uint64_t alone = shared ? orr : pr + orr;  // records of a workgroup's sequence
+        const uint64_t work = kv_heads * (pt * pr + batch * ot * alone);
         const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(least, (work + groups - 1u) / groups);
         p.prefix_tiles = (uint32_t)pt;
-        p.prefix_splits = prefix_len ? (uint32_t)((pr + per - 1u) / per) : 0u;
+        p.prefix_splits = shared ? (uint32_t)((pr + per - 1u) / per) : 0u;
         p.own_tiles = (uint32_t)ot;
-        p.own_splits = own_most ? (uint32_t)((orr + per - 1u) / per) : 0u;
-        if (!prefix_len && !own_most) p.own_splits = 1u;  // still writes zeros, or NaN past the tables
+        p.own_splits = (uint32_t)((alone + per - 1u) / per);
+        // without any keys a call still writes zeros, or NaN past the tables
+        if (!shared && !alone) p.own_splits = 1u;
         p.prefix_items = kv_heads * pt * p.prefix_splits;
         p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
         if (most == 1u || per >= 16u) break;

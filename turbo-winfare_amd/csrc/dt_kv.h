@@ -104,7 +104,8 @@ struct AttnArgs {
     uint32_t window;
     float scale_log2e;
     // the plan
-    uint32_t prefix_tiles, prefix_splits;    // row tiles and key splits of the prefix, per key/value head
+    uint32_t prefix_tiles, prefix_splits;    // row tiles and key splits of the prefix, per key/value head (0: the
+                                             // sequences take it with their own keys)
     uint32_t own_tiles, own_splits;          // of one sequence's own keys
     uint32_t prefix_items, items;            // workgroups
     Divider by_rows, by_group;               // by q_len * group, by group

@@ -111,7 +111,7 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in) 
     if (in.q_heads < 1 || in.q_heads > (int)kMaxQueryHeads || in.q_heads % (int)c.kv.heads != 0)
         fail("q_heads must be a multiple of the cache's kv_heads, at most " + std::to_string(kMaxQueryHeads));
     const uint64_t room = (uint64_t)in.page_stride * c.page_tokens;
-    if (in.prefix_len > 0x7FFFFF00u || room > 0x7FFFFF00u) fail("prefix_len and page_stride * page_tokens must be below 2^31 - 256");
+    if (in.prefix_len + room > 0x7FFFFF00u) fail("prefix_len + page_stride * page_tokens must be at most 2^31 - 256");
     const uint64_t beyond = in.max_kv_len > in.prefix_len ? in.max_kv_len - in.prefix_len : 0u;
     const tdt::AttnPlan p =
         tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype,
