@@ -35,7 +35,6 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWaves = 4;
-constexpr uint32_t kXcds = 8;
 constexpr uint32_t kJoinStats = 1024;
 constexpr float kNegInf = -__builtin_inff();
 
@@ -733,13 +732,6 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             }
         }
     }
-}
-
-// Workgroups are dealt out to the eight dies in turn. Tiles that read the same keys are neighbours in
-// `index`; this takes neighbours to one die, whose L2 then holds the keys for all of them.
-__device__ inline uint32_t same_die(uint32_t id, uint32_t n) {
-    const uint32_t per = n / kXcds, rest = n % kXcds, die = id % kXcds;
-    return die * per + min(die, rest) + id / kXcds;
 }
 
 template <int NG, uint32_t BITS, bool F32, int MTP, int MTO>

@@ -60,6 +60,14 @@ __host__ __device__ inline uint32_t kv_scale_byte(uint32_t groups, uint32_t whic
     return ((which * groups + group) * kKvBlock + t) * 4u;
 }
 
+constexpr uint32_t kXcds = 8;
+// Workgroups are dealt out to the eight dies in turn. Those that read or write the same lines are neighbours
+// in the returned number; this takes neighbours to one die, whose L2 then holds the lines for all of them.
+__host__ __device__ inline uint32_t same_die(uint32_t id, uint32_t n) {
+    const uint32_t per = n / kXcds, rest = n % kXcds, die = id % kXcds;
+    return die * per + (die < rest ? die : rest) + id / kXcds;
+}
+
 // kv_cache.hip: norms, rotation and the cache's write in one pass. Any part may be absent: q, k and v
 // null, turns null (no rotation), cache.base null.
 struct QkvArgs {

@@ -12,8 +12,8 @@
 //     registers.
 //   Values: 32 tokens are neighbours in the cache, so the codes pass through LDS, and four tokens in a row
 //     are transposed in registers to one 4-byte store per value; a decode step's lone tokens are bytes.
-// A code is (x - bias) / scale rounded to an integer, the quotient as IEEE division gives it, by one
-// multiplication with the group's reciprocal and one correction step of it (Markstein's theorem).
+// The cache's write is bound by its instructions, about 200 per 512 values (two thirds of the time at 4,001
+// tokens), so divisions are products with a group's reciprocal and one correction step.
 // k_kv_read: a thread takes four values of four tokens, 4-byte loads where the tokens are neighbours.
 #include <stdexcept>
 
@@ -26,7 +26,8 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxChunk = 32;      // tokens of a workgroup
 constexpr uint32_t kMaxHeads = 8;       // heads of a workgroup
-constexpr uint32_t kLdsBytes = 16384;   // for a workgroup's sines, or its values' codes
+constexpr uint32_t kGroups = 1000u;
+constexpr uint32_t kLdsBytes = 32768;   // for a workgroup's sines, or its values' codes
 
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -131,8 +132,13 @@ __device__ inline uint32_t quantise(const float (&x)[E], uint32_t (&code)[E / 4]
     lo = lanes_reduce<N>(lo, [](float a, float b) { return fminf(a, b); });
     hi = lanes_reduce<N>(hi, [](float a, float b) { return fmaxf(a, b); });
     const float bias = bf16_outward(lo, false);
-    const float scale = fmaxf(bf16_outward((hi - bias) / top, true), 0x1p-126f);
-    const float inv = finite ? 1.0f / scale : __builtin_nanf("");  // a code of NaN is 0
+    // quotients as IEEE division gives them: one correction step of a product with the correctly rounded
+    // reciprocal (Markstein's theorem); scale has 8 significant bits, so one Newton step rounds its
+    // reciprocal correctly
+    const float range = hi - bias, share = range * (1.0f / top);
+    const float scale = fmaxf(bf16_outward(fmaf(fmaf(-share, top, range), 1.0f / top, share), true), 0x1p-126f);
+    const float near = __builtin_amdgcn_rcpf(scale);
+    const float inv = finite ? fmaf(fmaf(-scale, near, 1.0f), near, near) : __builtin_nanf("");  // a code of NaN is 0
     // scale is rounded up and bias down, so the codes are within 0 .. top as they are
     float q[E];
 #pragma unroll
@@ -278,7 +284,7 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
     Walk at(n, heads, wave, HP);
     // lanes past the last head take it again and store nothing
     auto from = [&](const Walk& w) {
-        return src + (uint64_t)(t0 + w.t) * stride + (uint64_t)(h0 + min(w.h + sub, heads - 1u)) * D + d0;
+        return src + (uint64_t)(t0 + w.t) * stride + ((h0 + min(w.h + sub, heads - 1u)) * D + d0);
     };
     Vec<T, E> next;
     if (at.more()) next.load(from(at));
@@ -350,13 +356,13 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
                 for (int i = 0; i < E; ++i) x[i] = first ? x[i] * cs[i] - y[i] * sn[i] : x[i] * cs[i] + y[i] * sn[i];
             }
         }
-        if (dst && here) Vec<T, E>::store(dst + (uint64_t)(t0 + t) * out_stride + (uint64_t)head * D + d0, x);
+        if (dst && here) Vec<T, E>::store(dst + (uint64_t)(t0 + t) * out_stride + (head * D + d0), x);
         if constexpr (BITS != 0u) {
             if (stored) {
                 uint32_t code[E / 4];
                 constexpr int N = 64 / E;
                 const uint32_t word = quantise<E, N, BITS>(x, code);
-                const uint32_t slot = a.slots[t0 + t];
+                const uint32_t slot = __builtin_amdgcn_readfirstlane(a.slots[t0 + t]);
                 if (here && slot < a.kv.slots) {
                     uint8_t* rec = record_of(a.kv, slot, head);
                     if (lane % N == 0u)
@@ -386,7 +392,7 @@ __device__ inline void store_value_heads(const QkvArgs& a, const Division& v, ui
     const uint32_t d0 = (lane % LPH) * E, sub = lane / LPH;
     Walk at(n, heads, wave, HP);
     auto from = [&](const Walk& w) {
-        return static_cast<const T*>(a.v) + (uint64_t)(t0 + w.t) * a.v_stride + (uint64_t)(h0 + min(w.h + sub, heads - 1u)) * D + d0;
+        return static_cast<const T*>(a.v) + (uint64_t)(t0 + w.t) * a.v_stride + ((h0 + min(w.h + sub, heads - 1u)) * D + d0);
     };
     Vec<T, E> next;
     if (at.more()) next.load(from(at));
@@ -411,7 +417,7 @@ __device__ inline void store_value_heads(const QkvArgs& a, const Division& v, ui
         constexpr int N = 64 / E;
         const uint32_t word = quantise<E, N, BITS>(x, code);
         if (now.h + sub < heads) {
-            const uint32_t slot = places.slot[now.t];
+            const uint32_t slot = __builtin_amdgcn_readfirstlane(places.slot[now.t]);
             if (lane % N == 0u && slot != 0xFFFFFFFFu)
                 *reinterpret_cast<uint32_t*>(record_of(a.kv, slot, h0 + now.h + sub) + 2u * kv_part_bytes(NG, BITS) +
                                              kv_scale_byte(NG, 1u, slot & 31u, d0 / 64u)) = word;
@@ -427,11 +433,12 @@ __device__ inline void store_value_heads(const QkvArgs& a, const Division& v, ui
 template <int NG, class T, int E, uint32_t BITS>
 __global__ __launch_bounds__(kThreads) void k_qkv(const QkvArgs a, const Division v) {
     extern __shared__ __align__(16) uint8_t lds[];
+    // workgroups of neighbouring tokens on one die: they write the same lines of the cache
     if (blockIdx.x < v.turn_items) {
-        turn_heads<NG, T, E, BITS>(a, v, blockIdx.x, lds);
+        turn_heads<NG, T, E, BITS>(a, v, BITS != 0u ? same_die(blockIdx.x, v.turn_items) : blockIdx.x, lds);
     } else if constexpr (BITS != 0u) {
         __shared__ Places places;
-        store_value_heads<NG, T, E, BITS>(a, v, blockIdx.x - v.turn_items, lds, places);
+        store_value_heads<NG, T, E, BITS>(a, v, same_die(blockIdx.x - v.turn_items, gridDim.x - v.turn_items), lds, places);
     }
 }
 
@@ -500,14 +507,17 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(const KvReadArgs a, uint32
     }
 }
 
-// Tokens and heads of a workgroup, from the most that are useful: halved until there are a thousand workgroups,
-// first `first` (0: tokens, 1: heads), then the other, heads not below what four waves hold at once.
+// Tokens and heads of a workgroup, from the most that are useful, halved until there are a thousand workgroups:
+// the tokens first, which share a token's sines among more heads, or the heads first, which fill whole lines
+// of the cache (eight neighbouring tokens' keys, 32 tokens' values): a cache write of 4,001 tokens and its
+// read back measured 38.8 us with the tokens halved first, 32.5 so. Heads stay as many as least_heads, what
+// the waves hold at once, while tokens are left to halve.
 struct Shape {
     uint32_t chunk, heads;
 };
 Shape shape_for(uint32_t tokens, uint32_t all_heads, uint32_t chunk, uint32_t heads, uint32_t least_heads, bool heads_first) {
     Shape s{chunk, heads};
-    auto few = [&] { return (uint64_t)((tokens + s.chunk - 1u) / s.chunk) * ((all_heads + s.heads - 1u) / s.heads) < 1024u; };
+    auto few = [&] { return (uint64_t)((tokens + s.chunk - 1u) / s.chunk) * ((all_heads + s.heads - 1u) / s.heads) < kGroups; };
     auto fewer_heads = [&] {
         while (s.heads > least_heads && few()) s.heads = (s.heads + 1u) / 2u;
     };
@@ -527,10 +537,11 @@ void launch_qkv_typed(const QkvArgs& a, hipStream_t st) {
     size_t lds = 0u;
     const uint32_t turned = (a.q ? a.q_heads : 0u) + (keys ? a.kv_heads : 0u);
     if (turned) {
-        uint32_t chunk = kMaxChunk / 2u;
+        const bool lines = keys && a.kv.base != nullptr;
+        uint32_t chunk = lines ? kMaxChunk : kMaxChunk / 2u;
         while (a.turns && chunk > 1u && chunk * a.rotary_dim * 4u > kLdsBytes) chunk /= 2u;
         const uint32_t heads = min(max(a.q ? a.q_heads : 0u, keys ? a.kv_heads : 0u), kMaxHeads);
-        const Shape s = shape_for(a.tokens, turned, chunk, heads, min(4u * HP, heads), false);
+        const Shape s = shape_for(a.tokens, turned, chunk, heads, min(lines ? HP : 4u * HP, heads), lines);
         v.turn_chunk = s.chunk, v.turn_heads = s.heads;
         v.q_parts = a.q ? parts_of(a.q_heads, s.heads) : 0u;
         v.turn_parts = v.q_parts + (keys ? parts_of(a.kv_heads, s.heads) : 0u);
