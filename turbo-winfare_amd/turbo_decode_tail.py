@@ -548,11 +548,14 @@ def matvec_grouped(matrices, xs, outs, stream=None) -> None:
 def _stride(t) -> int:
     """Elements from one token to the next of a [tokens][heads][head_dim] tensor (0, packed, for a raw address).
     Heads of a token are contiguous; anything else cannot be passed."""
-    if t is None or not hasattr(t, "stride"):
+    try:
+        if t is None or t.is_contiguous():
+            return 0
+    except AttributeError:
         return 0
     if t.dim() == 3 and t.shape[0] and (t.stride(2) != 1 or t.stride(1) != t.shape[2]):
         raise ValueError("the heads of a token must be contiguous")
-    return 0 if t.is_contiguous() else t.stride(0)
+    return t.stride(0)
 
 
 class KvCache:
