@@ -411,7 +411,7 @@ TURBO_DT_API void* turbo_rotary_create(const TurboRotaryDesc* desc);
 TURBO_DT_API void turbo_rotary_destroy(void* rotary);
 
 typedef struct {
-    int tokens;                  /* >= 0 */
+    int tokens;                  /* 0 .. 2^28; refused where tokens x heads passes a grid */
     int dtype;                   /* TURBO_HIDDEN_* of q, k, v, q_out and k_out */
     int q_heads;
     int kv_heads;

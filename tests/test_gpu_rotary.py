@@ -202,3 +202,14 @@ def test_replayed_in_a_graph():
         torch.cuda.synchronize()
         close(qo, *plain(x[:, :4], None, True, pos, freqs(10000.0, dim), False), "f32")
         same(vr, L.stored(x[:, 6:], 8).astype(np.float32))
+
+
+def test_more_workgroups_than_a_grid_holds_are_refused():
+    # 2^28 tokens, 1,024 heads of 512: 2^32 workgroups of 32 tokens and 2 heads for the values alone
+    x = torch.zeros(64, device="cuda")
+    cache = T.KvCache(1, 32, 1024, 512)
+    with pytest.raises(T.TurboError, match="too large"):
+        cache.write(x, x, ids(np.arange(1)), 1 << 28)
+    r = T.Rotary(512)
+    with pytest.raises(T.TurboError, match="too large"):
+        r.apply(r.make_inputs(1 << 28, q=x, q_heads=8192, positions=ids(np.arange(1)), q_out=x))

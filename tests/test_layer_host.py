@@ -61,6 +61,17 @@ def test_every_value_has_its_place(tmp_path):
     assert subprocess.run([str(tmp_path / "kv")]).returncode == 0
 
 
+def test_a_grid_holds_fewer_than_two_to_the_32_threads(tmp_path):
+    (tmp_path / "grid.cpp").write_text("""
+#include "dt_kv.h"
+bool refused(uint64_t n) { try { return tdt::grid_blocks(n) != n; } catch (const std::runtime_error&) { return true; } }
+int main() { return refused(1) || refused((1u << 24) - 1u) || !refused(1u << 24) || !refused(1ull << 32) || !refused((1ull << 32) + 5u); }
+""")
+    subprocess.run(["g++", "-std=c++20", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{CSRC}", str(tmp_path / "grid.cpp"),
+                    "-o", str(tmp_path / "grid")], check=True)
+    assert subprocess.run([str(tmp_path / "grid")]).returncode == 0
+
+
 def test_struct_sizes():
     lib = T.load()
     for which, st in ((6, T.TurboKvCacheDesc), (7, T.TurboRotaryDesc), (8, T.TurboQkvInputs), (9, T.TurboAttentionInputs)):

@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+#include <stdexcept>
 
 namespace tdt {
 
@@ -36,6 +37,11 @@ struct KvView {
 __host__ __device__ inline uint32_t kv_part_bytes(uint32_t groups, uint32_t bits) { return groups * 64u * kKvBlock * bits / 8u; }
 __host__ __device__ inline uint32_t kv_record_bytes(uint32_t groups, uint32_t bits) {
     return 2u * kv_part_bytes(groups, bits) + 2u * groups * kKvBlock * 4u;
+}
+// Workgroups of 256 threads in one dimension of a grid, which holds fewer than 2^32 threads.
+inline uint32_t grid_blocks(uint64_t blocks) {
+    if (blocks >> 24) throw std::runtime_error("tokens * heads is too large for one call");
+    return (uint32_t)blocks;
 }
 // Byte offset of the record of 32 tokens number `block` of (page, head); 64 bits: caches pass 4 GiB.
 __host__ __device__ inline uint64_t kv_record_at(const KvView& kv, uint32_t page, uint32_t head, uint32_t block) {

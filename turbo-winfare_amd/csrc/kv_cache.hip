@@ -533,7 +533,7 @@ void launch_qkv_typed(const QkvArgs& a, hipStream_t st) {
     constexpr uint32_t D = NG * 64u, HP = 64u / (D / E);
     const bool keys = a.k != nullptr, values = a.v != nullptr && a.kv.base != nullptr;
     Division v{};
-    uint32_t value_items = 0u;
+    uint64_t turn_items = 0u, value_items = 0u;  // more than 32 bits at the most tokens of 1,024 heads of 512
     size_t lds = 0u;
     const uint32_t turned = (a.q ? a.q_heads : 0u) + (keys ? a.kv_heads : 0u);
     if (turned) {
@@ -545,7 +545,7 @@ void launch_qkv_typed(const QkvArgs& a, hipStream_t st) {
         v.turn_chunk = s.chunk, v.turn_heads = s.heads;
         v.q_parts = a.q ? parts_of(a.q_heads, s.heads) : 0u;
         v.turn_parts = v.q_parts + (keys ? parts_of(a.kv_heads, s.heads) : 0u);
-        v.turn_items = v.turn_parts * parts_of(a.tokens, s.chunk);
+        turn_items = (uint64_t)v.turn_parts * parts_of(a.tokens, s.chunk);
         if (a.turns) lds = (size_t)s.chunk * a.rotary_dim * 4u;
     }
     if (values) {
@@ -553,10 +553,11 @@ void launch_qkv_typed(const QkvArgs& a, hipStream_t st) {
         while (heads > 1u && kMaxChunk * heads * D > kLdsBytes) heads = (heads + 1u) / 2u;
         const Shape s = shape_for(a.tokens, a.kv_heads, kMaxChunk, heads, min(HP, heads), true);
         v.value_chunk = s.chunk, v.value_heads = s.heads, v.value_parts = parts_of(a.kv_heads, s.heads);
-        value_items = v.value_parts * parts_of(a.tokens, s.chunk);
+        value_items = (uint64_t)v.value_parts * parts_of(a.tokens, s.chunk);
         lds = max(lds, (size_t)s.chunk * s.heads * D);
     }
-    const dim3 grid(v.turn_items + value_items), block(kThreads);
+    const dim3 grid(grid_blocks(turn_items + value_items)), block(kThreads);
+    v.turn_items = (uint32_t)turn_items;
     if (!a.kv.base) hipLaunchKernelGGL((k_qkv<NG, T, E, 0u>), grid, block, lds, st, a, v);
     else if (a.kv.bits == 8u) hipLaunchKernelGGL((k_qkv<NG, T, E, 8u>), grid, block, lds, st, a, v);
     else hipLaunchKernelGGL((k_qkv<NG, T, E, 4u>), grid, block, lds, st, a, v);

@@ -16,7 +16,7 @@ namespace {
 
 constexpr uint32_t kCacheMagic = 0x564B4454u;   // "TDKV"
 constexpr uint32_t kRotaryMagic = 0x4F524454u;  // "TDRO"
-constexpr int kMaxTokens = 1 << 28;             // a grid holds at most 2^32 threads: 8 to a token
+constexpr int kMaxTokens = 1 << 28;             // a cache read takes 8 threads of one grid dimension to a token
 constexpr uint32_t kMaxKvHeads = 1024, kMaxQueryHeads = 8192;
 
 // The streams a handle's calls were enqueued on, waited for before it is freed.
