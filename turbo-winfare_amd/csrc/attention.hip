@@ -154,7 +154,8 @@ __device__ inline Pair unpack_fp16(uint32_t w) {
 // n / d for n below 2^31, by the multiplier that divider() made of d
 __device__ inline uint32_t quotient(uint32_t n, Divider d) { return d.factor ? __umulhi(n, d.factor) >> d.shift : n; }
 
-// A sequence's records in order: the prefix's, whose last one may hold fewer than 32 of its tokens, then its own.
+// What a workgroup takes. Records are numbered in order: the prefix's, whose last one may hold fewer than 32 of
+// its tokens, then the sequence's own.
 struct Item {
     bool shared;                   // rows of every sequence, over the prefix alone
     uint32_t head, row0, rows;     // key/value head, first row of the tile, rows there are
