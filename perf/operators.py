@@ -17,7 +17,6 @@ the other head sizes and ratios are generic.
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -170,7 +169,6 @@ def _code(dtype):
     return T().TURBO_HIDDEN_BF16 if dtype == "bf16" else T().TURBO_HIDDEN_F32
 
 
-@functools.cache
 def T():
     """The framework's binding; only the passes through the framework's own calls need it."""
     pkg = str(Path(__file__).resolve().parents[1] / "turbo-winfare_amd")
