@@ -300,7 +300,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             }
         top = rows_max(top);
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = sign == 0.0f ? 1.0f : ldexpf(fabsf(a.scale_log2e), -shift);
+        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), -shift), 0x1.fffffep127f);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if (n % kSharers != (int)wave / MT) continue;
@@ -533,10 +533,12 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         Frag pw[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const float by = F32 ? factor[mt] : ldexpf(factor[mt], kexp);
+            // The factor may leave FP32 (small keys and queries, a large scale): a score of 0 stays 0, and a
+            // hidden key's -infinity is set after the product, which would make it NaN.
+            const float by = F32 ? factor[mt] : fminf(ldexpf(factor[mt], kexp), 0x1.fffffep127f);
             seen[mt] = 0xFFu;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3];
+            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3] * by;
             if (bad || masked) {
                 asm volatile("");
 #pragma unroll
@@ -549,7 +551,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             float top = kNegInf;
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, p[mt][j]);
-            top = fmaf(rows_max(top), by, -kLift);
+            top = rows_max(top) - kLift;
             if (__any(top > m[mt] + kSlack)) {
                 top = fmaxf(m[mt], top);
                 const float alpha = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[mt] - top);
@@ -564,7 +566,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             const float zero = m[mt] == kNegInf ? 0.0f : m[mt];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[mt][j] = __builtin_amdgcn_exp2f(fmaf(p[mt][j], by, -zero));
+                p[mt][j] = __builtin_amdgcn_exp2f(p[mt][j] - zero);
                 l[mt] += p[mt][j];
             }
             if constexpr (!F32)
