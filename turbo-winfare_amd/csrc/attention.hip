@@ -551,9 +551,10 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             float top = kNegInf;
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, p[mt][j]);
-            top = rows_max(top) - kLift;
-            if (__any(top > m[mt] + kSlack)) {
-                top = fmaxf(m[mt], top);
+            top = rows_max(top);
+            // the difference that the exponential takes: at large scores m + kLift + kSlack would round
+            if (__any(top - m[mt] > kLift + kSlack)) {
+                top = top - m[mt] > kLift + kSlack ? top - (top - (top - kLift) > kLift + kSlack ? 0.0f : kLift) : m[mt];
                 const float alpha = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[mt] - top);
                 l[mt] *= alpha;
                 if constexpr (F32)
