@@ -445,8 +445,8 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * pass its page table, or lie on a page past the cache, gives NaN.
  * The prefix is read once for the whole batch: its products run over the rows of all sequences (a
  * sequence that fills the products' tiles by itself takes it along with its own tokens). Products
- * accumulate in FP32; for FP32 queries, queries and softmax weights keep 22 bits; for BF16 ones weights,
- * keys and values keep 11 (or 2^-24 of the largest of their 32 tokens, 2^-20 at 4 bits).
+ * accumulate in FP32. Keys and values enter as the cache holds them. For FP32 queries, queries and softmax
+ * weights keep 22 bits; for BF16 ones the weights keep 11.
  */
 typedef struct {
     int batch;                   /* >= 0 */

@@ -70,8 +70,70 @@ def test_scores_whose_last_place_is_more_than_one(dtype, size):
     size_v = s.stored(s.v)[1][:, 0]
     bound = w * np.maximum(size_v[:32].mean(0), size_v[128:160].mean(0))
     bound += 2.0**-8 * (np.abs(want) + bound) if dtype == "bf16" else 0.0
-    if dtype == "bf16":  # one running sum over the head: the small difference may be lost, the weights stay finite
-        ends = np.concatenate([v[:32], v[128:160]])
-        assert np.all(got <= ends.max(0) + bound) and np.all(got >= ends.min(0) - bound)
-        return
     assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / bound).max())
+
+
+def seen(s, q, b, q_len, kv_len, window, scale, dtype):
+    """Sequence b's outputs and a bound that knows of a row only the tokens that it sees. With a value as
+    (code - middle) * scale + centre, K the sum of both addends' sizes and S the larger of 128 scale and
+    |centre| over the head:
+      a score is off by scale * sum |q| K (2^-22 + 80 * 2^-24) (queries keep 22 bits; 64 products, the groups
+      and the centres add in FP32) and (2 |s| log2(e) + 2) 2^-23 of the weight (factor, difference, exponential);
+      a weight is rounded to 2^-12 (BF16) or 2^-22 of itself, or, where that is coarser, a weighted value to 2^-32
+      of the row's largest weighted S, known to a factor of 4;
+      40 + keys / 32 roundings of the sums."""
+    t = s.tokens(b)[:kv_len]
+    mid = 128.0 if s.bits == 8 else 8.0
+
+    def parts(x):
+        c, sc, bi = (a.astype(np.float64) for a in L.quantise(x[t], s.bits))
+        centre = bi + mid * sc
+        size = np.maximum(128 * sc, np.abs(centre)).max(-1)
+        add = np.abs(c - mid) * sc[..., None] + np.abs(centre)[..., None]
+        return (c * sc[..., None] + bi[..., None]).reshape(x[t].shape), add.reshape(x[t].shape), size
+
+    (k, kk, _), (v, vv, vs) = parts(s.k), parts(s.v)
+    q = q.astype(np.float64)
+    g = q.shape[1] // s.heads
+    out, bound = np.zeros_like(q), np.zeros_like(q)
+    for i in range(q_len):
+        p = kv_len - q_len + i
+        lo, hi = (max(0, p - window + 1) if window else 0), p + 1
+        if hi <= lo:
+            continue
+        for h in range(q.shape[1]):
+            at = (slice(lo, hi), h // g)
+            sc = k[at] @ q[i, h] * scale
+            w = np.exp(sc - sc.max())
+            w /= w.sum()
+            out[i, h] = w @ v[at]
+            e = scale * (kk[at] @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
+            rel = (2.0**-22 if dtype == "f32" else 2.0**-12) + (40 + (hi - lo) / 32) * 2.0**-24
+            bound[i, h] = (2 * e.max() + rel) * (w @ vv[at]) + (hi - lo) * 2.0**-30 * (w * vs[at]).max()
+    if dtype == "bf16":
+        bound += 2.0**-8 * (np.abs(out) + bound)
+    return out, bound + 1e-37
+
+
+def hold(s, q, out, kv_len, q_len, window, dtype, scale):
+    got = out.float().cpu().numpy().astype(np.float64)
+    for b, n in enumerate(kv_len):
+        rows = slice(b * q_len, (b + 1) * q_len)
+        want, bound = seen(s, q[rows], b, q_len, n, window, scale, dtype)
+        off = np.abs(got[rows] - want)
+        assert np.all(off <= bound), (b, n, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 8)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_large_scores_of_nearly_equal_keys(dtype, dim, bits):
+    """Pairs of keys whose large scores are close: their weights are as exact as the scores, to which a code
+    enters as it is."""
+    rng = np.random.default_rng(6)
+    s = Setup(rng, 1, dim, bits, 32, 64, [64])
+    near = rng.standard_normal((1, 1, dim)).astype(np.float32)
+    s.k = L.bf16((near * (1 + 0.01 * rng.standard_normal(s.k.shape))).astype(np.float32))
+    s.write(np.arange(128))
+    q = L.bf16(40.0 * queries(rng, 1, 16, dim, "f32"))
+    out = attend(s, q, 16, [128], dtype)
+    hold(s, q, out, [128], 1, 0, dtype, dim**-0.5)

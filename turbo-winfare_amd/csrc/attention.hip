@@ -9,17 +9,16 @@
 //     power of two of the row.
 //   O^T += V^T P^T: a lane holds the scores of 8 keys of one row, and those 8 keys' value codes are its
 //     bytes of the record, so the weights are the second operand as they are.
-// A code widened to 16 bits is the fp16 denormal code * 2^-24, exact, one byte permute for two.
-// BF16 queries: a key or value is code * s' + b', one packed fused multiply-add on two denormals, with the
-//   scales and biases brought below 1 for the record by a power of two: rounded to 11 bits, or to 2^-24 of
-//   the record's largest (2^-20 at 4 bits). The weights are rounded to 11 bits (2^-12 of each, against
-//   the output's 2^-9); q is exact.
-// FP32 queries: products of the codes themselves, q and the weights in two fp16 parts each (22 bits). A
-//   key's scale and bias enter its score in FP32, sum_g s_g (codes_g . q_g) + b_g sum(q_g) over the
-//   groups of 64, and a value's its weight; the record's largest value scale is brought just inside fp16.
-//   The codes are centred (code - 128 or - 8): products of denormals add up with 4 (8 bits) to 7 (4 bits)
-//   bits less than FP32 has, and a sum of codes that are all positive cancels against the biases.
-//   Measured against 64 bits at 777 keys, 4 bits: 2e-7, with plain codes 5e-5.
+// A code enters as a whole number in fp16, exact: code - 128 (8 bits) or code - 8 (4 bits), two by one byte
+// permute and one packed addition. (As denormals, code * 2^-24, they need no addition, but products of
+// denormals add up with 4 to 7 bits less than FP32 has; uncentred, sums of codes that are all positive cancel
+// against the biases: 5e-5 of the result in place of 2e-7, 777 keys of 4 bits.)
+//   A key's scale and centre (the value of the middle code) enter its score in FP32: sum over the groups of 64 of
+//   scale (codes . q) + centre sum(q), the second part by one FP32 matrix instruction per 16 keys and four groups.
+//   A value's scale enters its weight, sum of (weight * scale) codes, and the centres are added with the weights
+//   themselves, in FP32 matrix instructions.
+//   BF16 queries: q is exact in fp16, weights times scale are rounded to 11 bits, 2^-12 of each, against the
+//   output's 2^-9. FP32 queries: q and the weights times scale in two fp16 parts each (22 bits).
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
@@ -65,55 +64,51 @@ __device__ inline float rows_reduce(float v, Op op) {
 __device__ inline float rows_max(float v) { return rows_reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ inline float rows_sum(float v) { return rows_reduce(v, [](float a, float b) { return a + b; }); }
 
-// A pair of 16-bit codes as fp16: plain, the denormals code * 2^-24, or centred, the numbers
-// code - 128 (8 bits) or code - 8 (4 bits), by way of 1024 + code.
-template <uint32_t BITS, bool CENTRED>
-__device__ inline uint32_t as_fp16(uint32_t pair) {
-    if constexpr (!CENTRED) return pair;
+// A pair of 16-bit codes as fp16 numbers, code - 128 (8 bits) or code - 8 (4 bits), by way of 1024 + code,
+// whose upper bytes (0x64) are in the pair already.
+template <uint32_t BITS>
+__device__ inline uint32_t centred(uint32_t pair) {
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));
     union {
         uint32_t u;
         half2v h;
     } x;
-    x.u = pair | 0x64006400u;
+    x.u = pair;
     const _Float16 middle = (_Float16)(BITS == 8u ? -1152.0f : -1032.0f);
     x.h += half2v{middle, middle};
     return x.u;
 }
-// eight bytes, in order
-template <bool CENTRED>
+// eight bytes, in order; the permute takes the upper bytes from a constant
 __device__ inline Frag widen_bytes(uint32_t a, uint32_t b) {
-    constexpr uint32_t top = CENTRED ? 0x64646464u : 0u;  // the upper bytes, taken by the same permute
+    constexpr uint32_t top = 0x64646464u;
     Frag f;
-    f.u[0] = as_fp16<8u, CENTRED>(__builtin_amdgcn_perm(top, a, CENTRED ? 0x04010400u : 0x0C010C00u));
-    f.u[1] = as_fp16<8u, CENTRED>(__builtin_amdgcn_perm(top, a, CENTRED ? 0x04030402u : 0x0C030C02u));
-    f.u[2] = as_fp16<8u, CENTRED>(__builtin_amdgcn_perm(top, b, CENTRED ? 0x04010400u : 0x0C010C00u));
-    f.u[3] = as_fp16<8u, CENTRED>(__builtin_amdgcn_perm(top, b, CENTRED ? 0x04030402u : 0x0C030C02u));
+    f.u[0] = centred<8u>(__builtin_amdgcn_perm(top, a, 0x04010400u));
+    f.u[1] = centred<8u>(__builtin_amdgcn_perm(top, a, 0x04030402u));
+    f.u[2] = centred<8u>(__builtin_amdgcn_perm(top, b, 0x04010400u));
+    f.u[3] = centred<8u>(__builtin_amdgcn_perm(top, b, 0x04030402u));
     return f;
 }
 // eight nibbles of one word: operand elements 2 p, 2 p + 1 are nibbles p, p + 4 (the queries are laid out alike)
-template <bool CENTRED>
 __device__ inline Frag widen_nibbles(uint32_t w) {
     Frag f;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) f.u[p] = as_fp16<4u, CENTRED>((w >> (4 * p)) & 0x000F000Fu);
+    for (int p = 0; p < 4; ++p) f.u[p] = centred<4u>(((w >> (4 * p)) & 0x000F000Fu) | 0x64006400u);
     return f;
 }
 // the low (shift 0) or high (shift 4) halves of eight bytes: elements are bytes 0, 2, 1, 3 of each word
 // (the weights are laid out alike)
-template <bool CENTRED>
 __device__ inline Frag widen_halves(uint32_t a, uint32_t b, uint32_t shift) {
     Frag f;
-    f.u[0] = as_fp16<4u, CENTRED>((a >> shift) & 0x000F000Fu);
-    f.u[1] = as_fp16<4u, CENTRED>((a >> (8u + shift)) & 0x000F000Fu);
-    f.u[2] = as_fp16<4u, CENTRED>((b >> shift) & 0x000F000Fu);
-    f.u[3] = as_fp16<4u, CENTRED>((b >> (8u + shift)) & 0x000F000Fu);
+    f.u[0] = centred<4u>(((a >> shift) & 0x000F000Fu) | 0x64006400u);
+    f.u[1] = centred<4u>(((a >> (8u + shift)) & 0x000F000Fu) | 0x64006400u);
+    f.u[2] = centred<4u>(((b >> shift) & 0x000F000Fu) | 0x64006400u);
+    f.u[3] = centred<4u>(((b >> (8u + shift)) & 0x000F000Fu) | 0x64006400u);
     return f;
 }
-// A word's scale, and its bias as centred codes need it: that of the middle code
+// A word's scale, and its centre: the value of the middle code
 __device__ inline float scale_of(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 template <uint32_t BITS>
-__device__ inline float bias_of(uint32_t w) {
+__device__ inline float centre_of(uint32_t w) {
     return fmaf(BITS == 8u ? 128.0f : 8.0f, scale_of(w), __uint_as_float(w << 16));
 }
 
@@ -207,17 +202,6 @@ __device__ inline void store_out(void* out, uint64_t at, float4 v) {
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-// x * s + b on two fp16 numbers
-__device__ inline uint32_t fma_fp16(uint32_t x, uint32_t s, uint32_t b) {
-    union Half2 {
-        uint32_t u;
-        half2v h;
-    } p, q, r;
-    p.u = x, q.u = s, r.u = b;
-    p.h = p.h * q.h + r.h;
-    return p.u;
-}
 __device__ inline Frag operand(uint4 v) {
     Frag f;
     f.u[0] = v.x, f.u[1] = v.y, f.u[2] = v.z, f.u[3] = v.w;
@@ -230,12 +214,13 @@ struct Shared {
     union {
         struct {
             uint4 q[MT][NG][F32 ? 4 : 2][64];            // the queries as second operands: [.., chunk of 32 (and low parts)][lane]
-            uint32_t words[kWaves][2 * NG * kKvBlock];   // a wave's record: scales and biases, as they are or s', b' in fp16
+            // a wave's record: scales and centres, [keys, values][group][32 tokens]
+            float scale[kWaves][2 * NG * kKvBlock], centre[kWaves][2 * NG * kKvBlock];
         };
         float sums[kWaves][16 * MT][kRow];
     };
     float m[kWaves][16 * MT], l[kWaves][16 * MT], factor[16 * MT];
-    float qsum[F32 ? 16 * MT : 1][NG + 1];  // of a row's groups, fp32 queries
+    float qsum[16 * MT][NG + 1];  // of a row's groups
 };
 
 template <int NG, uint32_t BITS, bool F32, int MT>
@@ -323,30 +308,27 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 sh.q[mt][n][c][lane] = make_uint4(h.u[0], h.u[1], h.u[2], h.u[3]);
                 if constexpr (F32) sh.q[mt][n][2 + c][lane] = make_uint4(low.u[0], low.u[1], low.u[2], low.u[3]);
             }
-            if constexpr (F32) {
-                sum = rows_sum(sum);
-                if (g == 0u) sh.qsum[mt * 16 + lane][n] = sum;
-            }
+            sum = rows_sum(sum);
+            if (g == 0u) sh.qsum[mt * 16 + lane][n] = sum;
         }
     }
     __syncthreads();
-    float factor[MT], qsum[F32 ? MT : 1][F32 ? NG : 1];
+    // the groups' sums as the FP32 products' second operand: that of group 4 h + lane / 16
+    constexpr int kFours = NG > 4 ? NG / 4 : 1;
+    float factor[MT], qsum[MT][kFours];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         factor[mt] = sh.factor[mt * 16 + (lane & 15u)];
-        if constexpr (F32)
 #pragma unroll
-            for (int n = 0; n < NG; ++n) qsum[mt][n] = sh.qsum[mt * 16 + (lane & 15u)][n];
+        for (int h = 0; h < kFours; ++h) qsum[mt][h] = g < (uint32_t)NG ? sh.qsum[mt * 16 + (lane & 15u)][min(4u * h + g, NG - 1u)] : 0.0f;
     }
 
     float4v o[MT][NG * 4];
-    float obias[F32 ? MT : 1][F32 ? NG : 1], m[MT], l[MT];
+    float4v oc[MT];  // the centres' sums, rows of the product: element e of lane / 16 is group (4 (lane / 16) + e) mod NG
+    float m[MT], l[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = kNegInf, l[mt] = 0.0f;
-        if constexpr (F32)
-#pragma unroll
-            for (int n = 0; n < NG; ++n) obias[mt][n] = 0.0f;
+        m[mt] = kNegInf, l[mt] = 0.0f, oc[mt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NG * 4; ++i) o[mt][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -386,14 +368,13 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
         for (int i = 0; i < NG * KU; ++i) vc[i] = *reinterpret_cast<const uint4*>(rec + PART + i * 1024u + at16);
     };
-    uint32_t* words = sh.words[wave];
+    float *scales = sh.scale[wave], *centres = sh.centre[wave];
 
-    // Powers of two of a record's keys and values. BF16: 2^8 scales and the biases are below 2^(e - 2), so their
-    // sum is below 2^e. FP32: the values' scales are below 2^(e + 8), their weights below 2^7. Words of keys that no row sees become
-    // 0, as do a value's of NaN; the values' power is that of the sums, which never falls.
-    int kexp = 0, vexp = -1000;
+    // A record's scales and centres. Words of keys that no row sees become 0, as do a value's of NaN. The values'
+    // power of two, 2^(e + kTop) above the largest scale, is that of the sums and never falls.
+    constexpr int kTop = F32 ? 8 : 0;
+    int vexp = -1000;
     bool vnan = false;
-    auto size_of = [](uint32_t w) { return F32 ? w >> 16 : max((w >> 16) + (8u << 7), w & 0x7FFFu); };  // BF16 bits
     auto prepare = [&](int base, int end) {
         end = min(end, hi_max);
         if (base < lo_min || base + (int)kKvBlock > end) {
@@ -406,17 +387,15 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         }
         uint32_t top = 0u;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) top = max(top, size_of(sw[i]));
-        constexpr uint32_t kNan = F32 ? 0x7F80u : 0x7F80u + (8u << 7);
+        for (int i = 0; i < NG; ++i) top = max(top, sw[i]);
         vnan = false;
-        if (__any(top >= kNan)) {
+        if (__any(lane >= 32u && top >= 0x7F800000u)) {
             asm volatile("");
             top = 0u;
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                const uint32_t size = size_of(sw[i]);
-                if (size < kNan) top = max(top, size);
-                else if (!F32 && lane >= 32u) sw[i] = 0u, vnan = true;
+                if (lane >= 32u && sw[i] >= 0x7F800000u) sw[i] = 0u, vnan = true;
+                top = max(top, sw[i]);
             }
             vnan = __any(vnan);
         }
@@ -424,9 +403,8 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         top = max(top, dpp_mov<dpp::kXor2>(top));
         top = max(top, dpp_mov<dpp::kRor4>(top));
         top = max(top, dpp_mov<dpp::kRor8>(top));
-        const int kt = (int)max(lane_read(top, 0), lane_read(top, 16)) >> 7, vt = (int)max(lane_read(top, 32), lane_read(top, 48)) >> 7;
-        if constexpr (!F32) kexp = uniform(min(max(kt - 125, -120), 113));
-        const int want = uniform(min(max(vt - (F32 ? 134 : 125), -120), 113));
+        const int vt = (int)(max(lane_read(top, 32), lane_read(top, 48)) >> 23);
+        const int want = uniform(min(max(vt - 126 - kTop, -120), 113));
         if (want > vexp) {
             if (vexp > -1000) {
 #pragma unroll
@@ -438,16 +416,19 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             }
             vexp = want;
         }
-        uint32_t w[NG];
-        const int shift = lane < 32u ? -kexp : -vexp;
+        float sc[NG], ce[NG];
+        const float unit = lane < 32u ? 1.0f : __uint_as_float((uint32_t)(127 - vexp) << 23);
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
-            w[i] = F32 ? sw[i] : pack_fp16(ldexpf(__uint_as_float(sw[i] & 0xFFFF0000u), 24 + shift), ldexpf(__uint_as_float(sw[i] << 16), shift));
-        if constexpr (NG == 1) words[lane] = w[0];
-        if constexpr (NG == 2) *reinterpret_cast<uint2*>(words + lane * 2u) = make_uint2(w[0], w[1]);
-        if constexpr (NG >= 4)
+        for (int i = 0; i < NG; ++i) sc[i] = scale_of(sw[i]) * unit, ce[i] = centre_of<BITS>(sw[i]);
+        auto put = [&](float* to, const float (&x)[NG]) {
+            if constexpr (NG == 1) to[lane] = x[0];
+            if constexpr (NG == 2) *reinterpret_cast<float2*>(to + lane * 2u) = make_float2(x[0], x[1]);
+            if constexpr (NG >= 4)
 #pragma unroll
-            for (int i = 0; i < NG; i += 4) *reinterpret_cast<uint4*>(words + lane * NG + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+                for (int i = 0; i < NG; i += 4) *reinterpret_cast<float4*>(to + lane * NG + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        };
+        put(scales, sc);
+        put(centres, ce);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -475,7 +456,14 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         // ---- scores of the rows against 32 keys
         float4v s[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][0] = s[mt][1] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+            for (int h = 0; h < kFours; ++h) {
+                const float c = centres[(NG < 4 ? g % NG : 4u * h + g) * kKvBlock + tile * 16u + (lane & 15u)];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+                    s[mt][tile] = __builtin_amdgcn_mfma_f32_16x16x4f32(c, qsum[mt][h], h ? s[mt][tile] : float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            }
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             Frag q[MT][F32 ? 4 : 2];
@@ -488,37 +476,29 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 Frag k[2];
                 if constexpr (BITS == 8u) {
                     const uint4 c = kc[n * 2 + tile];
-                    k[0] = widen_bytes<F32>(c.x, c.y), k[1] = widen_bytes<F32>(c.z, c.w);
+                    k[0] = widen_bytes(c.x, c.y), k[1] = widen_bytes(c.z, c.w);
                 } else {
                     const uint4 c = kc[n];
-                    k[0] = widen_nibbles<F32>(tile ? c.z : c.x), k[1] = widen_nibbles<F32>(tile ? c.w : c.y);
+                    k[0] = widen_nibbles(tile ? c.z : c.x), k[1] = widen_nibbles(tile ? c.w : c.y);
                 }
-                if constexpr (!F32) {
-                    const uint32_t p = words[n * kKvBlock + tile * 16u + (lane & 15u)];  // of the lane's key
-                    const uint32_t sc = __builtin_amdgcn_perm(p, p, 0x01000100u), b = __builtin_amdgcn_perm(p, p, 0x03020302u);
+                const float4 sc = *reinterpret_cast<const float4*>(scales + n * kKvBlock + tile * 16u + g * 4u);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                for (int mt = 0; mt < MT; ++mt) {
+                    float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) k[c].u[e] = fma_fp16(k[c].u[e], sc, b);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) s[mt][tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[c].h, q[mt][c].h, s[mt][tile], 0, 0, 0);
-                } else {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(words + n * kKvBlock + tile * 16u + g * 4u);
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[c & 1].h, q[mt][c].h, acc, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[mt][tile][i] = fmaf(scale_of(w[i]), acc[i], fmaf(bias_of<BITS>(w[i]), qsum[mt][n], s[mt][tile][i]));
-                    }
+                    for (int c = 0; c < (F32 ? 4 : 2); ++c) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[c & 1].h, q[mt][c].h, acc, 0, 0, 0);
+                    s[mt][tile][0] = fmaf(sc.x, acc[0], s[mt][tile][0]);
+                    s[mt][tile][1] = fmaf(sc.y, acc[1], s[mt][tile][1]);
+                    s[mt][tile][2] = fmaf(sc.z, acc[2], s[mt][tile][2]);
+                    s[mt][tile][3] = fmaf(sc.w, acc[3], s[mt][tile][3]);
                 }
             }
         }
+        // The sums end here: left to itself the compiler moves them past the next loads, to where the scores are
+        // used, with all products and scales alive (100 registers).
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (!kEarly) load_values(rec);
         const uint8_t* next_rec = rec;
         if (next < s1) {
@@ -530,15 +510,13 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         const bool masked = base < lo_max || base + (int)kKvBlock > min(hi_min, end);
         float p[MT][8];
         uint32_t seen[MT];
-        Frag pw[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            // The factor may leave FP32 (small keys and queries, a large scale): a score of 0 stays 0, and a
-            // hidden key's -infinity is set after the product, which would make it NaN.
-            const float by = F32 ? factor[mt] : fminf(ldexpf(factor[mt], kexp), 0x1.fffffep127f);
+            // The factor may leave FP32 (small queries, a large scale): a score of 0 stays 0, and a hidden key's
+            // -infinity is set after the product, which would make it NaN.
             seen[mt] = 0xFFu;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3] * by;
+            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3] * factor[mt];
             if (bad || masked) {
                 asm volatile("");
 #pragma unroll
@@ -557,9 +535,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 top = top - m[mt] > kLift + kSlack ? top - (top - (top - kLift) > kLift + kSlack ? 0.0f : kLift) : m[mt];
                 const float alpha = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[mt] - top);
                 l[mt] *= alpha;
-                if constexpr (F32)
-#pragma unroll
-                    for (int n = 0; n < NG; ++n) obias[mt][n] *= alpha;
+                oc[mt] *= alpha;
 #pragma unroll
                 for (int i = 0; i < NG * 4; ++i) o[mt][i] *= alpha;
                 m[mt] = top;
@@ -570,95 +546,70 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 p[mt][j] = __builtin_amdgcn_exp2f(p[mt][j] - zero);
                 l[mt] += p[mt][j];
             }
-            if constexpr (!F32)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int x = BITS == 8u ? 2 * e : (e & 2) * 2 + (e & 1), y = x + (BITS == 8u ? 1 : 2);
-                    pw[mt].u[e] = pack_fp16(p[mt][x], p[mt][y]);
-                }
         }
 
         // ---- weighted values
-        const float unit = __uint_as_float((uint32_t)(127 - vexp) << 23);
+        {
+            const float* c = centres + (NG + lane % NG) * kKvBlock + g * 4u;
+            const float4 ca = *reinterpret_cast<const float4*>(c), cb = *reinterpret_cast<const float4*>(c + 16u);
+            const float c8[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) oc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(c8[j], p[mt][j], oc[mt], 0, 0, 0);
+        }
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            const uint4 wa = *reinterpret_cast<const uint4*>(words + (NG + n) * kKvBlock + g * 4u);
-            const uint4 wb = *reinterpret_cast<const uint4*>(words + (NG + n) * kKvBlock + 16u + g * 4u);
-            const uint32_t w8[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-            Frag ph[F32 ? MT : 1], pl[F32 ? MT : 1];
-            uint32_t sc[4], b[4];  // in the order of the codes
-            if constexpr (!F32) {
+            const float* sn = scales + (NG + n) * kKvBlock + g * 4u;
+            const float4 sa = *reinterpret_cast<const float4*>(sn), sb = *reinterpret_cast<const float4*>(sn + 16u);
+            const float s8[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+            Frag ph[MT], pl[F32 ? MT : 1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // in the order of the codes
                     const int x = BITS == 8u ? 2 * e : (e & 2) * 2 + (e & 1), y = x + (BITS == 8u ? 1 : 2);
-                    sc[e] = __builtin_amdgcn_perm(w8[y], w8[x], 0x05040100u), b[e] = __builtin_amdgcn_perm(w8[y], w8[x], 0x07060302u);
-                }
-            } else {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = w8[j];
-                    if (masked) {
-                        asm volatile("");
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (!((seen[mt] >> j) & 1u)) w[j] = 0u;  // NaN of a key that this row does not see
-                    }
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[j] = p[mt][j] * unit * scale_of(w[j]);
-                        obias[mt][n] = fmaf(p[mt][j], bias_of<BITS>(w[j]), obias[mt][n]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int x = BITS == 8u ? 2 * e : (e & 2) * 2 + (e & 1), y = x + (BITS == 8u ? 1 : 2);
-                        ph[mt].u[e] = pack_fp16(v[x], v[y]);
+                    const float u = p[mt][x] * s8[x], v = p[mt][y] * s8[y];
+                    ph[mt].u[e] = pack_fp16(u, v);
+                    if constexpr (F32) {
                         const Pair h = unpack_fp16(ph[mt].u[e]);
-                        pl[mt].u[e] = pack_fp16(v[x] - h.lo, v[y] - h.hi);
+                        pl[mt].u[e] = pack_fp16(u - h.lo, v - h.hi);
                     }
                 }
-            }
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 Frag f;
                 if constexpr (BITS == 8u) {
                     const uint4 c = vc[n * 2 + (d >> 1)];
-                    f = (d & 1) ? widen_bytes<F32>(c.z, c.w) : widen_bytes<F32>(c.x, c.y);
+                    f = (d & 1) ? widen_bytes(c.z, c.w) : widen_bytes(c.x, c.y);
                 } else {
                     const uint4 c = vc[n];
-                    f = (d & 2) ? widen_halves<F32>(c.z, c.w, (d & 1) * 4u) : widen_halves<F32>(c.x, c.y, (d & 1) * 4u);
+                    f = (d & 2) ? widen_halves(c.z, c.w, (d & 1) * 4u) : widen_halves(c.x, c.y, (d & 1) * 4u);
                 }
-                if constexpr (!F32)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) f.u[e] = fma_fp16(f.u[e], sc[e], b[e]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float4v& to = o[mt][n * 4 + d];
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, F32 ? ph[F32 ? mt : 0].h : pw[mt].h, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, ph[mt].h, to, 0, 0, 0);
                     if constexpr (F32) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, pl[mt].h, to, 0, 0, 0);
                 }
             }
         }
-        if constexpr (!F32) {
-            if (vnan) {  // rows that see a group of NaN, which was taken as 0
-                const uint32_t* raw = reinterpret_cast<const uint32_t*>(rec + 2u * PART);
+        if (vnan) {  // rows that see a group of NaN, which was taken as 0
+            const uint32_t* raw = reinterpret_cast<const uint32_t*>(rec + 2u * PART);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        float hit = 0.0f;
+                for (int n = 0; n < NG; ++n) {
+                    float hit = 0.0f;
 #pragma nounroll
-                        for (int j = 0; j < 8; ++j)
-                            if (((seen[mt] >> j) & 1u) && raw[(NG + n) * kKvBlock + (j >> 2) * 16 + g * 4 + (j & 3)] >= 0x7F800000u) hit = __builtin_nanf("");
-                        hit = rows_sum(hit);
+                    for (int j = 0; j < 8; ++j)
+                        if (((seen[mt] >> j) & 1u) && raw[(NG + n) * kKvBlock + (j >> 2) * 16 + g * 4 + (j & 3)] >= 0x7F800000u) hit = __builtin_nanf("");
+                    hit = rows_sum(hit);
 #pragma unroll
-                        for (int i = n * 4; i < n * 4 + 4; ++i)
+                    for (int i = n * 4; i < n * 4 + 4; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[mt][i][e] += hit;
-                    }
-            }
+                        for (int e = 0; e < 4; ++e) o[mt][i][e] += hit;
+                }
         }
         blk = next;
         page = next_page;
@@ -670,9 +621,6 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         l[mt] = rows_sum(l[mt]);
-        if constexpr (F32)
-#pragma unroll
-            for (int n = 0; n < NG; ++n) obias[mt][n] = rows_sum(obias[mt][n]);
         if (!live[mt]) m[mt] = kNegInf, l[mt] = 0.0f;
         if (row[mt].over) m[mt] = 0.0f, l[mt] = __builtin_nanf("");
         if (g == 0u) sh.m[wave][mt * 16 + lane] = m[mt], sh.l[wave][mt * 16 + lane] = l[mt];
@@ -704,14 +652,22 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
         if (n) __syncthreads();
+        float centre[MT];  // of group n
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            centre[mt] = oc[mt][NG < 4 ? n : n & 3];
+            if constexpr (NG == 8) {
+                const float across = __shfl_xor(centre[mt], 16);
+                if ((g & 1u) != (uint32_t)n / 4u) centre[mt] = across;
+            }
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = own[mt] != 0.0f ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], vexp) + (F32 ? obias[F32 ? mt : 0][F32 ? n : 0] : 0.0f)) : 0.0f;
+                for (int e = 0; e < 4; ++e) v[e] = own[mt] != 0.0f ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], vexp) + centre[mt]) : 0.0f;
                 *reinterpret_cast<float4*>(&sh.sums[wave][mt * 16 + (lane & 15u)][d * 16 + g * 4]) = make_float4(v[0], v[1], v[2], v[3]);
             }
         __syncthreads();
