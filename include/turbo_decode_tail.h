@@ -446,7 +446,8 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * The prefix is read once for the whole batch: its products run over the rows of all sequences (a
  * sequence that fills the products' tiles by itself takes it along with its own tokens). Products
  * accumulate in FP32. Keys and values enter as the cache holds them. For FP32 queries, queries and softmax
- * weights keep 22 bits; for BF16 ones the weights keep 11.
+ * weights keep 22 bits; for BF16 ones the weights keep 11; the smallest weighted values 2^-32 of the largest that
+ * the row weights. Tokens that a query does not see have no part in its result.
  */
 typedef struct {
     int batch;                   /* >= 0 */

@@ -137,3 +137,49 @@ def test_large_scores_of_nearly_equal_keys(dtype, dim, bits):
     q = L.bf16(40.0 * queries(rng, 1, 16, dim, "f32"))
     out = attend(s, q, 16, [128], dtype)
     hold(s, q, out, [128], 1, 0, dtype, dim**-0.5)
+
+
+OUTLIERS = {  # prefix, own tokens, q_len, window, the token that dwarfs all others, group, max_kv_len
+    "later_queries_see_it": (0, [200], 64, 0, 170, 1, None),
+    "left_behind_by_the_window": (0, [900], 24, 400, 484, 2, 1),
+    "in_the_window_of_the_first_query": (0, [900], 24, 400, 477, 3, 1),
+    "in_a_prefix_part_of_the_batch_reaches": (300, [10, 0, 0, 40], 1, 0, 130, 4, None),
+    "first_of_all_and_weightless": (0, [600], 3, 0, 0, 2, 1),
+    "weightless_in_a_prefix": (500, [1, 90, 7], 2, 0, 41, 2, None),
+}
+
+
+@pytest.mark.parametrize("case", list(OUTLIERS))
+@pytest.mark.parametrize("ratio", [2.0**14, 2.0**20, 2.0**30, 2.0**70])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 8), (512, 4)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_value_that_a_row_does_not_weight_costs_it_nothing(dtype, dim, bits, ratio, case):
+    prefix, own, q_len, window, at, group, most = OUTLIERS[case]
+    rng = np.random.default_rng(dim + len(case))
+    s = Setup(rng, 1, dim, bits, 32, prefix, own)
+    kv_len = [prefix + n for n in own] if "part" not in case else [310, 120, 60, 340]
+    base = rng.standard_normal(dim).astype(np.float32)
+    rows = len(kv_len) * q_len
+    q = 0.5 * queries(rng, rows, group, dim, "f32") + base
+    q = L.bf16(q)
+    scale = dim**-0.5
+    s.v[at] *= np.float32(ratio)
+    if "weightless" in case:
+        s.k[at] = -20.0 * base * 16.0 / np.sqrt(dim)
+    s.write(np.array([at]))
+    out = attend(s, q, group, kv_len, dtype, q_len=q_len, window=window, max_kv_len=most)
+    hold(s, q, out, kv_len, q_len, window, dtype, scale)
+
+
+@pytest.mark.parametrize("dim,bits", [(64, 4), (128, 8), (256, 4), (512, 8)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_small_groups_beside_large_ones(dtype, dim, bits):
+    """Groups of 64 whose keys and values differ by up to 2^8 inside a token, tokens by 2^20."""
+    rng = np.random.default_rng(5)
+    s = Setup(rng, 2, dim, bits, 64, 100, [90, 33])
+    by = 2.0 ** rng.uniform(-4, 4, (1, 1, dim // 64)).repeat(64, axis=2) * 2.0 ** rng.uniform(-10, 10, (223, 1, 1))
+    s.v = (s.v * by).astype(np.float32)
+    s.write(np.arange(223))
+    q = L.bf16(queries(rng, 2, 6, dim, "f32"))
+    out = attend(s, q, 6, [190, 133], dtype)
+    hold(s, q, out, [190, 133], 1, 0, dtype, dim**-0.5)

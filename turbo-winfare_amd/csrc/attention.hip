@@ -112,6 +112,9 @@ __device__ inline float centre_of(uint32_t w) {
     return fmaf(BITS == 8u ? 128.0f : 8.0f, scale_of(w), __uint_as_float(w << 16));
 }
 
+// floor(log2(x)) of a number that is not negative (-127 below 2^-126)
+__device__ inline float power_of(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
+
 // Two numbers rounded to fp16, and back. The packed word is opaque to the compiler: it would otherwise
 // round a product anew for each use, once from FP32 and once, fused with the product, from the exact
 // value, and what is left of a number after its first part would miss a step near a tie.
@@ -220,17 +223,25 @@ struct Shared {
         float sums[kWaves][16 * MT][kRow];
     };
     float m[kWaves][16 * MT], l[kWaves][16 * MT], factor[16 * MT];
+    int lo[16 * MT], hi[16 * MT];           // what the rows see, read where a record is not seen whole
     float qsum[16 * MT][NG + 1];  // of a row's groups
 };
 
 template <int NG, uint32_t BITS, bool F32, int MT>
 __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32, MT>& sh) {
     constexpr int KU = BITS == 8u ? 2 : 1;       // 16-byte loads per group of keys or values
-    constexpr bool kEarly = NG * MT <= 4;        // registers hold a record's keys and values at once
-    // A row's weights are relative to m, its running maximum less kLift, which is left alone while they stay
-    // below 2^(kLift + kSlack): of 16 rows one has a new maximum in most records, and the sums would be
-    // rescaled there. Lifted, small ones stay normal numbers in fp16.
-    constexpr float kLift = F32 ? 0.0f : 8.0f, kSlack = 7.0f;
+    // Registers hold a record's keys and values at once; otherwise the next keys are loaded when all but the last
+    // group's values are used. Earlier, two tiles of heads of 256 spill (64 sequences behind 32,768: 139 -> 186 us).
+    constexpr bool kEarly = NG * MT <= 4;
+    // A row's weights p are relative to m, a running maximum that is left alone while they stay below 2^kSlack:
+    // of 16 rows one has a new maximum in most records, and the sums would be rescaled there.
+    // The sums of weighted values are in units of 2^(m + u - kUnit). u is a whole number for each row: 2^u is at most
+    // the largest p * size that the row has met, a value's size being the larger of 128 scale and |centre| over its
+    // head, and u rises where a p * size could pass 2^(u + kRoom + 1). A weight times a scale is then below 2^15,
+    // and one that fp16 holds with fewer than 11 bits is off by 2^-32 of the row's largest weighted size. Tokens
+    // that a row does not see, or gives no weight, do not enter.
+    constexpr float kSlack = 7.0f, kRoom = 7.0f;
+    constexpr int kUnit = 14, kScaleUnit = 20;  // scales of values lie in LDS times 2^20, so that no power leaves FP32
     constexpr uint32_t D = NG * 64u, PART = NG * 64u * kKvBlock * BITS / 8u;
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -312,23 +323,24 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             if (g == 0u) sh.qsum[mt * 16 + lane][n] = sum;
         }
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        if (threadIdx.x < 16u) sh.lo[mt * 16 + lane] = row[mt].lo, sh.hi[mt * 16 + lane] = row[mt].hi;
     __syncthreads();
     // the groups' sums as the FP32 products' second operand: that of group 4 h + lane / 16
     constexpr int kFours = NG > 4 ? NG / 4 : 1;
-    float factor[MT], qsum[MT][kFours];
+    float qsum[MT][kFours];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        factor[mt] = sh.factor[mt * 16 + (lane & 15u)];
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int h = 0; h < kFours; ++h) qsum[mt][h] = g < (uint32_t)NG ? sh.qsum[mt * 16 + (lane & 15u)][min(4u * h + g, NG - 1u)] : 0.0f;
-    }
 
     float4v o[MT][NG * 4];
     float4v oc[MT];  // the centres' sums, rows of the product: element e of lane / 16 is group (4 (lane / 16) + e) mod NG
-    float m[MT], l[MT];
+    float m[MT], l[MT], u[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt] = kNegInf, l[mt] = 0.0f, oc[mt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        m[mt] = kNegInf, l[mt] = 0.0f, u[mt] = -119.0f, oc[mt] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NG * 4; ++i) o[mt][i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -370,10 +382,9 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     };
     float *scales = sh.scale[wave], *centres = sh.centre[wave];
 
-    // A record's scales and centres. Words of keys that no row sees become 0, as do a value's of NaN. The values'
-    // power of two, 2^(e + kTop) above the largest scale, is that of the sums and never falls.
-    constexpr int kTop = F32 ? 8 : 0;
-    int vexp = -1000;
+    // A record's scales and centres, and the power of two of its largest value's size. Words of keys that no row
+    // sees become 0, as do a value's of NaN.
+    float largest = 0.0f;
     bool vnan = false;
     auto prepare = [&](int base, int end) {
         end = min(end, hi_max);
@@ -391,35 +402,24 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         vnan = false;
         if (__any(lane >= 32u && top >= 0x7F800000u)) {
             asm volatile("");
-            top = 0u;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
+            for (int i = 0; i < NG; ++i)
                 if (lane >= 32u && sw[i] >= 0x7F800000u) sw[i] = 0u, vnan = true;
-                top = max(top, sw[i]);
-            }
             vnan = __any(vnan);
         }
-        top = max(top, dpp_mov<dpp::kXor1>(top));
-        top = max(top, dpp_mov<dpp::kXor2>(top));
-        top = max(top, dpp_mov<dpp::kRor4>(top));
-        top = max(top, dpp_mov<dpp::kRor8>(top));
-        const int vt = (int)(max(lane_read(top, 32), lane_read(top, 48)) >> 23);
-        const int want = uniform(min(max(vt - 126 - kTop, -120), 113));
-        if (want > vexp) {
-            if (vexp > -1000) {
+        float sc[NG], ce[NG], size = 0.0f;
+        const float by = lane < 32u ? 1.0f : (float)(1 << kScaleUnit);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < NG * 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[mt][i][e] = ldexpf(o[mt][i][e], vexp - want);
-            }
-            vexp = want;
+        for (int i = 0; i < NG; ++i) {
+            sc[i] = scale_of(sw[i]), ce[i] = centre_of<BITS>(sw[i]);
+            size = fmaxf(size, fmaxf(128.0f * sc[i], fabsf(ce[i])));
+            sc[i] *= by;
         }
-        float sc[NG], ce[NG];
-        const float unit = lane < 32u ? 1.0f : __uint_as_float((uint32_t)(127 - vexp) << 23);
-#pragma unroll
-        for (int i = 0; i < NG; ++i) sc[i] = scale_of(sw[i]) * unit, ce[i] = centre_of<BITS>(sw[i]);
+        size = fmaxf(size, dpp_mov<dpp::kXor1>(size));
+        size = fmaxf(size, dpp_mov<dpp::kXor2>(size));
+        size = fmaxf(size, dpp_mov<dpp::kRor4>(size));
+        size = fmaxf(size, dpp_mov<dpp::kRor8>(size));
+        largest = power_of(fmaxf(lane_read(size, 32), lane_read(size, 48)));
         auto put = [&](float* to, const float (&x)[NG]) {
             if constexpr (NG == 1) to[lane] = x[0];
             if constexpr (NG == 2) *reinterpret_cast<float2*>(to + lane * 2u) = make_float2(x[0], x[1]);
@@ -501,28 +501,27 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!kEarly) load_values(rec);
         const uint8_t* next_rec = rec;
-        if (next < s1) {
-            next_rec = record_at(next, next_page);
-            load_keys(next_rec);
+        if (next < s1) next_rec = record_at(next, next_page);
+        if constexpr (kEarly) {
+            if (next < s1) load_keys(next_rec);
         }
 
         // ---- weights
         const bool masked = base < lo_max || base + (int)kKvBlock > min(hi_min, end);
         float p[MT][8];
-        uint32_t seen[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             // The factor may leave FP32 (small queries, a large scale): a score of 0 stays 0, and a hidden key's
             // -infinity is set after the product, which would make it NaN.
-            seen[mt] = 0xFFu;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3] * factor[mt];
+            for (int j = 0; j < 8; ++j) p[mt][j] = s[mt][j >> 2][j & 3] * sh.factor[mt * 16 + (lane & 15u)];
             if (bad || masked) {
                 asm volatile("");
+                const int lo = sh.lo[mt * 16 + (lane & 15u)], hi = min(sh.hi[mt * 16 + (lane & 15u)], end);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = base + (j >> 2) * 16 + (int)g * 4 + (j & 3);
-                    if (key < row[mt].lo || key >= min(row[mt].hi, end)) p[mt][j] = kNegInf, seen[mt] &= ~(1u << j);
+                    if (key < lo || key >= hi) p[mt][j] = kNegInf;
                     else if (bad) p[mt][j] = __builtin_nanf("");
                 }
             }
@@ -530,21 +529,42 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, p[mt][j]);
             top = rows_max(top);
-            // the difference that the exponential takes: at large scores m + kLift + kSlack would round
-            if (__any(top - m[mt] > kLift + kSlack)) {
-                top = top - m[mt] > kLift + kSlack ? top - (top - (top - kLift) > kLift + kSlack ? 0.0f : kLift) : m[mt];
-                const float alpha = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[mt] - top);
-                l[mt] *= alpha;
+            // the differences that the exponential takes: a sum of m and a bound would round at large scores
+            const float rise = top - m[mt];
+            if (__any(rise > kSlack || rise + largest > u[mt] + kRoom)) {  // a bound; the row's own is found here
+                asm volatile("");
+                if (rise > kSlack) m[mt] = top;
+                const float by = rise > kSlack ? rise : 0.0f;
+                float need = kNegInf;
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    float4 size = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma nounroll
+                    for (int n = NG; n < 2 * NG; ++n) {
+                        constexpr float by = 128.0f / (1 << kScaleUnit);
+                        const uint32_t at = n * kKvBlock + tile * 16u + g * 4u;
+                        const float4 sc = *reinterpret_cast<const float4*>(scales + at), ce = *reinterpret_cast<const float4*>(centres + at);
+                        size.x = fmaxf(size.x, fmaxf(by * sc.x, fabsf(ce.x))), size.y = fmaxf(size.y, fmaxf(by * sc.y, fabsf(ce.y)));
+                        size.z = fmaxf(size.z, fmaxf(by * sc.z, fabsf(ce.z))), size.w = fmaxf(size.w, fmaxf(by * sc.w, fabsf(ce.w)));
+                    }
+                    const float s4[4] = {size.x, size.y, size.z, size.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) need = fmaxf(need, p[mt][tile * 4 + j] - m[mt] + power_of(s4[j]));
+                }
+                need = fmaxf(fmaxf(floorf(rows_max(need)), floorf(u[mt] - by)), -119.0f);
+                const float alpha = __builtin_amdgcn_exp2f(u[mt] - need - by);
+                l[mt] *= __builtin_amdgcn_exp2f(-by);
                 oc[mt] *= alpha;
 #pragma unroll
                 for (int i = 0; i < NG * 4; ++i) o[mt][i] *= alpha;
-                m[mt] = top;
+                u[mt] = need;
             }
-            const float zero = m[mt] == kNegInf ? 0.0f : m[mt];
+            const float zero = m[mt] == kNegInf ? 0.0f : m[mt], unit = ldexpf(1.0f, kUnit - kScaleUnit - (int)u[mt]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 p[mt][j] = __builtin_amdgcn_exp2f(p[mt][j] - zero);
                 l[mt] += p[mt][j];
+                p[mt][j] *= unit;
             }
         }
 
@@ -563,6 +583,17 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             const float* sn = scales + (NG + n) * kKvBlock + g * 4u;
             const float4 sa = *reinterpret_cast<const float4*>(sn), sb = *reinterpret_cast<const float4*>(sn + 16u);
             const float s8[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+            if constexpr (!kEarly)
+                if (n == NG - 1) {
+                    if (next < s1) {
+                        load_keys(next_rec);
+                    } else {  // the old ones end here: kept alive for a loop that is over, they cost their registers
+#pragma unroll
+                        for (int i = 0; i < NG * KU; ++i) kc[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                        for (int i = 0; i < NG; ++i) sw[i] = 0u;
+                    }
+                }
             Frag ph[MT], pl[F32 ? MT : 1];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -601,9 +632,12 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
                     float hit = 0.0f;
+                    const int lo = sh.lo[mt * 16 + (lane & 15u)], hi = min(sh.hi[mt * 16 + (lane & 15u)], end);
 #pragma nounroll
-                    for (int j = 0; j < 8; ++j)
-                        if (((seen[mt] >> j) & 1u) && raw[(NG + n) * kKvBlock + (j >> 2) * 16 + g * 4 + (j & 3)] >= 0x7F800000u) hit = __builtin_nanf("");
+                    for (int j = 0; j < 8; ++j) {
+                        const int in = (j >> 2) * 16 + (int)g * 4 + (j & 3);
+                        if (base + in >= lo && base + in < hi && raw[(NG + n) * kKvBlock + in] >= 0x7F800000u) hit = __builtin_nanf("");
+                    }
                     hit = rows_sum(hit);
 #pragma unroll
                     for (int i = n * 4; i < n * 4 + 4; ++i)
@@ -660,6 +694,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 const float across = __shfl_xor(centre[mt], 16);
                 if ((g & 1u) != (uint32_t)n / 4u) centre[mt] = across;
             }
+            centre[mt] = ldexpf(centre[mt], (int)u[mt] + kScaleUnit - kUnit);
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -667,7 +702,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             for (int d = 0; d < 4; ++d) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = own[mt] != 0.0f ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], vexp) + centre[mt]) : 0.0f;
+                for (int e = 0; e < 4; ++e) v[e] = own[mt] != 0.0f ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], (int)u[mt] - kUnit) + centre[mt]) : 0.0f;
                 *reinterpret_cast<float4*>(&sh.sums[wave][mt * 16 + (lane & 15u)][d * 16 + g * 4]) = make_float4(v[0], v[1], v[2], v[3]);
             }
         __syncthreads();
