@@ -183,3 +183,20 @@ def test_small_groups_beside_large_ones(dtype, dim, bits):
     q = L.bf16(queries(rng, 2, 6, dim, "f32"))
     out = attend(s, q, 6, [190, 133], dtype)
     hold(s, q, out, [190, 133], 1, 0, dtype, dim**-0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nan_with_a_weight_of_zero_is_nan(dtype):
+    """Wherever the token lies: in the record of the row's largest scores or far from them."""
+    rng = np.random.default_rng(8)
+    for own in (64, 600):
+        s = Setup(rng, 1, 64, 8, 32, 0, [own])
+        base = rng.standard_normal(64).astype(np.float32)
+        base *= np.float32(20.0 / np.linalg.norm(base))
+        s.k[:] = L.bf16(base)
+        s.k[32:64] = L.bf16(-base)
+        s.v[40] = np.nan
+        s.write(np.arange(own))
+        q = L.bf16(np.tile(base, (1, 2, 1)).astype(np.float32))
+        out = attend(s, q, 2, [own], dtype, scale=1.0)
+        assert torch.isnan(out).all(), own

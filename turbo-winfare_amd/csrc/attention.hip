@@ -661,11 +661,13 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     }
     __syncthreads();
     float own[MT];
+    bool counts[MT];  // also with a factor of 0, against which NaN stays NaN
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const uint32_t r = mt * 16u + (lane & 15u);
         const float top = fmaxf(fmaxf(sh.m[0][r], sh.m[1][r]), fmaxf(sh.m[2][r], sh.m[3][r]));
-        own[mt] = live[mt] && top != kNegInf ? __builtin_amdgcn_exp2f(m[mt] - top) : 0.0f;
+        counts[mt] = live[mt] && top != kNegInf;
+        own[mt] = counts[mt] ? __builtin_amdgcn_exp2f(m[mt] - top) : 0.0f;
     }
     // thread tid writes 4 values of row tid / 16 (and 16 + that); these are that row's
     const uint32_t out_row = threadIdx.x >> 4, col = (threadIdx.x & 15u) * 4u;
@@ -702,7 +704,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
             for (int d = 0; d < 4; ++d) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = own[mt] != 0.0f ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], (int)u[mt] - kUnit) + centre[mt]) : 0.0f;
+                for (int e = 0; e < 4; ++e) v[e] = counts[mt] ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], (int)u[mt] - kUnit) + centre[mt]) : 0.0f;
                 *reinterpret_cast<float4*>(&sh.sums[wave][mt * 16 + (lane & 15u)][d * 16 + g * 4]) = make_float4(v[0], v[1], v[2], v[3]);
             }
         __syncthreads();
