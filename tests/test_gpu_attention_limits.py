@@ -200,3 +200,19 @@ def test_nan_with_a_weight_of_zero_is_nan(dtype):
         q = L.bf16(np.tile(base, (1, 2, 1)).astype(np.float32))
         out = attend(s, q, 2, [own], dtype, scale=1.0)
         assert torch.isnan(out).all(), own
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_query_with_an_infinity_gives_nan(dtype, sign):
+    """Also where every key makes its score -inf, and in no other row."""
+    rng = np.random.default_rng(7)
+    s = Setup(rng, 1, 64, 8, 32, 0, [70])
+    s.k[:, 0, 5] = -np.abs(s.k[:, 0, 5]) - 2.0
+    s.write(np.arange(70))
+    q = queries(rng, 3, 2, 64, dtype)
+    q[1, 1, 5] = sign * np.inf
+    out = attend(s, q, 2, [70], dtype, q_len=3).float().cpu().numpy()
+    assert np.isnan(out[1, 1]).all()
+    out[1, 1] = 0.0
+    assert np.isfinite(out).all()

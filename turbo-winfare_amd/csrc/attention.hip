@@ -285,18 +285,20 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     for (int mt = 0; mt < MT; ++mt) {
         if (mt != (int)wave % MT) continue;
         const uint64_t at = row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + g * 16u;
-        float x[NG][2][8], top = 0.0f;
+        float x[NG][2][8], top = 0.0f, bad = 0.0f;
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 load_q8<F32>(a.q, at + n * 64u + c * 8u, x[n][c]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][c][i]));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][c][i])), bad = fmaf(x[n][c][i], 0.0f, bad);
             }
         top = rows_max(top);
+        bad = rows_sum(bad);  // NaN where a value is infinite or NaN: so is the row then, whatever its scores' signs
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), -shift), 0x1.fffffep127f);
+        const float factor = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), -shift), 0x1.fffffep127f);
+        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = factor + bad;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if (n % kSharers != (int)wave / MT) continue;
