@@ -1,0 +1,52 @@
+"""Rotation at the ends of its ranges: elements and pairs that stay as they are, positions up to 2^32,
+heads whose squares leave FP32."""
+import numpy as np
+import pytest
+
+import layer_util as L
+import turbo_decode_tail as T
+from test_gpu_layer_cache import code, ids, tensor
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def turned(r, x, pos, dtype="f32"):
+    xt = tensor(x, dtype)
+    out = torch.empty_like(xt)
+    r.apply(r.make_inputs(x.shape[0], dtype=code(dtype), q=xt, q_heads=x.shape[1], positions=ids(pos), q_out=out))
+    return out.float().cpu().numpy()
+
+
+@pytest.mark.parametrize("dim,rotary", [(64, 32), (128, 16), (256, 128), (512, 64)])
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_elements_past_the_rotation_pass_as_they_are(dtype, pairs, dim, rotary):
+    """Infinities and NaN among them too, and their neighbours."""
+    rng = np.random.default_rng(1)
+    x = L.bf16(rng.standard_normal((5, 3, dim)).astype(np.float32))
+    x[0, 0, rotary], x[1, 1, dim - 1], x[2, 2, rotary + 9], x[3, 0, rotary + 4] = np.inf, -np.inf, np.nan, -0.0
+    r = T.Rotary(dim, rotary_dim=rotary, layout=int(pairs), norms=0)
+    got = turned(r, x, np.arange(5) * 1000 + 7, dtype)
+    assert np.array_equal(got[..., rotary:].view(np.uint32) << 1 >> 23, x[..., rotary:].view(np.uint32) << 1 >> 23)  # NaN too
+    same = ~np.isnan(x[..., rotary:])
+    assert np.array_equal(got[..., rotary:][same].view(np.uint32), x[..., rotary:][same].view(np.uint32))
+    assert np.isfinite(got[..., :rotary]).all()
+
+
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pairs_of_frequency_zero_stay_as_they_are(dtype, pairs):
+    rng = np.random.default_rng(2)
+    dim = 128
+    f = rng.uniform(0.1, 2, dim // 2)
+    f[::5] = 0.0
+    x = L.bf16(rng.standard_normal((4, 2, dim)).astype(np.float32))
+    first = (np.arange(0, 64, 5) * 2) if pairs else np.arange(0, 64, 5)
+    second = first + 1 if pairs else first + 64
+    x[1, 0, first], x[2, 1, second] = np.inf, -np.inf
+    r = T.Rotary(dim, inv_freq=f, layout=int(pairs), norms=0)
+    got = turned(r, x, np.array([0, 5, 10**9, 2**32 - 1], np.uint32), dtype)
+    still = np.concatenate([first, second])
+    assert np.array_equal(got[..., still].view(np.uint32), x[..., still].view(np.uint32))
+    assert np.isfinite(np.delete(got, still, axis=2)).all()

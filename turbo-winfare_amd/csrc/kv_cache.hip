@@ -309,6 +309,7 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
 #pragma unroll
     for (int i = 0; i < E; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
     uint32_t angles = 0xFFFFFFFFu;  // the token whose sines are held
+    bool still = false;             // some turning lane of the wave has a pair that does not turn
     while (at.more()) {
         const Walk now = at;
         float x[E];
@@ -328,6 +329,10 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
                     }
                 }
             }
+            bool none = false;
+#pragma unroll
+            for (int i = 0; i < E; ++i) none = none || (sn[i] == 0.0f && !(a.pairs && (i & 1)));
+            still = __any(turning && none);
         }
         const bool here = now.h + sub < heads;
         const uint32_t t = now.t, head = h0 + min(now.h + sub, heads - 1u);
@@ -341,20 +346,30 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
             for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[i];
         }
         if (rot) {
+            // what does not turn stays as it is: a product with a sine of 0 would make NaN of infinities
+            float y[E], z[E];
             if (a.pairs) {
 #pragma unroll
                 for (int i = 0; i < E; i += 2) {
-                    const float p = x[i], q = x[i + 1];
-                    x[i] = p * cs[i] - q * sn[i];
-                    x[i + 1] = q * cs[i] + p * sn[i];
+                    y[i] = x[i] * cs[i] - x[i + 1] * sn[i];
+                    y[i + 1] = x[i + 1] * cs[i] + x[i] * sn[i];
                 }
             } else {
-                float y[E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) y[i] = __shfl(x[i], (int)other);
+                for (int i = 0; i < E; ++i) z[i] = __shfl(x[i], (int)other);
 #pragma unroll
-                for (int i = 0; i < E; ++i) x[i] = first ? x[i] * cs[i] - y[i] * sn[i] : x[i] * cs[i] + y[i] * sn[i];
+                for (int i = 0; i < E; ++i) y[i] = first ? x[i] * cs[i] - z[i] * sn[i] : x[i] * cs[i] + z[i] * sn[i];
             }
+            if (still) {
+                asm volatile("");
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const int at = a.pairs ? i & ~1 : i;
+                    if (sn[at] == 0.0f && cs[at] == 1.0f) y[i] = x[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = turning ? y[i] : x[i];
         }
         if (dst && here) Vec<T, E>::store(dst + (uint64_t)(t0 + t) * out_stride + (head * D + d0), x);
         if constexpr (BITS != 0u) {
