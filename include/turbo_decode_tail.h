@@ -387,7 +387,8 @@ enum { TURBO_NORM_Q = 1u, TURBO_NORM_K = 2u, TURBO_NORM_V = 4u };
  * the weight where there is one (plain w, as norm_weight of TurboLMHeadDesc; values have none). Then
  * pair i < rotary_dim / 2 of a query or key at position p turns by p * theta^(-2 i / rotary_dim)
  * radians, or p * inv_freq[i] where inv_freq is given (0 leaves a pair as it is); the other elements
- * pass. The angle is exact to 2^-32 turns for every position below 2^32.
+ * pass as they are. The angle is within 2^-31 turns of that at every position below 2^32 (a frequency f above 1:
+ * f times that).
  */
 typedef struct {
     uint32_t head_dim;

@@ -1,5 +1,7 @@
 """Rotation at the ends of its ranges: elements and pairs that stay as they are, positions up to 2^32,
 heads whose squares leave FP32."""
+from decimal import Decimal, getcontext
+
 import numpy as np
 import pytest
 
@@ -50,3 +52,26 @@ def test_pairs_of_frequency_zero_stay_as_they_are(dtype, pairs):
     still = np.concatenate([first, second])
     assert np.array_equal(got[..., still].view(np.uint32), x[..., still].view(np.uint32))
     assert np.isfinite(np.delete(got, still, axis=2)).all()
+
+
+@pytest.mark.parametrize("theta", [1e4, 5e5, 1e6])
+def test_angles_of_far_positions(theta):
+    """(1, 0) turned is (cos, sin). The angle is within 2^-31 turns of position * theta^(-2 i / R), in
+    decimal arithmetic of 60 digits; sine and cosine add 4 roundings of themselves."""
+    getcontext().prec = 60
+    two_pi = Decimal("6.28318530717958647692528676655900576839433879875021164194988918")
+    rng = np.random.default_rng(3)
+    dim, n = 64, 400
+    pos = rng.integers(2**32 - 2**30, 2**32, n, dtype=np.uint64).astype(np.uint32)
+    pos[0] = 2**32 - 1
+    x = np.zeros((n, 1, dim), np.float32)
+    x[..., :dim // 2] = 1.0
+    got = turned(T.Rotary(dim, theta=theta, norms=0), x, pos)[:, 0].astype(np.float64)
+    turn = np.empty((n, dim // 2))
+    for i in range(dim // 2):
+        per = Decimal(theta) ** (Decimal(-2 * i) / Decimal(dim)) / two_pi
+        turn[:, i] = [float((int(p) * per) % 1) for p in pos]
+    angle = 2 * np.pi * turn
+    want = np.concatenate([np.cos(angle), np.sin(angle)], axis=1)
+    bound = 2 * np.pi * 2.0**-31 + 4 * 2.0**-24 * np.abs(want)
+    assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / bound).max())

@@ -290,9 +290,10 @@ TURBO_DT_API void* turbo_rotary_create(const TurboRotaryDesc* desc) {
     // turns per position, modulo one turn, in 64-bit fixed point
     std::vector<uint64_t> turns(rd / 2u);
     for (uint32_t i = 0; i < rd / 2u; ++i) {
-        const double f = desc->inv_freq ? desc->inv_freq[i] : std::pow(desc->theta, -2.0 * i / rd);
+        // 64 bits throughout: a power rounded to double would be off by 2^-25 turns at position 2^32
+        const long double f = desc->inv_freq ? (long double)desc->inv_freq[i] : std::pow((long double)desc->theta, -2.0L * i / rd);
         if (!std::isfinite(f)) fail("inv_freq[" + std::to_string(i) + "] is not finite");
-        long double t = (long double)f / 6.283185307179586476925286766559L;
+        long double t = f / 6.283185307179586476925286766559L;
         t -= std::floor(t);
         t = std::ldexp(t, 64);
         turns[i] = t >= 18446744073709551615.0L ? 0u : (uint64_t)(t + 0.5L);
