@@ -86,6 +86,7 @@ struct QkvArgs {
     const uint64_t* turns;             // [rotary_dim / 2] turns per position, 64-bit fixed point
     uint32_t tokens, q_heads, kv_heads, rotary_dim;
     int pairs;                         // 0: halves
+    int still;                         // some frequency is 0
     uint32_t norms;                    // TURBO_NORM_*
     float eps;
     KvView kv;

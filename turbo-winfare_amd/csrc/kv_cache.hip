@@ -303,13 +303,13 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
     }
     // the lane with the other values of this lane's pairs (halves), and the sign of their sines
     const bool turning = d0 < rot, first = d0 < half;
+    const bool still = a.still || rot % E != 0u;  // pairs that do not turn lie in turning lanes
     const uint32_t other = !turning || a.pairs ? lane : first ? lane + half / E : lane - half / E;
 
     float cs[E], sn[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
     uint32_t angles = 0xFFFFFFFFu;  // the token whose sines are held
-    bool still = false;             // some turning lane of the wave has a pair that does not turn
     while (at.more()) {
         const Walk now = at;
         float x[E];
@@ -329,10 +329,6 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
                     }
                 }
             }
-            bool none = false;
-#pragma unroll
-            for (int i = 0; i < E; ++i) none = none || (sn[i] == 0.0f && !(a.pairs && (i & 1)));
-            still = __any(turning && none);
         }
         const bool here = now.h + sub < heads;
         const uint32_t t = now.t, head = h0 + min(now.h + sub, heads - 1u);

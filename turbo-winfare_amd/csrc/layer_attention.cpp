@@ -51,6 +51,7 @@ struct RotaryBox {
     int device = 0;
     uint32_t head_dim = 0, rotary_dim = 0, norms = 0;
     int layout = 0;
+    bool still = false;  // some frequency is 0
     float eps = 0.f;
     uint16_t *q_norm = nullptr, *k_norm = nullptr;
     uint64_t* turns = nullptr;
@@ -308,6 +309,7 @@ TURBO_DT_API void* turbo_rotary_create(const TurboRotaryDesc* desc) {
     r->head_dim = desc->head_dim;
     r->rotary_dim = rd;
     r->layout = desc->layout;
+    for (uint64_t t : turns) r->still = r->still || t == 0u;
     r->norms = desc->norms;
     r->eps = desc->eps;
     const hipMemcpyKind kind = desc->weights_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
@@ -376,6 +378,7 @@ TURBO_DT_API int turbo_qk_norm_rope(void* handle, const TurboQkvInputs* in, void
     a.kv_heads = in->k ? (uint32_t)in->kv_heads : 0u;
     a.rotary_dim = r->rotary_dim;
     a.pairs = r->layout == TURBO_ROPE_PAIRS;
+    a.still = r->still;
     a.norms = r->norms;
     a.eps = r->eps;
     if (c) a.kv = c->kv;
