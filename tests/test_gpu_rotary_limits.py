@@ -75,3 +75,47 @@ def test_angles_of_far_positions(theta):
     want = np.concatenate([np.cos(angle), np.sin(angle)], axis=1)
     bound = 2 * np.pi * 2.0**-31 + 4 * 2.0**-24 * np.abs(want)
     assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / bound).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norms_of_heads_whose_squares_leave_the_type(dtype, dim):
+    """Heads of 1e-30 to 1e38 with eps 0, tokens of all sizes in one call: 14 roundings of the mean's terms and
+    sum, halved by the root, and 7 of root, division, powers of two and products."""
+    rng = np.random.default_rng(4)
+    size = np.array([1e-30, 1e-22, 1e-10, 1.0, 1e10, 1e19, 1e25, 1e37], np.float32)
+    x = (rng.uniform(0.1, 1, (8, 3, dim)) * rng.choice([-1, 1], (8, 3, dim)) * size[:, None, None]).astype(np.float32)
+    x[4, 1] *= np.float32(1e15)  # and of one call's heads
+    x = L.bf16(x) if dtype == "bf16" else x
+    r = T.Rotary(dim, rotary_dim=0, eps=0.0)
+    got = turned(r, x, np.zeros(8, np.uint32), dtype)
+    want = L.norm(x, 0.0)
+    bound = 14 * 2.0**-24 * np.abs(want)
+    bound += 2.0**-8 * (np.abs(want) + bound) if dtype == "bf16" else 0.0
+    assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) / bound).max())
+    plain = np.array(x)
+    plain[[0, 1, 5, 6, 7]], plain[4, 1] = 1.0, 1.0
+    pos = np.arange(5, 13)
+    for r in (r, T.Rotary(dim, eps=0.0), T.Rotary(dim, eps=0.0, rotary_dim=32, layout=T.TURBO_ROPE_PAIRS)):
+        got, again = turned(r, x, pos, dtype), turned(r, plain, pos, dtype)  # the same bits whatever stands beside them
+        assert np.array_equal(again[[2, 3]], got[[2, 3]]) and np.array_equal(again[4, [0, 2]], got[4, [0, 2]])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_normed_values_whose_squares_leave_the_type(bits):
+    rng = np.random.default_rng(5)
+    n, dim = 40, 128
+    size = (10.0 ** rng.uniform(-35, 37, (n, 1, 1))).astype(np.float32)
+    v = (rng.uniform(0.1, 1, (n, 2, dim)) * size).astype(np.float32)
+    vt, pt = tensor(v, "f32"), ids(np.arange(n))
+    cache = T.KvCache(2, 32, 2, dim, bits=bits)
+    r = T.Rotary(dim, rotary_dim=0, norms=T.TURBO_NORM_V, eps=0.0)
+    r.apply(r.make_inputs(n, k=torch.zeros_like(vt), v=vt, kv_heads=2, cache=cache, slots=pt))
+    back = torch.empty_like(vt)
+    cache.read(pt, n, None, back)
+    want = L.norm(v, 0.0)
+    # half a step of a range below 2 with its two roundings up, and the norm's 14 roundings
+    g = want.reshape(n, 2, -1, 64)
+    step = (g.max(-1) - g.min(-1) * (1 - 2.0**-7)) * (1 + 2.0**-7) / (2**bits - 1)
+    bound = 0.5 * np.repeat(step, 64, axis=-1).reshape(want.shape) * (1 + 2.0**-12) + 14 * 2.0**-24 * np.abs(want).max(-1, keepdims=True)
+    assert np.all(np.abs(back.cpu().numpy() - want) <= bound)

@@ -93,6 +93,32 @@ __device__ inline float lanes_reduce(float v, Op op) {
     return v;
 }
 
+// 1 / sqrt(mean(x^2) + eps) of a head that lies in D / E lanes. Where the squares leave FP32 (or eps is 0 and they
+// vanish), x is brought near 1 by a power of two first; the lanes of other heads get the bits that they get alone.
+template <uint32_t D, int E>
+__device__ inline float norm_factor(float (&x)[E], float eps) {
+    auto mean = [&](float e) {
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) sq = fmaf(x[i], x[i], sq);
+        return lanes_reduce<D / E>(sq, [](float p, float q) { return p + q; }) * (1.0f / D) + e;
+    };
+    float m = mean(eps);
+    const bool out = !(m > 0x1p-100f && m < 0x1p127f);
+    if (__any(out)) {
+        asm volatile("");
+        float top = sqrtf(eps);
+#pragma unroll
+        for (int i = 0; i < E; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = lanes_reduce<D / E>(top, [](float p, float q) { return fmaxf(p, q); });
+        const int by = out ? 127 - (int)(__float_as_uint(top) >> 23) : 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = ldexpf(x[i], by);
+        m = mean(ldexpf(eps, 2 * by));
+    }
+    return 1.0f / sqrtf(m);
+}
+
 // cos and sin of `turn` / 2^32 turns
 __device__ inline void turn_cos_sin(uint32_t turn, float& c, float& s) {
     const uint32_t quadrant = (turn + 0x20000000u) >> 30;
@@ -333,11 +359,7 @@ __device__ inline void turn_heads(const QkvArgs& a, const Division& v, uint32_t 
         const bool here = now.h + sub < heads;
         const uint32_t t = now.t, head = h0 + min(now.h + sub, heads - 1u);
         if (normed) {
-            float sq = 0.0f;
-#pragma unroll
-            for (int i = 0; i < E; ++i) sq = fmaf(x[i], x[i], sq);
-            sq = lanes_reduce<LPH>(sq, [](float p, float q) { return p + q; });
-            const float r = 1.0f / sqrtf(sq * (1.0f / D) + a.eps);
+            const float r = norm_factor<D, E>(x, a.eps);
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] = x[i] * r * w[i];
         }
@@ -416,11 +438,7 @@ __device__ inline void store_value_heads(const QkvArgs& a, const Division& v, ui
         at.next();
         if (at.more()) next.load(from(at));
         if (normed) {
-            float sq = 0.0f;
-#pragma unroll
-            for (int i = 0; i < E; ++i) sq = fmaf(x[i], x[i], sq);
-            sq = lanes_reduce<LPH>(sq, [](float p, float q) { return p + q; });
-            const float r = 1.0f / sqrtf(sq * (1.0f / D) + a.eps);
+            const float r = norm_factor<D, E>(x, a.eps);
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] *= r;
         }
