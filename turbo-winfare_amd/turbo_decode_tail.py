@@ -558,6 +558,16 @@ def _stride(t) -> int:
     return t.stride(0)
 
 
+def _ids(t) -> int | None:
+    """The address of device ids: a contiguous tensor of 32-bit integers, or a raw address."""
+    try:
+        if t is not None and (t.element_size() != 4 or t.is_floating_point() or not t.is_contiguous()):
+            raise ValueError("slots, positions, lengths and page tables must be contiguous 32-bit integers")
+    except AttributeError:
+        pass
+    return _ptr(t)
+
+
 class KvCache:
     """One turbo_kv_cache handle: a layer's keys and values in pages, quantised to 4 or 8 bits.
     Buffers are torch CUDA tensors [tokens][kv_heads][head_dim] or raw addresses (packed)."""
@@ -572,20 +582,22 @@ class KvCache:
 
     def write(self, k, v, slots, tokens: int, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
         """Quantises k and v of `tokens` tokens into slots (device ids; TURBO_NO_SLOT skips a token)."""
-        _ok(self.lib.turbo_kv_cache_write(self.h, _ptr(k), _stride(k), _ptr(v), _stride(v), dtype, _ptr(slots), tokens, stream))
+        _ok(self.lib.turbo_kv_cache_write(self.h, _ptr(k), _stride(k), _ptr(v), _stride(v), dtype,
+                                          _ids(slots), tokens, stream))
 
     def read(self, slots, tokens: int, k_out, v_out, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
         """k_out, v_out (either may be None) = the tokens at slots; NaN for a slot past the cache."""
-        _ok(self.lib.turbo_kv_cache_read(self.h, _ptr(slots), tokens, dtype, _ptr(k_out), _stride(k_out), _ptr(v_out),
+        _ok(self.lib.turbo_kv_cache_read(self.h, _ids(slots), tokens, dtype, _ptr(k_out), _stride(k_out), _ptr(v_out),
                                          _stride(v_out), stream))
 
     @staticmethod
     def make_attention_inputs(batch: int, *, dtype: int = TURBO_HIDDEN_F32, q, out, q_heads: int, q_len: int = 1, kv_len,
                               max_kv_len: int, pages=None, prefix_len: int = 0, prefix_pages=None, window: int = 0, scale: float,
                               workspace=None) -> TurboAttentionInputs:
-        """pages: [batch][page_stride] device ids. workspace: a uint8 tensor of attention_workspace(inputs) bytes."""
-        return TurboAttentionInputs(batch, q_len, q_heads, dtype, _ptr(q), _ptr(out), _stride(q), _stride(out), _ptr(kv_len),
-                                    max_kv_len, prefix_len, _ptr(prefix_pages) if prefix_len else None, _ptr(pages),
+        """pages: [batch][page_stride] device ids, whole rows (a slice of a wider table is copied first). workspace: a
+        uint8 tensor of attention_workspace(inputs) bytes."""
+        return TurboAttentionInputs(batch, q_len, q_heads, dtype, _ptr(q), _ptr(out), _stride(q), _stride(out),
+                                    _ids(kv_len), max_kv_len, prefix_len, _ids(prefix_pages) if prefix_len else None, _ids(pages),
                                     int(pages.shape[1]) if pages is not None else 0, window, scale, _ptr(workspace),
                                     workspace.numel() if workspace is not None else 0)
 
@@ -629,6 +641,9 @@ class Rotary:
         for w in weights:
             if len(w) != head_dim:
                 raise ValueError("a norm weight has head_dim values")
+            if (w.element_size() if d.weights_on_device else w.itemsize) != 2 or not (
+                    w.is_contiguous() if d.weights_on_device else w.flags.c_contiguous):
+                raise ValueError("a norm weight is contiguous BF16")
         hp = (lambda w: None if w is None else w.data_ptr()) if d.weights_on_device else (
             lambda w: None if w is None else w.ctypes.data)
         d.q_norm, d.k_norm = hp(q_norm), hp(k_norm)
@@ -645,9 +660,9 @@ class Rotary:
     @staticmethod
     def make_inputs(tokens: int, *, dtype: int = TURBO_HIDDEN_F32, q=None, k=None, v=None, q_heads: int = 0, kv_heads: int = 0,
                     positions=None, q_out=None, k_out=None, cache: KvCache | None = None, slots=None) -> TurboQkvInputs:
-        inp = TurboQkvInputs(tokens, dtype, q_heads, kv_heads, _ptr(q), _ptr(k), _ptr(v), _stride(q), _stride(k), _stride(v),
-                             _ptr(positions), _ptr(q_out), _ptr(k_out), _stride(q_out), _stride(k_out),
-                             cache.h if cache is not None else None, _ptr(slots))
+        inp = TurboQkvInputs(tokens, dtype, q_heads, kv_heads, _ptr(q), _ptr(k), _ptr(v), _stride(q), _stride(k),
+                             _stride(v), _ids(positions), _ptr(q_out), _ptr(k_out), _stride(q_out),
+                             _stride(k_out), cache.h if cache is not None else None, _ids(slots))
         return inp
 
     def apply(self, inp: TurboQkvInputs, stream=None) -> None:
