@@ -1,11 +1,12 @@
-"""The binding's view of the layer operators' buffers, without a GPU: tensors that a call would read at the wrong
-places are refused before any call."""
+"""The binding's view of the layer operators' buffers, without a GPU: strides of heads that are slices of wider
+rows, and tensors that a call would read at the wrong places, which are refused before any call."""
 import numpy as np
 import pytest
 
 import turbo_decode_tail as T
 
 torch = pytest.importorskip("torch")
+F32, BF16 = T.TURBO_HIDDEN_F32, T.TURBO_HIDDEN_BF16
 
 
 class Library:
@@ -22,6 +23,48 @@ def cache():
 
 def zeros(*shape, dtype=torch.float32):
     return torch.zeros(shape, dtype=dtype)
+
+
+def test_strides_of_slices():
+    wide = zeros(6, 10, 64)
+    assert T._stride(wide, F32) == 0 and T._stride(None, F32) == 0 and T._stride(12345, F32) == 0
+    assert T._stride(wide[:, 2:6], F32) == 640
+    assert T._stride(wide.bfloat16()[:, 2:6], BF16) == 640
+    assert T._stride(wide[:, 3:4], F32) == 640
+    assert T._stride(wide[::2], F32) == 1280                       # every other token
+    assert T._stride(wide.view(6, 640)[:, 64:192], F32) == 640     # heads and values in one dimension
+    assert T._stride(zeros(2, 3, 10, 64)[:, :, 1:5], F32) == 640   # [batch][q_len][heads][head_dim]
+    assert T._stride(zeros(1, 10, 64)[:, 1:5], F32) == 0           # one token: any stride
+    assert T._stride(zeros(2, 1, 10, 64)[:, :, 1:5], F32) == 640
+    assert T._stride(zeros(4, 1, 64).transpose(0, 1).contiguous().transpose(0, 1), F32) == 0
+
+
+@pytest.mark.parametrize("t,word", [
+    (zeros(6, 10, 64).transpose(0, 1), "contiguous"),              # heads outside tokens
+    (zeros(6, 10, 128)[:, :, :64], "contiguous"),                  # a gap between heads
+    (zeros(6, 10, 128)[:, :, ::2], "contiguous"),
+    (zeros(6, 1280)[:, ::2], "contiguous"),
+    (zeros(1280)[::2], "contiguous"),
+    (zeros(1, 4, 64).expand(6, 4, 64), "overlap"),                 # one token for all
+    (zeros(640).as_strided((6, 2, 64), (64, 64, 1)), "overlap"),
+    (zeros(4, 3, 10, 64)[:, :2], "one stride"),                    # two of three queries of each sequence
+    (zeros(3, 2, 10, 64).transpose(0, 1), "one stride"),
+])
+def test_refused_layouts(t, word):
+    with pytest.raises(ValueError, match=word):
+        T._stride(t, F32)
+
+
+def test_another_element_size_is_refused():
+    x, sl = zeros(4, 2, 64, dtype=torch.bfloat16), zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="element size"):
+        cache().write(x, x, sl, 4)  # dtype is FP32 unless given: the call would read past the end
+    with pytest.raises(ValueError, match="element size"):
+        cache().read(sl, 4, zeros(4, 2, 64), None, dtype=BF16)
+    with pytest.raises(ValueError, match="element size"):
+        T.Rotary.make_inputs(4, q=x, q_heads=2, positions=sl, q_out=x)
+    with pytest.raises(ValueError, match="element size"):
+        T.KvCache.make_attention_inputs(4, q=x, out=x, q_heads=2, kv_len=sl, max_kv_len=1, scale=1.0)
 
 
 def attention(**kw):

@@ -545,17 +545,43 @@ def matvec_grouped(matrices, xs, outs, stream=None) -> None:
     _ok(load().turbo_int4_matvec_grouped(mats.buffer_info()[0], n, xp.buffer_info()[0], op.buffer_info()[0], stream))
 
 
-def _stride(t) -> int:
-    """Elements from one token to the next of a [tokens][heads][head_dim] tensor (0, packed, for a raw address).
-    Heads of a token are contiguous; anything else cannot be passed."""
+_SIZES = {TURBO_HIDDEN_F32: 4, TURBO_HIDDEN_BF16: 2}
+
+
+def _stride(t, dtype: int) -> int:
+    """Elements from one token to the next of a tensor [...tokens][heads][head_dim] or [tokens][heads * head_dim]
+    (0, packed, for None and a raw address). The values of a token are contiguous and its dtype is the call's;
+    anything else cannot be passed."""
     try:
-        if t is None or t.is_contiguous():
-            return 0
+        packed = t is None or t.is_contiguous()
     except AttributeError:
         return 0
-    if t.dim() == 3 and t.shape[0] and (t.stride(2) != 1 or t.stride(1) != t.shape[2]):
-        raise ValueError("the heads of a token must be contiguous")
-    return t.stride(0)
+    if t is None:
+        return 0
+    if t.element_size() != _SIZES.get(dtype, t.element_size()):
+        raise ValueError("the buffer's element size is not that of dtype")
+    if packed:
+        return 0
+    shape, strides = tuple(t.shape), t.stride()
+    inner = max(1, min(2, len(shape) - 1))  # dimensions of a token
+    step = 1
+    for n, st in zip(shape[:-inner - 1:-1], strides[:-inner - 1:-1]):
+        if n != 1 and st != step:
+            raise ValueError("the heads of a token must be contiguous")
+        step *= n
+    stride = after = 0
+    for n, st in zip(shape[-inner - 1::-1], strides[-inner - 1::-1]):  # the token dimensions, from the last
+        if n == 1:
+            continue
+        if stride == 0:
+            stride, after = st, st * n
+        elif st != after:
+            raise ValueError("the tokens must lie at one stride")
+        else:
+            after = st * n
+        if st < step:
+            raise ValueError("the tokens overlap")
+    return stride
 
 
 def _ids(t) -> int | None:
@@ -582,13 +608,13 @@ class KvCache:
 
     def write(self, k, v, slots, tokens: int, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
         """Quantises k and v of `tokens` tokens into slots (device ids; TURBO_NO_SLOT skips a token)."""
-        _ok(self.lib.turbo_kv_cache_write(self.h, _ptr(k), _stride(k), _ptr(v), _stride(v), dtype,
+        _ok(self.lib.turbo_kv_cache_write(self.h, _ptr(k), _stride(k, dtype), _ptr(v), _stride(v, dtype), dtype,
                                           _ids(slots), tokens, stream))
 
     def read(self, slots, tokens: int, k_out, v_out, *, dtype: int = TURBO_HIDDEN_F32, stream=None) -> None:
         """k_out, v_out (either may be None) = the tokens at slots; NaN for a slot past the cache."""
-        _ok(self.lib.turbo_kv_cache_read(self.h, _ids(slots), tokens, dtype, _ptr(k_out), _stride(k_out), _ptr(v_out),
-                                         _stride(v_out), stream))
+        _ok(self.lib.turbo_kv_cache_read(self.h, _ids(slots), tokens, dtype, _ptr(k_out), _stride(k_out, dtype), _ptr(v_out),
+                                         _stride(v_out, dtype), stream))
 
     @staticmethod
     def make_attention_inputs(batch: int, *, dtype: int = TURBO_HIDDEN_F32, q, out, q_heads: int, q_len: int = 1, kv_len,
@@ -596,7 +622,7 @@ class KvCache:
                               workspace=None) -> TurboAttentionInputs:
         """pages: [batch][page_stride] device ids, whole rows (a slice of a wider table is copied first). workspace: a
         uint8 tensor of attention_workspace(inputs) bytes."""
-        return TurboAttentionInputs(batch, q_len, q_heads, dtype, _ptr(q), _ptr(out), _stride(q), _stride(out),
+        return TurboAttentionInputs(batch, q_len, q_heads, dtype, _ptr(q), _ptr(out), _stride(q, dtype), _stride(out, dtype),
                                     _ids(kv_len), max_kv_len, prefix_len, _ids(prefix_pages) if prefix_len else None, _ids(pages),
                                     int(pages.shape[1]) if pages is not None else 0, window, scale, _ptr(workspace),
                                     workspace.numel() if workspace is not None else 0)
@@ -660,9 +686,9 @@ class Rotary:
     @staticmethod
     def make_inputs(tokens: int, *, dtype: int = TURBO_HIDDEN_F32, q=None, k=None, v=None, q_heads: int = 0, kv_heads: int = 0,
                     positions=None, q_out=None, k_out=None, cache: KvCache | None = None, slots=None) -> TurboQkvInputs:
-        inp = TurboQkvInputs(tokens, dtype, q_heads, kv_heads, _ptr(q), _ptr(k), _ptr(v), _stride(q), _stride(k),
-                             _stride(v), _ids(positions), _ptr(q_out), _ptr(k_out), _stride(q_out),
-                             _stride(k_out), cache.h if cache is not None else None, _ids(slots))
+        inp = TurboQkvInputs(tokens, dtype, q_heads, kv_heads, _ptr(q), _ptr(k), _ptr(v), _stride(q, dtype), _stride(k, dtype),
+                             _stride(v, dtype), _ids(positions), _ptr(q_out), _ptr(k_out), _stride(q_out, dtype),
+                             _stride(k_out, dtype), cache.h if cache is not None else None, _ids(slots))
         return inp
 
     def apply(self, inp: TurboQkvInputs, stream=None) -> None:
