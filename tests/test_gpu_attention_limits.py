@@ -107,7 +107,7 @@ def seen(s, q, b, q_len, kv_len, window, scale, dtype):
             w = np.exp(sc - sc.max())
             w /= w.sum()
             out[i, h] = w @ v[at]
-            e = scale * (kk[at] @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
+            e = abs(scale) * (kk[at] @ np.abs(q[i, h])) * (2.0**-22 + 80 * 2.0**-24) + (2 * np.abs(sc) * 1.4427 + 2) * 2.0**-23
             rel = (2.0**-22 if dtype == "f32" else 2.0**-12) + (40 + (hi - lo) / 32) * 2.0**-24
             bound[i, h] = (2 * e.max() + rel) * (w @ vv[at]) + (hi - lo) * 2.0**-30 * (w * vs[at]).max()
     if dtype == "bf16":
@@ -216,3 +216,16 @@ def test_a_query_with_an_infinity_gives_nan(dtype, sign):
     assert np.isnan(out[1, 1]).all()
     out[1, 1] = 0.0
     assert np.isfinite(out).all()
+
+
+@pytest.mark.parametrize("scale,q_size", [(3e38, 2.0**-126), (-3e38, 2.0**-126), (2.0**-126, 2.0**126), (2.0**-140, 2.0**127)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scales_at_the_ends_of_the_type(dtype, scale, q_size):
+    """scale * log2(e) may be above FP32's largest number, or below its smallest normal one."""
+    rng = np.random.default_rng(9)
+    s = Setup(rng, 1, 64, 8, 32, 0, [70], k_size=2.0**10 if scale == 2.0**-140 else 1.0)
+    q = (np.clip(queries(rng, 1, 2, 64, "f32"), -1.9, 1.9) * np.float32(q_size)).astype(np.float32)
+    q = L.bf16(q) if dtype == "bf16" else q
+    out = attend(s, q, 2, [70], dtype, scale=scale)
+    want, bound = seen(s, q, 0, 1, 70, 0, float(np.float32(scale)), dtype)
+    assert np.all(np.abs(out.float().cpu().numpy() - want) <= bound)

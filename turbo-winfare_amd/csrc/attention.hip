@@ -17,7 +17,7 @@
 //   scale (codes . q) + centre sum(q), the second part by one FP32 matrix instruction per 16 keys and four groups.
 //   A value's scale enters its weight, sum of (weight * scale) codes, and the centres are added with the weights
 //   themselves, in FP32 matrix instructions.
-//   BF16 queries: q is exact in fp16, weights times scale are rounded to 11 bits, 2^-12 of each, against the
+//   BF16 queries: q is exact in fp16 (to 2^-40 of the row's largest), weights times scale are rounded to 11 bits, 2^-12 of each, against the
 //   output's 2^-9. FP32 queries: q and the weights times scale in two fp16 parts each (22 bits).
 #include <algorithm>
 #include <cmath>
@@ -297,7 +297,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         top = rows_max(top);
         bad = rows_sum(bad);  // NaN where a value is infinite or NaN: so is the row then, whatever its scores' signs
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-        const float factor = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), -shift), 0x1.fffffep127f);
+        const float factor = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), a.scale_power - shift), 0x1.fffffep127f);
         if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = factor + bad;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {

@@ -117,7 +117,8 @@ struct AttnArgs {
     uint32_t prefix_len, page_stride;
     uint32_t batch, q_len, q_heads, group;   // group: query heads per key/value head
     uint32_t window;
-    float scale_log2e;
+    float scale_log2e;                       // times 2^scale_power: scale * log2(e), which may leave FP32
+    int scale_power;
     // the plan
     uint32_t prefix_tiles, prefix_splits;    // row tiles and key splits of the prefix, per key/value head (0: the
                                              // sequences take it with their own keys)

@@ -435,7 +435,7 @@ TURBO_DT_API int turbo_prefix_attention(void* handle, const TurboAttentionInputs
     a.q_heads = (uint32_t)in->q_heads;
     a.group = a.q_heads / c->kv.heads;
     a.window = in->window;
-    a.scale_log2e = (float)((double)in->scale * 1.4426950408889634);
+    a.scale_log2e = (float)std::frexp((double)in->scale * 1.4426950408889634, &a.scale_power);
     a.stats = static_cast<float2*>(in->workspace);
     a.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(in->workspace) + plan.stats_bytes);
     tdt::DeviceGuard dg(c->device);
