@@ -444,11 +444,12 @@ TURBO_DT_API int turbo_qk_norm_rope(void* rotary, const TurboQkvInputs* in, void
  * over the tokens that it sees, query head h over key/value head h / (q_heads / kv_heads). A query at
  * a negative position sees nothing and gives zeros (kv_len 0: a padded sequence). A query whose tokens
  * pass its page table, or lie on a page past the cache, gives NaN.
- * The prefix is read once for the whole batch: its products run over the rows of all sequences (a
- * sequence that fills the products' tiles by itself takes it along with its own tokens). Products
- * accumulate in FP32. Keys and values enter as the cache holds them. For FP32 queries, queries and softmax
- * weights keep 22 bits; for BF16 ones the weights keep 11; the smallest weighted values 2^-32 of the largest that
- * the row weights. Tokens that a query does not see have no part in its result.
+ * The prefix is not read once for each sequence: its products run over the rows of all sequences, 16 or 32 rows of
+ * a key/value head at a time (sequences that fill such tiles by themselves take it along with their own
+ * tokens). Scores, softmax statistics and sums are FP32; a score beyond FP32's range gives NaN. Keys and
+ * values enter as the cache holds them. For FP32 queries, queries and softmax weights keep 22 bits; for BF16
+ * ones the weights keep 11; the smallest weighted values 2^-32 of the largest that the row weights. Tokens that
+ * a query does not see have no part in its result.
  */
 typedef struct {
     int batch;                   /* >= 0 */

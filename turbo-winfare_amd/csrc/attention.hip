@@ -1,4 +1,4 @@
-// Attention of a batch over the quantised cache, its shared prefix read once for all sequences.
+// Attention of a batch over the quantised cache; the rows of all sequences share a workgroup over the prefix.
 //
 // A workgroup takes one key/value head, a tile of 16 MT query rows and a range of keys: of the prefix
 // (rows of every sequence of the batch) or of one sequence's own keys (its rows). Its four waves take the
@@ -832,9 +832,10 @@ __global__ __launch_bounds__(kThreads) void k_join(const AttnArgs a, uint32_t he
     store_out<F32>(a.out, token * a.out_stride + (uint64_t)head * head_dim + col, make_float4(v.x * r1, v.y * r1, v.z * r1, v.w * r1));
 }
 
-// 16-row tiles of a workgroup at most: what the registers of two waves per SIMD hold. Four at a head_dim of
-// 128 or less spill a little and measured 25.2 -> 30.2 us (32 sequences behind 8,000 tokens), 124 -> 129 us
-// (a chunk of 512 tokens); one in place of two 120 -> 139 us (head_dim 256, 64 sequences behind 32,768).
+// 16-row tiles of a workgroup at most: what the registers of two waves per SIMD hold without spills (heads of 256:
+// all 256). One in place of two: 94 -> 117 us (2 x 512 prompt tokens behind 2,000), 100 -> 121 us (128 sequences
+// behind 16,000, heads of 128), but 40 -> 34 us (300 prompt tokens with heads of 128, whose workgroups then fill the
+// card).
 constexpr int most_tiles(uint32_t head_dim, bool f32) { return head_dim <= (f32 ? 128u : 256u) ? 2 : 1; }
 uint32_t tiles_for(uint64_t rows, uint32_t most) {
     uint32_t mt = 1u;
@@ -881,14 +882,18 @@ void launch_dtype(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, hi
 
 }  // namespace
 
-// Keys are split until every compute unit has as many workgroups as its registers hold (two; one at a
-// head_dim of 512), but not below 8 records, where a workgroup's start and end and its partial results
-// weigh more than its keys, or 4 where the rows are few: one sequence of 2,000 tokens 14.2 -> 12.7 us, but
-// 8 behind 2,000 13.9 -> 15.3. The prefix is taken apart from the sequences' own keys where that leaves
-// fewer tiles: with as many rows in a sequence as in a tile, a tile goes on from the prefix to its own
-// keys, without partial results to join. Two tiles of rows to a workgroup share the widening of codes,
-// one makes more workgroups: where two left fewer than 16 records to each, 7 x 8 drafts measured
-// 19 -> 16 us with one.
+// Keys are split until every compute unit has two workgroups (one at a head_dim of 512, whose registers hold no
+// more). Three or four, which the registers of smaller heads hold, bring more partial results to join: 29.5 -> 31.7
+// and 33.7 us (32 sequences of 2,000 with heads of 128), 38 -> 40 and 41 us (64 behind 4,000); only 300 prompt
+// tokens with heads of 128 gain, 40 -> 37 us. No split is below 4 records, one to a wave: with 8 at least one
+// sequence of 2,000 measured 12.7 -> 13.6 us, 8 sequences behind 2,000 14.3 -> 15.1.
+// The prefix is taken apart from the sequences' own keys where that leaves two thirds of the tiles or fewer: 16
+// sequences of 8 rows behind 6,000 (heads of 512) measured 44 us together, 34 apart. With as many rows in a
+// sequence as in a tile, a tile goes on from the prefix to its own keys, without partial results to join.
+// Two tiles of rows to a workgroup share the widening of codes, one makes more workgroups: one is taken
+// where two left fewer than 16 records to each. With a border of 8 records 16 sequences of 2,000 measured
+// 17 -> 19 us and 7 x 8 drafts 18 -> 19, though 3 x 10 drafts behind 4,000 31 -> 27; with one of 32, 32 sequences
+// behind 8,000 30 -> 36 us, though 300 prompt tokens 40 -> 34.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -899,7 +904,6 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
     const uint64_t pr = prefix_len ? records(prefix_len, prefix_len / 4u) : 0u, orr = own_most ? records(own_most, q_len) : 0u;
     AttnPlan p{};
     p.rows = (uint64_t)batch * q_len * q_heads;
-    const uint64_t least = p.rows <= 64u ? 4u : 8u;
     for (uint32_t most = most_tiles(head_dim, dtype == TURBO_HIDDEN_F32);; most /= 2u) {
         p.own_tile_rows = 16u * tiles_for(own_rows, most);
         const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
@@ -909,7 +913,7 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         if (!shared) p.prefix_tile_rows = p.own_tile_rows, pt = 0u;
         const uint64_t alone = shared ? orr : pr + orr;  // records of a workgroup's sequence
         const uint64_t work = kv_heads * (pt * pr + batch * ot * alone);
-        const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(least, (work + groups - 1u) / groups);
+        const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(4u, (work + groups - 1u) / groups);
         p.prefix_tiles = (uint32_t)pt;
         p.prefix_splits = shared ? (uint32_t)((pr + per - 1u) / per) : 0u;
         p.own_tiles = (uint32_t)ot;

@@ -26,7 +26,7 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxChunk = 32;      // tokens of a workgroup
 constexpr uint32_t kMaxHeads = 8;       // heads of a workgroup
-constexpr uint32_t kGroups = 1000u;
+constexpr uint32_t kGroups = 1000u;     // workgroups that a call is divided into, at least (shape_for)
 constexpr uint32_t kLdsBytes = 32768;   // for a workgroup's sines, or its values' codes
 
 typedef float float2v __attribute__((ext_vector_type(2)));
@@ -539,7 +539,9 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(const KvReadArgs a, uint32
 // Tokens and heads of a workgroup, from the most that are useful, halved until there are a thousand workgroups:
 // the tokens first, which share a token's sines among more heads, or the heads first, which fill whole lines
 // of the cache (eight neighbouring tokens' keys, 32 tokens' values): a cache write of 4,001 tokens and its
-// read back measured 38.8 us with the tokens halved first, 32.5 so. Heads stay as many as least_heads, what
+// read back measured 38.8 us with the tokens halved first, 32.5 so. With 500 workgroups in place of a thousand that
+// is 33 -> 36 us, 1,500 tokens rotated into the cache and read 27 -> 31, but 256 of them 18 -> 15; with 2,000 workgroups
+// 35 and 31 us, and a rotation of 2,048 tokens 15 -> 19. Heads stay as many as least_heads, what
 // the waves hold at once, while tokens are left to halve.
 struct Shape {
     uint32_t chunk, heads;
