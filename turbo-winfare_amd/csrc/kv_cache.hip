@@ -12,8 +12,8 @@
 //     registers.
 //   Values: 32 tokens are neighbours in the cache, so the codes pass through LDS, and four tokens in a row
 //     are transposed in registers to one 4-byte store per value; a decode step's lone tokens are bytes.
-// The cache's write takes about 200 instructions per 512 values: at 4,001 tokens the vector units are busy 72 % of its
-// time, and waves wait 45 % of theirs, so divisions are products with a group's reciprocal and one correction step.
+// The cache's write takes about 200 instructions per 512 values: at 4,001 tokens the vector units are busy 65 % of its
+// time, and waves wait 43 % of theirs, so divisions are products with a group's reciprocal and one correction step.
 // k_kv_read: a thread takes four values of four tokens, 4-byte loads where the tokens are neighbours.
 #include <stdexcept>
 
