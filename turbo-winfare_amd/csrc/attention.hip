@@ -17,8 +17,9 @@
 //   scale (codes . q) + centre sum(q), the second part by one FP32 matrix instruction per 16 keys and four groups.
 //   A value's scale enters its weight, sum of (weight * scale) codes, and the centres are added with the weights
 //   themselves, in FP32 matrix instructions.
-//   BF16 queries: q is exact in fp16 (to 2^-40 of the row's largest), weights times scale are rounded to 11 bits, 2^-12 of each, against the
-//   output's 2^-9. FP32 queries: q and the weights times scale in two fp16 parts each (22 bits).
+//   BF16 queries: q is exact in fp16 (to 2^-40 of the row's largest), weights times scale are rounded to 11
+//   bits, 2^-12 of each, against the output's 2^-9. FP32 queries: q and the weights times scale in two fp16
+//   parts each (22 bits).
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>

@@ -5,9 +5,9 @@
 // to eight heads at once, and the mean square and a group's range are reductions over neighbouring lanes.
 // The next heads' values are on their way while these are worked on.
 //   Queries and keys: the sines of the run's tokens are computed once, into LDS, and serve all its heads.
-//     Angle: position * turns[i] modulo 2^64 is the fraction of a turn in fixed point, exact in turns[i], which
-//     is rounded to 2^-64, whatever the position; its quadrant is removed as an integer and the remainder, at most pi / 4, goes through the
-//     Taylor series to degree 9 and 10 (first term left out below 2^-28). The other value of a pair in
+//     Angle: position * turns[i] modulo 2^64 is the fraction of a turn in fixed point, exact for turns[i]
+//     (rounded to 2^-64) whatever the position; its quadrant is removed as an integer and the remainder, at
+//     most pi / 4, goes through the Taylor series to degree 9 and 10 (first term left out below 2^-28). The other value of a pair in
 //     halves comes from the lane rotary_dim / 2 / E away. A key's codes go to the cache straight from the
 //     registers.
 //   Values: 32 tokens are neighbours in the cache, so the codes pass through LDS, and four tokens in a row
