@@ -327,7 +327,8 @@ def _prepare_keep(c, seed, st):
     st.parents = _trees(c, seed, b, t)
     st.tokens = torch.randint(0, VOCAB, (b, t), generator=g, device="cuda", dtype=torch.int32)
     child = torch.full((b, t + 1), -1, device="cuda")
-    child.scatter_(1, torch.where(st.parents < 0, t, st.parents).long(), torch.arange(t, device="cuda").expand(b, t))
+    child.scatter_reduce_(1, torch.where(st.parents < 0, t, st.parents).long(), torch.arange(t, device="cuda").expand(b, t),
+                          "amax")
     child = child[:, :t]
     follow = (child >= 0) & (torch.rand((b, t), generator=g, device="cuda") < 0.85)
     st.chosen = torch.where(follow, st.tokens.gather(1, child.clamp_min(0)),
