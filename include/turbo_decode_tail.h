@@ -52,7 +52,11 @@ enum {
     TURBO_ABI_KV_CACHE_DESC = 6,  /* TurboKvCacheDesc */
     TURBO_ABI_ROTARY_DESC = 7,    /* TurboRotaryDesc */
     TURBO_ABI_QKV_INPUTS = 8,     /* TurboQkvInputs */
-    TURBO_ABI_ATTENTION_INPUTS = 9 /* TurboAttentionInputs */
+    TURBO_ABI_ATTENTION_INPUTS = 9, /* TurboAttentionInputs */
+    TURBO_ABI_BATCH_PLAN = 10,    /* TurboBatchPlan */
+    TURBO_ABI_PAGES_RELEASE = 11, /* TurboPagesRelease */
+    TURBO_ABI_TREE_ACCEPT = 12,   /* TurboTreeAccept */
+    TURBO_ABI_PROMPT_INPUTS = 13  /* TurboPromptInputs */
 };
 TURBO_DT_API uint32_t turbo_abi_version(void);
 /* sizeof of the struct TURBO_ABI_* names, as the library was built; 0 for an unknown id. */
@@ -476,6 +480,156 @@ typedef struct {
 /* The scratch a call with these sizes needs (0: none); pointers are not looked at. */
 TURBO_DT_API int turbo_attention_workspace(void* cache, const TurboAttentionInputs* in, size_t* bytes);
 TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs* in, void* hip_stream);
+
+/*
+ * Attention of drafted trees: turbo_prefix_attention for sequences whose last q_len tokens (1 .. 64) are a tree's
+ * nodes in place of a run. masks: [batch][q_len] device words, bit j of one: the query sees node j of its own
+ * sequence (turbo_batch_plan makes them of the nodes' parents; bits from q_len on are ignored). A query sees the
+ * kv_len[b] - q_len tokens before the tree and the nodes of its mask, in this order the last `window` of them
+ * where window is not 0. A mask of 0 marks an absent node, which gives zeros; nodes that a query does not see
+ * have no part in its result, whatever their slots hold. Everything else, the workspace too, is as there.
+ */
+TURBO_DT_API int turbo_tree_attention(void* cache, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream);
+
+/*
+ * Moves tokens inside the cache, codes, scales and biases bit by bit: the token at source[r * width + i] goes to
+ * target[r * width + i] for `rows` rows of `width` (1 .. 64) moves, device slots. What a row moves is read before
+ * the row writes anything, so a row may write slots that it reads; the targets of a row differ, and different
+ * rows share no slot that one of them writes. A move from or to a slot past the cache (TURBO_NO_SLOT) is skipped.
+ */
+TURBO_DT_API int turbo_kv_cache_move(void* cache, const uint32_t* source, const uint32_t* target, int rows, int width,
+                                     void* hip_stream);
+
+/*
+ * ---- a serving step's requests --------------------------------------------------------------
+ * What the calls above take as slots, positions, lengths, page tables and masks, made on the device from the
+ * lengths of the sequences, and attention over prompts that are not in a cache yet. No counterpart in the reference
+ * (one sequence, a ring of 4096). The calls have no handle: they run on the device that they name, on hip_stream,
+ * allocate nothing and may be captured into a HIP graph.
+ */
+
+/* A page that a sequence needs and the pool did not have. */
+#define TURBO_NO_PAGE 0xFFFFFFFFu
+
+/*
+ * One step of a batch: sequence b holds past_len[b] tokens and adds new_len[b]. The first prefix_len tokens of every
+ * sequence are the shared prefix, on pages of its own; the others are on the sequence's pages, as
+ * TurboAttentionInputs has them. The table of sequence b holds held[b] pages. It gets those that it lacks from the
+ * end of the pool's list, in the order of the sequences and of their pages: the k-th page taken is
+ * free_pages[free_count - 1 - k]. Where the pool is empty the table gets TURBO_NO_PAGE, held_out does not count it,
+ * and the tokens on it get TURBO_NO_SLOT, as do tokens past the table (totals[3] counts such pages; once the pool has
+ * pages again the same plan gets them).
+ *
+ * The tokens added are packed, sequence after sequence (row_tokens 0), or lie in rows of row_tokens, of which a
+ * sequence fills the first new_len (what passes row_tokens is left out). Entries that no token has get position 0 and
+ * TURBO_NO_SLOT. With parents the rows are drafted trees: node t of sequence b hangs on node parents[b][t] < t, or on
+ * the sequence's last token (-1). A node with any other parent, past new_len, or whose parent is absent is absent.
+ * Its mask holds the bits of its ancestors and its own; its position is past_len plus the number of its ancestors; its
+ * slot is that of token past_len + t.
+ */
+typedef struct {
+    int batch;                      /* 0 .. 8192 */
+    uint32_t page_tokens;           /* the caches' */
+    uint32_t prefix_len;
+    const uint32_t* past_len;       /* [batch], the prefix included */
+    const uint32_t* new_len;        /* [batch] */
+    uint32_t row_tokens;
+    uint32_t max_tokens;            /* entries of positions and slots, at most 2^28; batch * row_tokens for rows */
+    const int32_t* parents;         /* [batch][row_tokens] or NULL; row_tokens is at most 64 then */
+    uint32_t* pages;                /* [batch][page_stride], the new pages are written */
+    uint32_t page_stride;
+    const uint32_t* held;           /* [batch] */
+    const uint32_t* free_pages;     /* [free_capacity] */
+    const uint32_t* free_count;     /* [1] */
+    uint32_t free_capacity;
+    /* the pool's state after the step; may be held and free_count themselves */
+    uint32_t* held_out;
+    uint32_t* free_count_out;
+    /* results, each may be NULL */
+    uint32_t* starts;               /* [batch + 1] first entry of every sequence */
+    uint32_t* kv_len;               /* [batch] past + new; for rows past + row_tokens, as the attention counts its
+                                       queries (0 for a sequence that adds nothing) */
+    uint32_t* positions;            /* [max_tokens] */
+    uint32_t* slots;                /* [max_tokens] */
+    uint64_t* masks;                /* [batch][row_tokens], with parents */
+    uint32_t* totals;               /* [4] tokens added, tokens left out, pages taken, pages missing */
+    int device;                     /* HIP device ordinal */
+} TurboBatchPlan;
+TURBO_DT_API int turbo_batch_plan(const TurboBatchPlan* in, void* hip_stream);
+
+/* Gives pages back: sequence b keeps those of its first keep_len[b] tokens (the prefix included; 0: none), the others
+ * go to the end of the pool's list in the order of the sequences. The list has room for every page of the caches. */
+typedef struct {
+    int batch;                      /* 0 .. 8192 */
+    uint32_t page_tokens;
+    uint32_t prefix_len;
+    const uint32_t* keep_len;       /* [batch] */
+    const uint32_t* pages;          /* [batch][page_stride] */
+    uint32_t page_stride;
+    uint32_t* held;                 /* [batch], updated */
+    uint32_t* free_pages;           /* [free_capacity], updated */
+    uint32_t* free_count;           /* [1], updated */
+    uint32_t free_capacity;
+    int device;
+} TurboPagesRelease;
+TURBO_DT_API int turbo_pages_release(const TurboPagesRelease* in, void* hip_stream);
+
+/*
+ * The path of every tree that the model confirms. Node 0 is the token that the step before drew, so it is kept;
+ * then, from the last kept node on, the first child whose token is the one chosen after that node (turbo_lmhead_step's
+ * tokens over the nodes as rows; 0xFFFFFFFF, its mark of a degenerate row, confirms nothing). next is the choice after the last kept node:
+ * node 0 of the following step. The i-th kept node's key and value belong at the slot of node i: source and target
+ * say so to turbo_kv_cache_move, once for each layer's cache. Parents as in TurboBatchPlan.
+ */
+typedef struct {
+    int batch;                      /* 0 .. 2^20 */
+    uint32_t row_tokens;            /* 1 .. 64 */
+    const int32_t* parents;         /* [batch][row_tokens] */
+    const uint32_t* new_len;        /* [batch] nodes of each tree */
+    const uint32_t* tokens;         /* [batch][row_tokens] */
+    const uint32_t* chosen;         /* [batch][row_tokens] */
+    const uint32_t* past_len;       /* [batch], for length */
+    const uint32_t* slots;          /* [batch][row_tokens], for source and target */
+    uint32_t* kept;                 /* [batch] nodes kept */
+    uint32_t* next;                 /* [batch]; 0xFFFFFFFF where nothing is kept */
+    /* each may be NULL, source and target together */
+    uint32_t* length;               /* [batch] past_len + kept */
+    uint32_t* path;                 /* [batch][row_tokens] the kept nodes, then 0xFFFFFFFF */
+    uint32_t* source;               /* [batch][row_tokens] their slots, then TURBO_NO_SLOT */
+    uint32_t* target;               /* [batch][row_tokens] where they belong, then TURBO_NO_SLOT */
+    int device;
+} TurboTreeAccept;
+TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream);
+
+/*
+ * Causal attention of whole prompts over their own keys and values, before or without a cache. Sequence b is rows
+ * starts[b] .. starts[b + 1] - 1 of q, k, v and out (starts is not decreasing; rows past `tokens` are left out).
+ * Query i of it sees keys 0 .. i, the last `window` of them where window is not 0:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * query head h over key/value head h / (q_heads / kv_heads). Buffers as the layer loop's common rules have them, with
+ * strides of at most 2^24 elements. Rows of no sequence are left as they were. Scores, softmax statistics and sums are
+ * FP32; BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-9 of each), FP32 ones in FP32.
+ * A score beyond FP32's range, an infinity or NaN in a query or in a key that it sees gives NaN, in a value that it
+ * sees the same or an infinity. What a query does not see has no part in its result.
+ */
+typedef struct {
+    int batch;                   /* 0 .. 2^20 */
+    int tokens;                  /* rows of the buffers, 0 .. 2^28 */
+    int q_heads;                 /* a multiple of kv_heads */
+    int kv_heads;
+    uint32_t head_dim;           /* 64, 128, 256 or 512 */
+    int dtype;                   /* TURBO_HIDDEN_* of q, k, v and out */
+    const void* q;               /* [tokens][q_heads][head_dim] */
+    const void* k;               /* [tokens][kv_heads][head_dim] */
+    const void* v;
+    void* out;                   /* as q; overlaps nothing else */
+    size_t q_stride, k_stride, v_stride, out_stride;
+    const uint32_t* starts;      /* [batch + 1] */
+    uint32_t window;
+    float scale;                 /* magnitude below 2^127 */
+    int device;                  /* HIP device ordinal */
+} TurboPromptInputs;
+TURBO_DT_API int turbo_prompt_attention(const TurboPromptInputs* in, void* hip_stream);
 
 /*
  * Embedding lookup on the same tied table (shaders/EmbedLookup.hlsl:1-45; CPU

@@ -18,7 +18,8 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "lib" / "libturbo_decode_tail.so"
 SOURCES = ["api.cpp", "bundle.cpp", "prep.hip", "gemv_digits.hip", "gemm_mfma.hip", "gemm_split.hip", "select.hip", "misc.hip", "noalloc.hip", "matrix.cpp",
-           "layer_attention.cpp", "kv_cache.hip", "attention.hip"]
+           "layer_attention.cpp", "kv_cache.hip", "attention.hip", "tree_attention.hip", "kv_move.hip", "step.cpp", "step_plan.hip",
+           "prompt_attention.hip"]
 ARCH = "gfx950"
 FLAGS = [
     f"--offload-arch={ARCH}",

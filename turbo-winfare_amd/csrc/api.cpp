@@ -592,6 +592,10 @@ TURBO_DT_API size_t turbo_abi_struct_size(int which) {
         case TURBO_ABI_ROTARY_DESC: return sizeof(TurboRotaryDesc);
         case TURBO_ABI_QKV_INPUTS: return sizeof(TurboQkvInputs);
         case TURBO_ABI_ATTENTION_INPUTS: return sizeof(TurboAttentionInputs);
+        case TURBO_ABI_BATCH_PLAN: return sizeof(TurboBatchPlan);
+        case TURBO_ABI_PAGES_RELEASE: return sizeof(TurboPagesRelease);
+        case TURBO_ABI_TREE_ACCEPT: return sizeof(TurboTreeAccept);
+        case TURBO_ABI_PROMPT_INPUTS: return sizeof(TurboPromptInputs);
         default: return 0;
     }
 }

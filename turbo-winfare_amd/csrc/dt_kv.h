@@ -124,6 +124,7 @@ struct AttnArgs {
                                              // sequences take it with their own keys)
     uint32_t own_tiles, own_splits;          // of one sequence's own keys
     uint32_t prefix_items, items;            // workgroups
+    const uint64_t* masks;                   // [batch][q_len] the nodes that a row of a drafted tree sees, or null
     Divider by_rows, by_group;               // by q_len * group, by group
     uint32_t parts;                          // partial results per row (1: written to out directly)
     float2* stats;                           // [rows][parts] (running maximum, sum)
@@ -138,6 +139,8 @@ struct AttnPlan {
 };
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus);
+// tree_attention.hip: the workgroups' kernel of a call with masks; the plan and the join are attention.hip's.
+void launch_tree_attend(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);
 void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);
 
 }  // namespace tdt

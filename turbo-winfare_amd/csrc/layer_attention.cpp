@@ -9,15 +9,16 @@
 #include <string>
 #include <vector>
 
+#include "dt_checks.h"
 #include "dt_internal.h"
-#include "dt_kv.h"
+#include "dt_step.h"
+
+using namespace tdt;
 
 namespace {
 
 constexpr uint32_t kCacheMagic = 0x564B4454u;   // "TDKV"
 constexpr uint32_t kRotaryMagic = 0x4F524454u;  // "TDRO"
-constexpr int kMaxTokens = 1 << 28;             // a cache read takes 8 threads of one grid dimension to a token
-constexpr uint32_t kMaxKvHeads = 1024, kMaxQueryHeads = 8192;
 
 // The streams a handle's calls were enqueued on, waited for before it is freed.
 struct Streams {
@@ -58,8 +59,6 @@ struct RotaryBox {
     Streams streams;
 };
 
-[[noreturn]] void fail(const std::string& what) { throw std::runtime_error(what); }
-
 CacheBox* cbox(void* p) {
     if (!p) fail("null cache handle");
     auto* c = static_cast<CacheBox*>(p);
@@ -72,36 +71,6 @@ RotaryBox* rbox(void* p) {
     auto* r = static_cast<RotaryBox*>(p);
     if (r->magic != kRotaryMagic) fail("invalid rotary handle");
     return r;
-}
-
-void check_head_dim(uint32_t d) {
-    if (d != 64u && d != 128u && d != 256u && d != 512u) fail("head_dim must be 64, 128, 256 or 512");
-}
-
-void check_device(int device) {
-    int ndev = 0;
-    tdt::check_hip(hipGetDeviceCount(&ndev), "hipGetDeviceCount");
-    if (device < 0 || device >= ndev) fail("no such HIP device");
-}
-
-size_t dtype_size(int dtype) {
-    if (dtype != TURBO_HIDDEN_F32 && dtype != TURBO_HIDDEN_BF16) fail("dtype must be TURBO_HIDDEN_F32 or TURBO_HIDDEN_BF16");
-    return dtype == TURBO_HIDDEN_BF16 ? 2u : 4u;
-}
-
-void check_tokens(int tokens) {
-    if (tokens < 0 || tokens > kMaxTokens) fail("tokens must be in 0.." + std::to_string(kMaxTokens));
-}
-
-// A buffer of rows and its stride in elements (0: packed); the stride it has.
-size_t check_rows(const char* name, const void* p, size_t stride, size_t packed, size_t size) {
-    if (!p) fail(std::string(name) + " is NULL");
-    if (reinterpret_cast<uintptr_t>(p) % 16u != 0u) fail(std::string(name) + " must be 16-byte aligned");
-    if (stride == 0u) return packed;
-    if (stride < packed) fail(std::string(name) + "_stride is smaller than a token's heads");
-    if (stride > (size_t{1} << 32)) fail(std::string(name) + "_stride is above 2^32 elements");
-    if (stride * size % 16u != 0u) fail(std::string(name) + "_stride must be a multiple of 16 bytes");
-    return stride;
 }
 
 // The sizes of an attention call, checked, and how it is split.
@@ -123,20 +92,6 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in) 
 }
 
 }  // namespace
-
-#define ATT_TRY            \
-    tdt::set_last_error(""); \
-    try {
-#define ATT_CATCH(ret)                        \
-    }                                         \
-    catch (const std::exception& ex) {        \
-        tdt::set_last_error(ex.what());       \
-        return ret;                           \
-    }                                         \
-    catch (...) {                             \
-        tdt::set_last_error("unknown error"); \
-        return ret;                           \
-    }
 
 extern "C" {
 
@@ -244,6 +199,27 @@ TURBO_DT_API int turbo_kv_cache_read(void* handle, const uint32_t* slots, int to
     tdt::DeviceGuard dg(c->device);
     c->streams.note(static_cast<hipStream_t>(hip_stream));
     tdt::launch_kv_read(a, c->head_dim, dtype, static_cast<hipStream_t>(hip_stream));
+    return 1;
+    ATT_CATCH(0)
+}
+
+TURBO_DT_API int turbo_kv_cache_move(void* handle, const uint32_t* source, const uint32_t* target, int rows, int width,
+                                     void* hip_stream) {
+    ATT_TRY
+    CacheBox* c = cbox(handle);
+    if (width < 1 || width > (int)tdt::kTreeNodes) fail("width must be in 1..64");
+    if (rows < 0 || rows > (1 << 20)) fail("rows must be in 0..1048576");
+    if (rows == 0) return 1;
+    if (!source || !target) fail("source or target is NULL");
+    tdt::KvMoveArgs a{};
+    a.kv = c->kv;
+    a.source = source;
+    a.target = target;
+    a.rows = (uint32_t)rows;
+    a.width = (uint32_t)width;
+    tdt::DeviceGuard dg(c->device);
+    c->streams.note(static_cast<hipStream_t>(hip_stream));
+    tdt::launch_kv_move(a, static_cast<hipStream_t>(hip_stream));
     return 1;
     ATT_CATCH(0)
 }
@@ -401,13 +377,12 @@ TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInp
     ATT_CATCH(0)
 }
 
-TURBO_DT_API int turbo_prefix_attention(void* handle, const TurboAttentionInputs* in, void* hip_stream) {
-    ATT_TRY
+static void attend(void* handle, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream) {
     CacheBox* c = cbox(handle);
     if (!in) fail("in is NULL");
     const tdt::AttnPlan plan = attention_plan(*c, *in);
     if (!std::isfinite(in->scale)) fail("scale must be finite");
-    if (in->batch == 0) return 1;
+    if (in->batch == 0) return;
     const size_t size = dtype_size(in->dtype), packed = (size_t)in->q_heads * c->head_dim;
     tdt::AttnArgs a{};
     a.q_stride = check_rows("q", in->q, in->q_stride, packed, size);
@@ -435,12 +410,30 @@ TURBO_DT_API int turbo_prefix_attention(void* handle, const TurboAttentionInputs
     a.q_heads = (uint32_t)in->q_heads;
     a.group = a.q_heads / c->kv.heads;
     a.window = in->window;
+    a.masks = masks;
     a.scale_log2e = (float)std::frexp((double)in->scale * 1.4426950408889634, &a.scale_power);
     a.stats = static_cast<float2*>(in->workspace);
     a.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(in->workspace) + plan.stats_bytes);
     tdt::DeviceGuard dg(c->device);
     c->streams.note(static_cast<hipStream_t>(hip_stream));
     tdt::launch_attention(a, plan, c->head_dim, in->dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+TURBO_DT_API int turbo_prefix_attention(void* handle, const TurboAttentionInputs* in, void* hip_stream) {
+    ATT_TRY
+    attend(handle, in, nullptr, hip_stream);
+    return 1;
+    ATT_CATCH(0)
+}
+
+TURBO_DT_API int turbo_tree_attention(void* handle, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream) {
+    ATT_TRY
+    cbox(handle);
+    if (!in) fail("in is NULL");
+    if (in->q_len < 1 || in->q_len > (int)tdt::kTreeNodes) fail("q_len must be in 1..64 for a tree");
+    if (in->batch > 0 && !masks) fail("masks is NULL");
+    if (reinterpret_cast<uintptr_t>(masks) % 8u != 0u) fail("masks must be 8-byte aligned");
+    attend(handle, in, masks, hip_stream);
     return 1;
     ATT_CATCH(0)
 }

@@ -24,6 +24,7 @@ TURBO_STEP_NORMED = 1
 TURBO_STEP_APPEND_HISTORY = 2
 TURBO_STATUS_HISTORY_FULL = 1
 TURBO_NO_SLOT = 0xFFFFFFFF
+TURBO_NO_PAGE = 0xFFFFFFFF
 TURBO_ROPE_HALVES = 0
 TURBO_ROPE_PAIRS = 1
 TURBO_NORM_Q = 1
@@ -76,6 +77,12 @@ EXPORTS = (
     "turbo_qk_norm_rope",
     "turbo_attention_workspace",
     "turbo_prefix_attention",
+    "turbo_tree_attention",
+    "turbo_kv_cache_move",
+    "turbo_batch_plan",
+    "turbo_pages_release",
+    "turbo_tree_accept",
+    "turbo_prompt_attention",
 )
 
 TURBO_NOALLOC_MAX_BATCH = 4
@@ -250,6 +257,93 @@ class TurboAttentionInputs(C.Structure):
 _lib = None
 
 
+class TurboBatchPlan(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("page_tokens", C.c_uint32),
+        ("prefix_len", C.c_uint32),
+        ("past_len", C.c_void_p),
+        ("new_len", C.c_void_p),
+        ("row_tokens", C.c_uint32),
+        ("max_tokens", C.c_uint32),
+        ("parents", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("page_stride", C.c_uint32),
+        ("held", C.c_void_p),
+        ("free_pages", C.c_void_p),
+        ("free_count", C.c_void_p),
+        ("free_capacity", C.c_uint32),
+        ("held_out", C.c_void_p),
+        ("free_count_out", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("masks", C.c_void_p),
+        ("totals", C.c_void_p),
+        ("device", C.c_int),
+    ]
+
+
+class TurboPagesRelease(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("page_tokens", C.c_uint32),
+        ("prefix_len", C.c_uint32),
+        ("keep_len", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("page_stride", C.c_uint32),
+        ("held", C.c_void_p),
+        ("free_pages", C.c_void_p),
+        ("free_count", C.c_void_p),
+        ("free_capacity", C.c_uint32),
+        ("device", C.c_int),
+    ]
+
+
+class TurboTreeAccept(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("row_tokens", C.c_uint32),
+        ("parents", C.c_void_p),
+        ("new_len", C.c_void_p),
+        ("tokens", C.c_void_p),
+        ("chosen", C.c_void_p),
+        ("past_len", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("next", C.c_void_p),
+        ("length", C.c_void_p),
+        ("path", C.c_void_p),
+        ("source", C.c_void_p),
+        ("target", C.c_void_p),
+        ("device", C.c_int),
+    ]
+
+
+class TurboPromptInputs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("tokens", C.c_int),
+        ("q_heads", C.c_int),
+        ("kv_heads", C.c_int),
+        ("head_dim", C.c_uint32),
+        ("dtype", C.c_int),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_stride", C.c_size_t),
+        ("k_stride", C.c_size_t),
+        ("v_stride", C.c_size_t),
+        ("out_stride", C.c_size_t),
+        ("starts", C.c_void_p),
+        ("window", C.c_uint32),
+        ("scale", C.c_float),
+        ("device", C.c_int),
+    ]
+
+
 def load(path: os.PathLike | str | None = None) -> C.CDLL:
     """Loads the built library (raises if it is missing)."""
     global _lib
@@ -308,6 +402,12 @@ def load(path: os.PathLike | str | None = None) -> C.CDLL:
         "turbo_qk_norm_rope": (i32, [vp, C.POINTER(TurboQkvInputs), vp]),
         "turbo_attention_workspace": (i32, [vp, C.POINTER(TurboAttentionInputs), C.POINTER(C.c_size_t)]),
         "turbo_prefix_attention": (i32, [vp, C.POINTER(TurboAttentionInputs), vp]),
+        "turbo_tree_attention": (i32, [vp, C.POINTER(TurboAttentionInputs), vp, vp]),
+        "turbo_kv_cache_move": (i32, [vp, vp, vp, i32, i32, vp]),
+        "turbo_batch_plan": (i32, [C.POINTER(TurboBatchPlan), vp]),
+        "turbo_pages_release": (i32, [C.POINTER(TurboPagesRelease), vp]),
+        "turbo_tree_accept": (i32, [C.POINTER(TurboTreeAccept), vp]),
+        "turbo_prompt_attention": (i32, [C.POINTER(TurboPromptInputs), vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -594,6 +694,33 @@ def _ids(t) -> int | None:
     return _ptr(t)
 
 
+def _masks(t, n: int) -> int | None:
+    """The address of n 64-bit masks: a contiguous tensor of 64-bit integers, or a raw address."""
+    try:
+        if t is not None and (t.element_size() != 8 or t.is_floating_point() or not t.is_contiguous() or t.numel() < n):
+            raise ValueError("masks must be contiguous 64-bit integers, one for each row")
+    except AttributeError:
+        pass
+    return _ptr(t)
+
+
+def _count(name: str, t, n: int) -> int | None:
+    """The address of device ids, a tensor of at least n of them."""
+    at = _ids(t)
+    if t is not None and hasattr(t, "numel") and t.numel() < n:
+        raise ValueError(f"{name} holds {t.numel()} values, {n} are needed")
+    return at
+
+
+def _device(*ts) -> int:
+    """The HIP device of the first tensor that has one (0 for raw addresses)."""
+    for t in ts:
+        d = getattr(getattr(t, "device", None), "index", None)
+        if d is not None:
+            return int(d)
+    return 0
+
+
 class KvCache:
     """One turbo_kv_cache handle: a layer's keys and values in pages, quantised to 4 or 8 bits.
     Buffers are torch CUDA tensors [tokens][kv_heads][head_dim] or raw addresses (packed)."""
@@ -635,6 +762,18 @@ class KvCache:
     def attend(self, inp: TurboAttentionInputs, stream=None) -> None:
         """turbo_prefix_attention: out = softmax(scale q k) v over the shared prefix and each sequence's own keys."""
         _ok(self.lib.turbo_prefix_attention(self.h, C.byref(inp), stream))
+
+    def attend_tree(self, inp: TurboAttentionInputs, masks, stream=None) -> None:
+        """turbo_tree_attention: the last q_len tokens of every sequence are a tree; masks [batch][q_len] 64-bit words,
+        bit j: the query sees node j."""
+        _ok(self.lib.turbo_tree_attention(self.h, C.byref(inp), _masks(masks, inp.batch * inp.q_len), stream))
+
+    def move(self, source, target, stream=None) -> None:
+        """turbo_kv_cache_move: the tokens at the slots source [rows][width] go to target, bit by bit."""
+        if tuple(source.shape) != tuple(target.shape) or len(source.shape) != 2:
+            raise ValueError("source and target are [rows][width]")
+        rows, width = source.shape
+        _ok(self.lib.turbo_kv_cache_move(self.h, _ids(source), _ids(target), rows, width, stream))
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -704,6 +843,72 @@ class Rotary:
             self.close()
         except Exception:
             pass
+
+
+def make_batch_plan(batch: int, *, page_tokens: int, past_len, new_len, max_tokens: int, pages, held, free_pages, free_count,
+                    prefix_len: int = 0, row_tokens: int = 0, parents=None, held_out=None, free_count_out=None, starts=None,
+                    kv_len=None, positions=None, slots=None, masks=None, totals=None) -> TurboBatchPlan:
+    """Device ids throughout; pages: [batch][page_stride]. held_out and free_count_out: held and free_count, updated in
+    place, unless given. The tensors must outlive the struct."""
+    held_out = held if held_out is None else held_out
+    free_count_out = free_count if free_count_out is None else free_count_out
+    if pages is not None and (len(pages.shape) != 2 or pages.shape[0] < batch):
+        raise ValueError("pages is [batch][page_stride]")
+    return TurboBatchPlan(batch, page_tokens, prefix_len, _count("past_len", past_len, batch), _count("new_len", new_len, batch),
+                          row_tokens, max_tokens, _count("parents", parents, batch * row_tokens), _ids(pages),
+                          int(pages.shape[1]) if pages is not None else 0, _count("held", held, batch), _ids(free_pages),
+                          _count("free_count", free_count, 1), int(free_pages.numel()), _count("held_out", held_out, batch),
+                          _count("free_count_out", free_count_out, 1), _count("starts", starts, batch + 1),
+                          _count("kv_len", kv_len, batch), _count("positions", positions, max_tokens),
+                          _count("slots", slots, max_tokens), _masks(masks, batch * row_tokens), _count("totals", totals, 4),
+                          _device(past_len, pages, held))
+
+
+def batch_plan(inp: TurboBatchPlan, stream=None) -> None:
+    """turbo_batch_plan: a step's page tables, slots, positions, lengths and masks from its sequences' lengths."""
+    _ok(load().turbo_batch_plan(C.byref(inp), stream))
+
+
+def pages_release(batch: int, *, page_tokens: int, keep_len, pages, held, free_pages, free_count, prefix_len: int = 0,
+                  stream=None) -> None:
+    """turbo_pages_release: every sequence keeps the pages of its first keep_len tokens; held, free_pages and
+    free_count are updated."""
+    if len(pages.shape) != 2 or pages.shape[0] < batch:
+        raise ValueError("pages is [batch][page_stride]")
+    inp = TurboPagesRelease(batch, page_tokens, prefix_len, _count("keep_len", keep_len, batch), _ids(pages), int(pages.shape[1]),
+                            _count("held", held, batch), _ids(free_pages), _count("free_count", free_count, 1),
+                            int(free_pages.numel()), _device(keep_len, pages, held))
+    _ok(load().turbo_pages_release(C.byref(inp), stream))
+
+
+def make_tree_accept(batch: int, row_tokens: int, *, parents, new_len, tokens, chosen, kept, next, past_len=None, slots=None,
+                     length=None, path=None, source=None, target=None) -> TurboTreeAccept:
+    """Device ids: parents, tokens, chosen, slots, path, source and target [batch][row_tokens], the others [batch]."""
+    n = batch * row_tokens
+    return TurboTreeAccept(batch, row_tokens, _count("parents", parents, n), _count("new_len", new_len, batch),
+                           _count("tokens", tokens, n), _count("chosen", chosen, n), _count("past_len", past_len, batch),
+                           _count("slots", slots, n), _count("kept", kept, batch), _count("next", next, batch),
+                           _count("length", length, batch), _count("path", path, n), _count("source", source, n),
+                           _count("target", target, n), _device(parents, tokens, chosen))
+
+
+def tree_accept(inp: TurboTreeAccept, stream=None) -> None:
+    """turbo_tree_accept: the path of every tree that the model's choices confirm."""
+    _ok(load().turbo_tree_accept(C.byref(inp), stream))
+
+
+def make_prompt_inputs(batch: int, tokens: int, *, dtype: int = TURBO_HIDDEN_F32, q, k, v, out, q_heads: int, kv_heads: int,
+                       head_dim: int, starts, window: int = 0, scale: float) -> TurboPromptInputs:
+    """q, k, v, out: torch CUDA tensors [tokens][heads][head_dim] (slices of wider rows too) or raw addresses (packed);
+    starts: [batch + 1] device ids."""
+    return TurboPromptInputs(batch, tokens, q_heads, kv_heads, head_dim, dtype, _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                             _stride(q, dtype), _stride(k, dtype), _stride(v, dtype), _stride(out, dtype),
+                             _count("starts", starts, batch + 1), window, scale, _device(q, k, v))
+
+
+def prompt_attention(inp: TurboPromptInputs, stream=None) -> None:
+    """turbo_prompt_attention: causal attention of packed prompts over their own keys and values."""
+    _ok(load().turbo_prompt_attention(C.byref(inp), stream))
 
 
 def sample_logits_noalloc(logits, vocab: int, inp: TurboStepInputs, tokens, report=None, *,
