@@ -608,7 +608,7 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream);
  *   out = sum_j softmax_j(scale * q . k_j) v_j
  * query head h over key/value head h / (q_heads / kv_heads). Buffers as the layer loop's common rules have them, with
  * strides of at most 2^24 elements. Rows of no sequence are left as they were. Scores, softmax statistics and sums are
- * FP32; BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-9 of each), FP32 ones in FP32.
+ * FP32; BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-8 of each at most), FP32 ones in FP32.
  * A score beyond FP32's range, an infinity or NaN in a query or in a key that it sees gives NaN, in a value that it
  * sees the same or an infinity. What a query does not see has no part in its result.
  */

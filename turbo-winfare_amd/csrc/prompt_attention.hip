@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "dt_internal.h"
+#include "dt_mfma.h"
 #include "dt_step.h"
 
 namespace tdt {
@@ -59,7 +60,7 @@ struct Item {
     bool exists;
 };
 
-// Tile number `id` of all sequences' tiles of `rows` rows: the last tiles, which have most keys, come first, and
+// Tile number `id` of all sequences' tiles of `rows` rows (a token's heads that share keys have one each): the last tiles, which have most keys, come first, and
 // among equal ones the sequences in order. Every wave finds it for itself: the number of tiles at a level or above
 // falls with the level, so the level is found by halving.
 __device__ inline Item locate(const PromptArgs& a, uint32_t id, uint32_t rows) {
@@ -73,7 +74,7 @@ __device__ inline Item locate(const PromptArgs& a, uint32_t id, uint32_t rows) {
     auto tiles_of = [&](uint32_t b) {
         uint32_t first = first0, len = len0;
         if (b >= 64u) bounds(b, first, len);
-        return (len + rows - 1u) / rows;
+        return (len * a.group + rows - 1u) / rows;
     };
     auto at_least = [&](uint32_t level) {  // tiles of all sequences from this level on
         uint32_t n = 0;
@@ -84,7 +85,7 @@ __device__ inline Item locate(const PromptArgs& a, uint32_t id, uint32_t rows) {
         return (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_reduce(n, [](uint32_t x, uint32_t y) { return x + y; }));
     };
     Item it{};
-    uint32_t lo = 0u, hi = (a.tokens + rows - 1u) / rows;  // at_least(lo) > id >= at_least(hi)
+    uint32_t lo = 0u, hi = (a.tokens * a.group + rows - 1u) / rows;  // at_least(lo) > id >= at_least(hi)
     if (at_least(0u) <= id) return it;
     while (hi - lo > 1u) {
         const uint32_t mid = (lo + hi) / 2u;
@@ -112,16 +113,19 @@ __device__ inline Item locate(const PromptArgs& a, uint32_t id, uint32_t rows) {
     return it;
 }
 
-// A row's running maximum (times scale) and sum, and the weights of a block's 16 scores of a lane.
+// A row's running maximum (times scale) and sum, and the weights of a lane's scores.
 struct Softmax {
     float m = kNegInf, l = 0.0f;
     // Scores to weights; true where the sums have to be multiplied by alpha first.
-    __device__ inline bool weights(f32x16& s, float c, float& alpha) {
+    template <int N>
+    __device__ inline bool weights(f32x16 (&s)[N], float c, float& alpha) {
         float top = kNegInf;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
         top = halves_max(top) * c;
-        const bool moves = __any(top > m + kSlack || (m == kNegInf && top > kNegInf));
+        const bool moves = __any(top > m + kSlack);
         alpha = 1.0f;
         if (moves) {
             const float now = fmaxf(m, top);
@@ -131,63 +135,122 @@ struct Softmax {
         }
         const float zero = m == kNegInf ? 0.0f : m;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -zero));
-            l += s[r];
-        }
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], c, -zero));
+                l += s[b][r];
+            }
         return moves;
     }
 };
 
 __device__ inline bool not_finite(float v) { return !(fabsf(v) < __builtin_inff()); }
-// Whether one of two BF16 numbers is infinite or NaN, and the pair with 0 in its place
-__device__ inline bool odd_pair(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
-__device__ inline uint32_t clean_pair(uint32_t w) {
-    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
-    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0x0000FFFFu;
-    return w;
+__device__ inline float number(float x) { return x; }
+__device__ inline float number(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+
+// The 32 rows of a wave, or of a workgroup: row r of a sequence is head r % group of token r / group, so the heads that
+// share keys lie side by side and their rows end at the same key.
+struct Rows {
+    uint32_t pos, lo;      // of the lane's row: its token, and the first key that it sees
+    uint32_t first, last;  // tokens of the 32 rows
+    uint32_t head;
+    bool exists;
+    Rows() = default;
+    __device__ inline Rows(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row0) {
+        const uint32_t col = threadIdx.x & 31u, all = it.len * a.group;
+        const uint32_t r = min(row0 + col, all - 1u);
+        exists = row0 + col < all;
+        pos = r / a.group;
+        head = kv_head * a.group + r - pos * a.group;
+        lo = from(a, pos);
+        first = min(row0, all - 1u) / a.group;
+        last = min(row0 + kRows - 1u, all - 1u) / a.group;
+    }
+    static __device__ inline uint32_t from(const PromptArgs& a, uint32_t token) {
+        return a.window && token + 1u > a.window ? token + 1u - a.window : 0u;
+    }
+    // Whether some row sees some of n keys from base on, and whether all rows see all of them
+    __device__ inline bool some(const PromptArgs& a, uint32_t base, uint32_t n) const { return base <= last && base + n > from(a, first); }
+    __device__ inline bool all(const PromptArgs& a, uint32_t base, uint32_t n) const { return base + n <= first + 1u && base >= from(a, last); }
+};
+
+// DW columns of one row again, by one wave, where the products gave a number that is not finite. An infinite or NaN value turns
+// every row of its tile to NaN, also those that do not see it, as its weight is 0 there; here such values are added as
+// they are to the rows that see them. A lane takes a key for the scores and a column of 64 for the values.
+template <int D, int DW, class E>
+__device__ inline void redo_row(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row, uint32_t column) {
+    const uint32_t lane = threadIdx.x & 63u, token = row / a.group, head = kv_head * a.group + row - token * a.group;
+    const uint32_t lo = Rows::from(a, token);
+    const E* q = static_cast<const E*>(a.q) + (uint64_t)(it.first + token) * a.q_stride + (uint64_t)head * D;
+    const E* k = static_cast<const E*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
+    const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D + column;
+    float m = kNegInf, l = 0.0f, sum[DW / 64];
+#pragma unroll
+    for (int i = 0; i < DW / 64; ++i) sum[i] = 0.0f;
+#pragma nounroll
+    for (uint32_t base = lo; base <= token; base += 64u) {
+        const E* key = k + (uint64_t)min(base + lane, token) * a.k_stride;
+        float s = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < D; ++i) s = fmaf(number(q[i]), number(key[i]), s);
+        if (a.flip) s = -s;
+        s = base + lane <= token ? s * a.scale_log2e : kNegInf;
+        const float now = fmaxf(m, wave_max(s)), zero = now == kNegInf ? 0.0f : now;
+        const float alpha = __builtin_amdgcn_exp2f(m - zero), p = __builtin_amdgcn_exp2f(s - zero);
+        m = now;
+        l = l * alpha + wave_sum(p);
+#pragma unroll
+        for (int i = 0; i < DW / 64; ++i) sum[i] *= alpha;
+#pragma nounroll
+        for (uint32_t j = 0; j < min(64u, token + 1u - base); ++j) {
+            const float w = lane_read(p, (int)j);
+#pragma unroll
+            for (int i = 0; i < DW / 64; ++i) {
+                const float x = number(v[(uint64_t)(base + j) * a.v_stride + i * 64 + lane]);
+                sum[i] = not_finite(x) ? sum[i] + x : fmaf(w, x, sum[i]);
+            }
+        }
+    }
+    E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token) * a.out_stride + (uint64_t)head * D + column + lane;
+#pragma unroll
+    for (int i = 0; i < DW / 64; ++i) {
+        if constexpr (sizeof(E) == 4) to[i * 64] = sum[i] / l;
+        else to[i * 64] = (uint16_t)pack_bf16(sum[i] / l, 0.0f);
+    }
 }
 
+// Few rows: a workgroup takes 32 of them. Its four waves take the blocks of 32 keys in turn, each with its own maximum
+// and sums, and join at the end.
 template <int D, bool F32>
-struct Shared {
+struct Few {
     union {
         float4 q[F32 ? D / 8 : 1][64];                 // FP32 queries as second operands
         uint4 v[F32 ? 1 : kWaves][kKeys * D / 8];      // a wave's block of BF16 values, [key][D]
         float sums[kWaves][kRows][68];
     };
     float m[kWaves][kRows], l[kWaves][kRows];
+    uint32_t odd;  // rows whose result is not finite
 };
 
 template <int D, bool F32>
-__global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_prompt(const PromptArgs a) {
-    __shared__ Shared<D, F32> sh;
+__global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const PromptArgs a) {
+    typedef typename std::conditional<F32, float, uint16_t>::type E;
+    __shared__ Few<D, F32> sh;
     const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // heads change fastest, the key/value heads before the heads that share one
-    const uint32_t turn = blockIdx.x % a.q_heads, kv_head = turn % a.kv_heads, head = kv_head * a.group + turn / a.kv_heads;
-    const Item it = locate(a, blockIdx.x / a.q_heads, kRows);
+    const uint32_t kv_head = blockIdx.x % a.kv_heads;
+    const Item it = locate(a, blockIdx.x / a.kv_heads, kRows);
     if (!it.exists) return;
-    const uint32_t row0 = it.tile * kRows, pos = row0 + col, last = it.len - 1u;
-    const uint32_t end = min(it.len, row0 + kRows);
-    const uint32_t begin = a.window && row0 + 1u > a.window ? row0 + 1u - a.window : 0u;
-    const uint32_t lo = a.window && pos + 1u > a.window ? pos + 1u - a.window : 0u;  // what this lane's row sees: lo .. pos
-    // rows from full0 .. full1 on see every key of a block that lies between them
-    const uint32_t all_lo = a.window && end > a.window ? end - a.window : 0u;
-
-    typedef typename std::conditional<F32, float, uint16_t>::type E;
-    const E* q = static_cast<const E*>(a.q) + (uint64_t)(it.first + min(pos, last)) * a.q_stride + (uint64_t)head * D;
+    const uint32_t last = it.len - 1u;
+    const Rows rows(a, it, kv_head, it.tile * kRows);
+    const uint32_t begin = Rows::from(a, rows.first), end = rows.last + 1u;
+    const E* q = static_cast<const E*>(a.q) + (uint64_t)(it.first + rows.pos) * a.q_stride + (uint64_t)rows.head * D;
     const E* k = static_cast<const E*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
     const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D;
 
     Frag qf[F32 ? 1 : D / 16];
-    if constexpr (F32) {
-        for (int i = wave; i < D / 8; i += kWaves) {
-            uint4 x = *reinterpret_cast<const uint4*>(q + i * 8 + half * 4u);
-            x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
-            sh.q[i][lane] = __builtin_bit_cast(float4, x);
-        }
-        __syncthreads();
-    } else {
+    if constexpr (!F32) {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             qf[i].u = *reinterpret_cast<const uint4*>(q + i * 16 + half * 8u);
@@ -195,130 +258,101 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_prompt(const Pro
             for (int j = 0; j < 4; ++j) qf[i].w[j] ^= a.flip;
         }
     }
-
     f32x16 o[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = zeros();
     Softmax sm;
-
-    for (uint32_t base = begin / kKeys * kKeys + wave * kKeys; base < end; base += kWaves * kKeys) {
-        const bool masked = base < all_lo || base + kKeys > row0 + 1u;
-        // ---- scores
-        const E* krow = k + (uint64_t)min(base + col, last) * a.k_stride;
-        f32x16 s = zeros();
+    {
         if constexpr (F32) {
+            for (int i = wave; i < D / 8; i += kWaves) {
+                uint4 x = *reinterpret_cast<const uint4*>(q + i * 8 + half * 4u);
+                x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
+                sh.q[i][lane] = __builtin_bit_cast(float4, x);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] = zeros();
+        sm = Softmax();
+        for (uint32_t base = begin / kKeys * kKeys + wave * kKeys; base < end; base += kWaves * kKeys) {
+            // ---- scores
+            const E* krow = k + (uint64_t)min(base + col, last) * a.k_stride;
+            f32x16 s[1] = {zeros()};
+            if constexpr (F32) {
 #pragma unroll 8
-            for (int i = 0; i < D / 8; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(krow + i * 8 + half * 4u), y = sh.q[i][lane];
-                s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s, 0, 0, 0);
-            }
-        } else {
-            // the values' block on its way to LDS meanwhile, whole rows of D
-            constexpr int kLoads = kKeys * D / 512;
-            uint4 held[kLoads];
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const uint32_t at = i * 512u + lane * 8u, row = at / D;
-                held[i] = *reinterpret_cast<const uint4*>(v + (uint64_t)min(base + row, last) * a.v_stride + at % D);
-            }
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                Frag x;
-                x.u = *reinterpret_cast<const uint4*>(krow + i * 16 + half * 8u);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, qf[i].b, s, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) sh.v[wave][i * 64u + lane] = held[i];
-        }
-        if (masked) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const uint32_t key = base + element(r, half);
-                if (key < lo || key > pos) s[r] = kNegInf;
-            }
-        }
-        // ---- weights
-        float alpha;
-        if (sm.weights(s, a.scale_log2e, alpha)) {
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
-        }
-        // ---- weighted values. A value that is infinite or NaN has no part in a row that does not see it, where
-        // its weight is 0: such values are taken out of the product and added to the rows that see them.
-        bool odd = false;
-        if constexpr (F32) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const E* vrow = v + (uint64_t)min(base + element(r, half), last) * a.v_stride + col;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    float x = vrow[i * 32];
-                    if (masked && not_finite(x)) odd = true, x = 0.0f;
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[r], o[i], 0, 0, 0);
+                for (int i = 0; i < D / 8; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(krow + i * 8 + half * 4u), y = sh.q[i][lane];
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s[0], 0, 0, 0);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s[0], 0, 0, 0);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s[0], 0, 0, 0);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s[0], 0, 0, 0);
                 }
-            }
-        } else {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            Frag p[2];
+            } else {
+                constexpr int kLoads = kKeys * D / 512;  // the values' block on its way to LDS meanwhile
+                uint4 held[kLoads];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j >> 2].w[j & 3] = pack_bf16(s[2 * j], s[2 * j + 1]);
-            if (masked) {
-                bool any = false;
-#pragma unroll 4
-                for (int i = 0; i < (int)kKeys * D / 512; ++i) {
-                    const uint4 x = sh.v[wave][i * 64u + lane];
-                    any = any || odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w);
+                for (int i = 0; i < kLoads; ++i) {
+                    const uint32_t at = i * 512u + lane * 8u, row = at / D;
+                    held[i] = *reinterpret_cast<const uint4*>(v + (uint64_t)min(base + row, last) * a.v_stride + at % D);
                 }
-                odd = __any(any);
-            }
-            // keys 4 half .. and 8 + 4 half .. of 16, columns col of 32: 16 lanes read four keys of 16 columns and
-            // get a column each
-            const uint16_t* vs = reinterpret_cast<const uint16_t*>(sh.v[wave]) + (4u * half + ((lane & 15u) >> 2)) * D + (lane & 16u) + (lane & 3u) * 4u;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int i = 0; i < D / 16; ++i) {
                     Frag x;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) short4v*)(vs + (16 * j + 8 * e) * D + i * 32));
-                    if (odd) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x.w[e] = clean_pair(x.w[e]);
-                    }
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, p[j].b, o[i], 0, 0, 0);
+                    x.u = *reinterpret_cast<const uint4*>(krow + i * 16 + half * 8u);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, qf[i].b, s[0], 0, 0, 0);
                 }
-        }
-        if (masked && __any(odd)) {
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i)
+                for (int i = 0; i < kLoads; ++i) sh.v[wave][i * 64u + lane] = held[i];
+            }
+            if (!rows.all(a, base, kKeys)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float add = 0.0f;
-#pragma unroll 1
-                    for (uint32_t j = 0; j < kKeys; ++j) {
-                        const uint32_t key = base + j;
-                        if (key < lo || key > pos || key > last) continue;
-                        const E x = v[(uint64_t)key * a.v_stride + i * 32 + element(r, half)];
-                        float y;
-                        if constexpr (F32) y = x;
-                        else y = __uint_as_float((uint32_t)x << 16);
-                        if (not_finite(y)) add += y;
-                    }
-                    o[i][r] += add;
+                    const uint32_t key = base + element(r, half);
+                    if (key < rows.lo || key > rows.pos) s[0][r] = kNegInf;
                 }
+            }
+            // ---- weights
+            float alpha;
+            if (sm.weights(s, a.scale_log2e, alpha)) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+            }
+            // ---- weighted values
+            if constexpr (F32) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const E* vrow = v + (uint64_t)min(base + element(r, half), last) * a.v_stride + col;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[i * 32], s[0][r], o[i], 0, 0, 0);
+                }
+            } else {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                Frag p[2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j >> 2].w[j & 3] = pack_bf16(s[0][2 * j], s[0][2 * j + 1]);
+                // keys 4 half .. and 8 + 4 half .. of 16, columns col of 32: 16 lanes read four keys of 16 columns and
+                // get a column each
+                const uint16_t* vs = reinterpret_cast<const uint16_t*>(sh.v[wave]) + (4u * half + ((lane & 15u) >> 2)) * D + (lane & 16u) + (lane & 3u) * 4u;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        Frag x;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) short4v*)(vs + (16 * j + 8 * e) * D + i * 32));
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, p[j].b, o[i], 0, 0, 0);
+                    }
+            }
         }
     }
 
     // ---- the four waves join
     sm.l = halves_sum(sm.l);
     if (half == 0u) sh.m[wave][col] = sm.m, sh.l[wave][col] = sm.l;
+    if (threadIdx.x == 0u) sh.odd = 0u;
     __syncthreads();
     float top = fmaxf(fmaxf(sh.m[0][col], sh.m[1][col]), fmaxf(sh.m[2][col], sh.m[3][col]));  // of the lane's row
     const float mine = sm.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sm.m - top);
@@ -331,6 +365,10 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_prompt(const Pro
     for (uint32_t w = 0; w < kWaves; ++w)
         if (sh.l[w][row] != 0.0f) total += sh.l[w][row] * __builtin_amdgcn_exp2f(sh.m[w][row] - top);
     const float by = 1.0f / total;
+    bool odd = false;
+    const uint32_t out_row = it.tile * kRows + row, token = out_row / a.group;
+    E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token) * a.out_stride +
+            (uint64_t)(kv_head * a.group + out_row - token * a.group) * D + c8;
 #pragma unroll
     for (int n = 0; n < D / 64; ++n) {
         __syncthreads();
@@ -350,37 +388,268 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_prompt(const Pro
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) x[i] += sh.sums[w][row][c8 + i];
             x[i] *= by;
+            odd = odd || not_finite(x[i]);
         }
-        if (row0 + row < it.len) {
-            E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + row0 + row) * a.out_stride + (uint64_t)head * D + n * 64u + c8;
+        if (token < it.len) {
             if constexpr (F32) {
-                *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                *reinterpret_cast<float4*>(to + n * 64) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(to + n * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
             } else {
-                *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                *reinterpret_cast<uint4*>(to + n * 64) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
             }
         }
     }
+    if (odd && token < it.len) atomicOr(&sh.odd, 1u << row);
+    __syncthreads();  // what was written is written over, in order
+    for (uint32_t left = sh.odd, n = 0; left; left &= left - 1u, ++n)
+        if (n % kWaves == wave) redo_row<D, D, E>(a, it, kv_head, it.tile * kRows + (uint32_t)__ffs(left) - 1u, 0u);
+}
+
+// Many rows: every wave has 32 RT rows of its own, and tiles of KT keys and values go from memory to LDS, without
+// passing registers, for all of them, one tile ahead. A row of a tile is D values, whose 16-byte chunks are exchanged
+// (chunk c lies at c ^ f(row)) so that neither the key reads, 16 bytes of 32 rows, nor the transposing value reads, 64
+// bytes of 8 rows, meet in a bank.
+template <int D, int KT, int W, int PARTS>
+struct Many {
+    uint16_t k[2][KT * D], v[2][KT * D];
+    float4 scores[PARTS > 1 ? W : 1][PARTS > 1 ? 4 : 1][64];
+};
+template <int D>
+__device__ inline uint32_t key_turn(uint32_t row) { return D >= 128 ? row & 15u : (row >> 1) & 7u; }
+template <int D>
+__device__ inline uint32_t value_turn(uint32_t row) {
+    const uint32_t r = row & 3u;
+    return (D >= 128 ? r | (r & 1u) << 2 : r) << 1;
+}
+
+// W waves in groups of PARTS, of which each has DW columns of the queries, keys, values and sums of its group's rows
+// (heads of 512: the registers of two waves per SIMD hold 256), softmax in steps of SK keys, WAVES waves per SIMD.
+template <int D, int W, int RT, int KT, int SK, int PARTS, int WAVES>
+__global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
+    constexpr int kBlocks = SK / 32, kLoads = KT * D / 512 / W;  // a wave's loads of 1 KB
+    constexpr uint32_t kChunks = D / 8, kLoadRows = 64 / kChunks, kStep = W * kLoadRows, R = 32 * RT * W / PARTS;
+    constexpr int DW = D / PARTS;  // columns of a wave
+    __shared__ __attribute__((aligned(1024))) Many<D, KT, W, PARTS> sh;
+    const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t kv_head = blockIdx.x % a.kv_heads;
+    const Item it = locate(a, blockIdx.x / a.kv_heads, R);
+    if (!it.exists) return;
+    const uint32_t all = it.len * a.group, row0 = it.tile * R, mine = row0 + wave / PARTS * 32u * RT, column = wave % PARTS * DW;
+    const uint32_t begin = Rows::from(a, row0 / a.group) / KT * KT, end = min(row0 + R - 1u, all - 1u) / a.group + 1u;
+    const uint16_t* k = static_cast<const uint16_t*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
+    const uint16_t* v = static_cast<const uint16_t*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D;
+
+    Rows rows[RT];
+    Frag qf[RT][DW / 16];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        rows[t] = Rows(a, it, kv_head, mine + t * 32u);
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (uint64_t)(it.first + rows[t].pos) * a.q_stride + (uint64_t)rows[t].head * D + column;
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) {
+            qf[t][i].u = *reinterpret_cast<const uint4*>(q + i * 16 + half * 8u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) qf[t][i].w[j] ^= a.flip;
+        }
+    }
+
+    // Load n of a wave fills rows (wave + W n) kLoadRows .. of a tile, lane l chunk l % kChunks of row l / kChunks of
+    // these. Rows past the sequence are its last row again.
+    const uint32_t load_row = wave * kLoadRows + lane / kChunks, chunk = lane % kChunks;
+    const uint32_t k_bytes = (uint32_t)a.k_stride * 2u, v_bytes = (uint32_t)a.v_stride * 2u;
+    auto fetch = [&](uint32_t base, uint32_t buf) {
+        const uint32_t there = min((uint32_t)KT, it.len - base);
+        const __amdgpu_buffer_rsrc_t kr =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(k + (uint64_t)base * a.k_stride), 0, (int)((there - 1u) * k_bytes + D * 2u), kBufDword3);
+        const __amdgpu_buffer_rsrc_t vr =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(v + (uint64_t)base * a.v_stride), 0, (int)((there - 1u) * v_bytes + D * 2u), kBufDword3);
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const uint32_t row = load_row + n * kStep, from = min(row, there - 1u);
+            const uint32_t at = (wave + W * n) * 512u;
+            buf_dma_16(kr, reinterpret_cast<unsigned char*>(sh.k[buf] + at), from * k_bytes + ((chunk ^ key_turn<D>(row)) * 16u), 0u);
+            buf_dma_16(vr, reinterpret_cast<unsigned char*>(sh.v[buf] + at), from * v_bytes + ((chunk ^ value_turn<D>(row)) * 16u), 0u);
+        }
+    };
+
+    f32x16 o[RT][DW / 32];
+    Softmax sm[RT];
+    // The operands of C products are read from LDS while the C before them run; without the barriers the compiler
+    // asks for all of a step's at once and spills.
+    constexpr int C = 4;
+    auto step = [&](uint32_t base, const uint16_t* kt, const uint16_t* vt) {
+        constexpr int kKeyReads = DW / 16 * kBlocks, kValueReads = DW / 32 * 2 * kBlocks;
+        const uint16_t* kp = kt + col * D + column;
+        const uint32_t turn = half ^ key_turn<D>(col);
+        auto key_read = [&](int n) {  // a chunk's number is exchanged in its low four bits (three for heads of 64)
+            constexpr uint32_t kLow = D >= 128 ? 16u : 8u;
+            const uint32_t i = 2u * (n / kBlocks);
+            Frag x;
+            x.u = *reinterpret_cast<const uint4*>(kp + (((i % kLow) ^ turn) * 8u) + (n % kBlocks) * 32 * D + i / kLow * kLow * 8u);
+            return x;
+        };
+        const uint32_t vrow = 4u * half + ((lane >> 2) & 3u), vchunk = ((lane >> 4) & 1u) * 2u + ((lane & 3u) >> 1);
+        const uint32_t vturn = vchunk ^ value_turn<D>(lane >> 2);
+        const uint16_t* vp = vt + vrow * D + column + (lane & 1u) * 4u;
+        auto value_read = [&](int n) {
+            Frag x;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                constexpr uint32_t kLow = D >= 128 ? 16u : 8u;
+                const uint32_t i = 4u * (n / (2 * kBlocks));
+                x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                    vp + (((i % kLow) ^ vturn) * 8u) + (16 * (n % (2 * kBlocks)) + 8 * e) * D + i / kLow * kLow * 8u));
+            }
+            return x;
+        };
+        f32x16 s[RT][kBlocks];
+        Frag x[2][C];
+#pragma unroll
+        for (int n = 0; n < C; ++n) x[0][n] = key_read(n);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) s[t][b] = zeros();
+#pragma unroll
+        for (int c = 0; c < kKeyReads / C; ++c) {
+#pragma unroll
+            for (int n = 0; n < C; ++n) x[(c + 1) & 1][n] = c + 1 < kKeyReads / C ? key_read((c + 1) * C + n) : value_read(n);
+#pragma unroll
+            for (int n = 0; n < C; ++n)
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    s[t][(c * C + n) % kBlocks] =
+                        __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, qf[t][(c * C + n) / kBlocks].b, s[t][(c * C + n) % kBlocks], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        static_assert(kKeyReads / C % 2 == 0);
+        if constexpr (PARTS > 1) {  // the two halves' products add up
+            static_assert(PARTS == 2 && RT == 1 && kBlocks == 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sh.scores[wave][e][lane] = make_float4(s[0][0][4 * e], s[0][0][4 * e + 1], s[0][0][4 * e + 2], s[0][0][4 * e + 3]);
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 y = sh.scores[wave ^ 1u][e][lane];
+                s[0][0][4 * e] += y.x, s[0][0][4 * e + 1] += y.y, s[0][0][4 * e + 2] += y.z, s[0][0][4 * e + 3] += y.w;
+            }
+        }
+        Frag p[RT][2 * kBlocks];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if (!rows[t].all(a, base, SK)) {
+                asm volatile("");  // a branch, not selects: few blocks are not seen whole
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t key = base + 32u * b + element(r, half);
+                        if (key < rows[t].lo || key > rows[t].pos) s[t][b][r] = kNegInf;
+                    }
+            }
+            float alpha;
+            if (sm[t].weights(s[t], a.scale_log2e, alpha)) {
+#pragma unroll
+                for (int i = 0; i < DW / 32; ++i) o[t][i] *= alpha;
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[t][2 * b + (j >> 2)].w[j & 3] = pack_bf16(s[t][b][2 * j], s[t][b][2 * j + 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < kValueReads / C; ++c) {
+            if (c + 1 < kValueReads / C) {
+#pragma unroll
+                for (int n = 0; n < C; ++n) x[(c + 1) & 1][n] = value_read((c + 1) * C + n);
+            }
+#pragma unroll
+            for (int n = 0; n < C; ++n)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    f32x16& to = o[t][(c * C + n) / (2 * kBlocks)];
+                    to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, p[t][(c * C + n) % (2 * kBlocks)].b, to, 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+#pragma unroll
+        for (int i = 0; i < DW / 32; ++i) o[t][i] = zeros();
+    }
+    fetch(begin, 0u);
+    for (uint32_t base = begin, buf = 0; base < end; base += KT, buf ^= 1u) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile is there
+        __syncthreads();                     // the others' too, and nobody reads the other buffer any more
+        if (base + KT < end) fetch(base + KT, buf ^ 1u);
+#pragma unroll 1
+        for (uint32_t at = 0; at < KT; at += SK) {
+            bool some = false;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) some = some || rows[t].some(a, base + at, SK);
+            if (PARTS > 1 || (some && mine < all)) step(base + at, sh.k[buf] + at * D, sh.v[buf] + at * D);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float by = 1.0f / halves_sum(sm[t].l);
+        uint16_t* to = static_cast<uint16_t*>(a.out) + (uint64_t)(it.first + rows[t].pos) * a.out_stride + (uint64_t)rows[t].head * D + column + half * 4u;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < DW / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x16 x = o[t][i];
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = x[r + e] * by, odd = odd || not_finite(y[e]);
+                if (rows[t].exists) *reinterpret_cast<uint2*>(to + i * 32 + 2 * r) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+            }
+        const unsigned long long both = __ballot(odd && rows[t].exists);
+        for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
+            redo_row<D, DW, uint16_t>(a, it, kv_head, mine + t * 32u + (uint32_t)__ffs(left) - 1u, column);
+    }
+}
+
+// As many workgroups as tiles of `rows` rows that the sequences can have (all but one row of each one's last may be
+// missing) over all key/value heads.
+uint32_t items_of(const PromptArgs& a, uint32_t rows) {
+    return grid_blocks(((uint64_t)a.tokens * a.group + (uint64_t)a.batch * (rows - 1u)) / rows * a.kv_heads);
+}
+
+template <int D, bool F32>
+void launch_few(const PromptArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_few<D, F32>), dim3(items_of(a, kRows)), dim3(kThreads), 0, st, a);
+}
+
+template <int D, int W, int RT, int KT, int SK, int PARTS, int WAVES>
+void launch_many(const PromptArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_many<D, W, RT, KT, SK, PARTS, WAVES>), dim3(items_of(a, 32u * RT * W / PARTS)), dim3(64 * W), 0, st, a);
 }
 
 template <int D>
-void launch_dim(const PromptArgs& a, int dtype, uint32_t items, hipStream_t st) {
-    if (dtype == TURBO_HIDDEN_F32) hipLaunchKernelGGL((k_prompt<D, true>), dim3(items), dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((k_prompt<D, false>), dim3(items), dim3(kThreads), 0, st, a);
+void launch_dim(const PromptArgs& a, int dtype, uint32_t cus, hipStream_t st) {
+    if (dtype == TURBO_HIDDEN_F32) return launch_few<D, true>(a, st);
+    if constexpr (D <= 128)
+        if (items_of(a, 128u) < cus) return launch_few<D, false>(a, st);
+    if constexpr (D == 64) return launch_many<D, 4, 1, 64, 64, 1, 3>(a, st);
+    if constexpr (D == 128) return launch_many<D, 4, 1, 64, 64, 1, 2>(a, st);
+    if constexpr (D == 256) return launch_many<D, 4, 1, 32, 32, 1, 2>(a, st);
+    if constexpr (D == 512) return launch_many<D, 8, 1, 32, 32, 2, 2>(a, st);
 }
 
 }  // namespace
 
 void launch_prompt(const PromptArgs& a, uint32_t head_dim, int dtype, uint32_t cus, hipStream_t st) {
-    (void)cus;
-    // as many tiles as the sequences can have: all but one row of each sequence's last tile may be missing
-    const uint64_t tiles = ((uint64_t)a.tokens + (uint64_t)a.batch * (kRows - 1u)) / kRows;
-    const uint32_t items = grid_blocks(tiles * a.q_heads);
     switch (head_dim) {
-        case 64u: launch_dim<64>(a, dtype, items, st); break;
-        case 128u: launch_dim<128>(a, dtype, items, st); break;
-        case 256u: launch_dim<256>(a, dtype, items, st); break;
-        default: launch_dim<512>(a, dtype, items, st); break;
+        case 64u: launch_dim<64>(a, dtype, cus, st); break;
+        case 128u: launch_dim<128>(a, dtype, cus, st); break;
+        case 256u: launch_dim<256>(a, dtype, cus, st); break;
+        default: launch_dim<512>(a, dtype, cus, st); break;
     }
     check_hip(hipGetLastError(), "prompt attention");
 }

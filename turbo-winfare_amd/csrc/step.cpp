@@ -31,13 +31,13 @@ void check_words(const char* name, const void* p, uintptr_t align = 4u) {
 }
 
 // The page tables and the pool, as the plan and the release take them.
-void check_pool(uint32_t page_stride, const void* pages, const void* held, const void* free_pages, const void* free_count,
-                uint32_t prefix_len) {
+void check_pool(int batch, uint32_t page_stride, const void* pages, const void* held, const void* free_pages, uint32_t free_capacity,
+                const void* free_count, uint32_t prefix_len) {
     if (page_stride > 0x7FFFFFFFu) fail("page_stride is above 2^31 - 1");
     if (prefix_len > 0x7FFFFF00u) fail("prefix_len must be at most 2^31 - 256");
-    if (page_stride) check_words("pages", pages);
-    check_words("held", held);
-    check_words("free_pages", free_pages);
+    if (batch && page_stride) check_words("pages", pages);
+    if (batch) check_words("held", held);
+    if (free_capacity) check_words("free_pages", free_pages);
     check_words("free_count", free_count);
 }
 
@@ -66,10 +66,12 @@ TURBO_DT_API int turbo_batch_plan(const TurboBatchPlan* in, void* hip_stream) {
     if (in->row_tokens && in->max_tokens != (uint64_t)in->batch * in->row_tokens) fail("max_tokens must be batch * row_tokens");
     if (in->parents) tree_rows(in->row_tokens);
     else if (in->masks) fail("masks need parents");
-    check_words("past_len", in->past_len);
-    check_words("new_len", in->new_len);
-    check_pool(in->page_stride, in->pages, in->held, in->free_pages, in->free_count, in->prefix_len);
-    check_words("held_out", in->held_out);
+    if (in->batch) {  // otherwise arrays of no sequences
+        check_words("past_len", in->past_len);
+        check_words("new_len", in->new_len);
+        check_words("held_out", in->held_out);
+    }
+    check_pool(in->batch, in->page_stride, in->pages, in->held, in->free_pages, in->free_capacity, in->free_count, in->prefix_len);
     check_words("free_count_out", in->free_count_out);
     if (in->masks) check_words("masks", in->masks, 8u);
     for (const void* p : {static_cast<const void*>(in->parents), static_cast<const void*>(in->starts), static_cast<const void*>(in->kv_len),
@@ -109,10 +111,10 @@ TURBO_DT_API int turbo_pages_release(const TurboPagesRelease* in, void* hip_stre
     ReleaseArgs a{};
     check_batch(in->batch);
     a.page_shift = page_shift(in->page_tokens);
-    check_words("keep_len", in->keep_len);
-    check_pool(in->page_stride, in->pages, in->held, in->free_pages, in->free_count, in->prefix_len);
-    check_device(in->device);
     if (in->batch == 0) return 1;
+    check_words("keep_len", in->keep_len);
+    check_pool(in->batch, in->page_stride, in->pages, in->held, in->free_pages, in->free_capacity, in->free_count, in->prefix_len);
+    check_device(in->device);
     a.batch = (uint32_t)in->batch;
     a.prefix_len = in->prefix_len;
     a.page_stride = in->page_stride;
@@ -134,6 +136,7 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream) 
     AcceptArgs a{};
     if (in->batch < 0 || in->batch > (1 << 20)) fail("batch must be in 0..1048576");
     a.row_tokens = tree_rows(in->row_tokens);
+    if (in->batch == 0) return 1;
     check_words("parents", in->parents);
     check_words("new_len", in->new_len);
     check_words("tokens", in->tokens);
@@ -147,7 +150,6 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream) 
                           static_cast<const void*>(in->target)})
         if (reinterpret_cast<uintptr_t>(p) % 4u != 0u) fail("an array of the tree is not 4-byte aligned");
     check_device(in->device);
-    if (in->batch == 0) return 1;
     a.batch = (uint32_t)in->batch;
     a.parents = in->parents;
     a.add = in->new_len;
@@ -179,6 +181,7 @@ TURBO_DT_API int turbo_prompt_attention(const TurboPromptInputs* in, void* hip_s
         fail("q_heads must be a multiple of kv_heads, at most " + std::to_string(kMaxQueryHeads));
     const double scale = (double)in->scale * 1.4426950408889634;
     if (!(std::fabs(scale) <= (double)FLT_MAX)) fail("scale must be finite and below 2^127");
+    if ((uint64_t)in->tokens * (uint64_t)(in->q_heads / in->kv_heads) > (1ull << 31) - 65536u) fail("tokens * q_heads / kv_heads is too large for one call");
     if (in->batch == 0 || in->tokens == 0) return 1;
     PromptArgs a{};
     const size_t q_packed = (size_t)in->q_heads * in->head_dim, kv_packed = (size_t)in->kv_heads * in->head_dim;

@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void k_accept(const AcceptArgs a) {
     const uint32_t n = min(a.add[b], a.row_tokens);
     const bool node = lane < n;
     const int above = node ? a.parents[at] : -2;
-    const uint32_t token = node ? a.tokens[at] : 0u, chosen = node ? a.chosen[at] : kNone, slot = in ? a.slots[at] : kNone;
+    const uint32_t token = node ? a.tokens[at] : 0u, chosen = node ? a.chosen[at] : kNone, slot = in && a.slots ? a.slots[at] : kNone;
     uint32_t kept = 0, next = kNone, mine = kNone;  // mine: the node that is number `lane` of the path
     unsigned long long found = __ballot(lane == 0u && above == -1);
     while (found) {
