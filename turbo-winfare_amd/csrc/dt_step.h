@@ -16,7 +16,8 @@ struct PlanArgs {
     uint32_t* pages;
     uint32_t *held_out, *free_out, *starts, *kv_len, *positions, *slots, *totals;
     uint64_t* masks;
-    int tokens, state;  // what a launch writes: the tokens' and pages' entries, the sequences' and the pool's
+    uint32_t tokens, pages_from;  // workgroups of the tokens' entries, and the first that writes pages
+    int state;                    // the last one writes the lengths and the pool after the step
 };
 void launch_plan(PlanArgs a, hipStream_t st);
 

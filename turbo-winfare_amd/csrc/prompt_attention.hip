@@ -25,8 +25,11 @@ constexpr uint32_t kRows = 32, kKeys = 32;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;  // a weight is at most 2^kSlack before the maximum moves
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 union Frag {
     uint4 u;
+    u32x4 x;
     uint32_t w[4];
     bf16x8 b;
     short4v h[2];
@@ -156,7 +159,6 @@ struct Rows {
     uint32_t first, last;  // tokens of the 32 rows
     uint32_t head;
     bool exists;
-    Rows() = default;
     __device__ inline Rows(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row0) {
         const uint32_t col = threadIdx.x & 31u, all = it.len * a.group;
         const uint32_t r = min(row0 + col, all - 1u);
@@ -409,6 +411,24 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const Prompt
 // passing registers, for all of them, one tile ahead. A row of a tile is D values, whose 16-byte chunks are exchanged
 // (chunk c lies at c ^ f(row)) so that neither the key reads, 16 bytes of 32 rows, nor the transposing value reads, 64
 // bytes of 8 rows, meet in a bank.
+// Memory that a wave's buffer-to-LDS loads read, 16 bytes to a lane at its byte offset, 1 KB side by side in LDS. They are
+// written as assembly because the compiler takes every later LDS read for one of theirs and waits for them there, before
+// the tile in hand is begun (2,096 us for 16,384 tokens with heads of 128). The wait is the caller's, before the barrier in
+// front of the tile. A load has no result register; its address register is read at issue.
+struct TileSource {
+    u32x4 words;
+    __device__ inline TileSource(const void* p, uint32_t bytes) {
+        const uint64_t at = reinterpret_cast<uint64_t>(p);
+        words = u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufDword3};
+    }
+    __device__ inline void load(uint16_t* lds, uint32_t offset) const {
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)lds);
+        // five wait states between a scalar register that the vector unit wrote and its use by a buffer load, one behind
+        // M0, which nothing else here uses
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(words) : "memory");
+    }
+};
 template <int D, int KT, int W, int PARTS>
 struct Many {
     uint16_t k[2][KT * D], v[2][KT * D];
@@ -421,145 +441,143 @@ __device__ inline uint32_t value_turn(uint32_t row) {
     const uint32_t r = row & 3u;
     return (D >= 128 ? r | (r & 1u) << 2 : r) << 1;
 }
+template <class T>
+__device__ inline uint32_t lds_at(T* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)p; }
 
-// W waves in groups of PARTS, of which each has DW columns of the queries, keys, values and sums of its group's rows
-// (heads of 512: the registers of two waves per SIMD hold 256), softmax in steps of SK keys, WAVES waves per SIMD.
-template <int D, int W, int RT, int KT, int SK, int PARTS, int WAVES>
+// W waves in pairs (PARTS 2) or alone, of which each has DW columns of the queries, keys, values and sums of 32 rows:
+// the registers of two waves per SIMD hold 256. WAVES waves per SIMD; C operands are read from LDS while the C products
+// before them run.
+template <int D, int W, int KT, int PARTS, int C, int WAVES>
 __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
-    constexpr int kBlocks = SK / 32, kLoads = KT * D / 512 / W;  // a wave's loads of 1 KB
-    constexpr uint32_t kChunks = D / 8, kLoadRows = 64 / kChunks, kStep = W * kLoadRows, R = 32 * RT * W / PARTS;
-    constexpr int DW = D / PARTS;  // columns of a wave
+    constexpr int DW = D / PARTS, kBlocks = KT / 32, kLoads = KT * D / 512 / W;  // kLoads: a wave's loads of 1 KB
+    constexpr uint32_t kChunks = D / 8, kLoadRows = 64 / kChunks, kStep = W * kLoadRows, R = 32 * W / PARTS;
     __shared__ __attribute__((aligned(1024))) Many<D, KT, W, PARTS> sh;
     const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
     const Item it = locate(a, blockIdx.x / a.kv_heads, R);
     if (!it.exists) return;
-    const uint32_t all = it.len * a.group, row0 = it.tile * R, mine = row0 + wave / PARTS * 32u * RT, column = wave % PARTS * DW;
+    const uint32_t all = it.len * a.group, row0 = it.tile * R, mine = row0 + wave / PARTS * 32u, column = wave % PARTS * DW;
     const uint32_t begin = Rows::from(a, row0 / a.group) / KT * KT, end = min(row0 + R - 1u, all - 1u) / a.group + 1u;
     const uint16_t* k = static_cast<const uint16_t*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
     const uint16_t* v = static_cast<const uint16_t*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D;
-
-    Rows rows[RT];
-    Frag qf[RT][DW / 16];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        rows[t] = Rows(a, it, kv_head, mine + t * 32u);
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (uint64_t)(it.first + rows[t].pos) * a.q_stride + (uint64_t)rows[t].head * D + column;
-#pragma unroll
-        for (int i = 0; i < DW / 16; ++i) {
-            qf[t][i].u = *reinterpret_cast<const uint4*>(q + i * 16 + half * 8u);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) qf[t][i].w[j] ^= a.flip;
-        }
-    }
 
     // Load n of a wave fills rows (wave + W n) kLoadRows .. of a tile, lane l chunk l % kChunks of row l / kChunks of
     // these. Rows past the sequence are its last row again.
     const uint32_t load_row = wave * kLoadRows + lane / kChunks, chunk = lane % kChunks;
     const uint32_t k_bytes = (uint32_t)a.k_stride * 2u, v_bytes = (uint32_t)a.v_stride * 2u;
-    auto fetch = [&](uint32_t base, uint32_t buf) {
+    auto fetch_keys = [&](uint32_t base, uint16_t* to) {
         const uint32_t there = min((uint32_t)KT, it.len - base);
-        const __amdgpu_buffer_rsrc_t kr =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(k + (uint64_t)base * a.k_stride), 0, (int)((there - 1u) * k_bytes + D * 2u), kBufDword3);
-        const __amdgpu_buffer_rsrc_t vr =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(v + (uint64_t)base * a.v_stride), 0, (int)((there - 1u) * v_bytes + D * 2u), kBufDword3);
+        const TileSource from(k + (uint64_t)base * a.k_stride, (there - 1u) * k_bytes + D * 2u);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
-            const uint32_t row = load_row + n * kStep, from = min(row, there - 1u);
-            const uint32_t at = (wave + W * n) * 512u;
-            buf_dma_16(kr, reinterpret_cast<unsigned char*>(sh.k[buf] + at), from * k_bytes + ((chunk ^ key_turn<D>(row)) * 16u), 0u);
-            buf_dma_16(vr, reinterpret_cast<unsigned char*>(sh.v[buf] + at), from * v_bytes + ((chunk ^ value_turn<D>(row)) * 16u), 0u);
+            const uint32_t row = load_row + n * kStep;
+            from.load(to + (wave + W * n) * 512u, min(row, there - 1u) * k_bytes + ((chunk ^ key_turn<D>(row)) * 16u));
         }
     };
-
-    f32x16 o[RT][DW / 32];
-    Softmax sm[RT];
-    // The operands of C products are read from LDS while the C before them run; without the barriers the compiler
-    // asks for all of a step's at once and spills.
-    constexpr int C = 4;
-    auto step = [&](uint32_t base, const uint16_t* kt, const uint16_t* vt) {
-        constexpr int kKeyReads = DW / 16 * kBlocks, kValueReads = DW / 32 * 2 * kBlocks;
-        const uint16_t* kp = kt + col * D + column;
-        const uint32_t turn = half ^ key_turn<D>(col);
-        auto key_read = [&](int n) {  // a chunk's number is exchanged in its low four bits (three for heads of 64)
-            constexpr uint32_t kLow = D >= 128 ? 16u : 8u;
-            const uint32_t i = 2u * (n / kBlocks);
-            Frag x;
-            x.u = *reinterpret_cast<const uint4*>(kp + (((i % kLow) ^ turn) * 8u) + (n % kBlocks) * 32 * D + i / kLow * kLow * 8u);
-            return x;
-        };
-        const uint32_t vrow = 4u * half + ((lane >> 2) & 3u), vchunk = ((lane >> 4) & 1u) * 2u + ((lane & 3u) >> 1);
-        const uint32_t vturn = vchunk ^ value_turn<D>(lane >> 2);
-        const uint16_t* vp = vt + vrow * D + column + (lane & 1u) * 4u;
-        auto value_read = [&](int n) {
-            Frag x;
+    auto fetch_values = [&](uint32_t base, uint16_t* to) {
+        const uint32_t there = min((uint32_t)KT, it.len - base);
+        const TileSource from(v + (uint64_t)base * a.v_stride, (there - 1u) * v_bytes + D * 2u);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                constexpr uint32_t kLow = D >= 128 ? 16u : 8u;
-                const uint32_t i = 4u * (n / (2 * kBlocks));
-                x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
-                    vp + (((i % kLow) ^ vturn) * 8u) + (16 * (n % (2 * kBlocks)) + 8 * e) * D + i / kLow * kLow * 8u));
-            }
-            return x;
-        };
-        f32x16 s[RT][kBlocks];
-        Frag x[2][C];
+        for (int n = 0; n < kLoads; ++n) {
+            const uint32_t row = load_row + n * kStep;
+            from.load(to + (wave + W * n) * 512u, min(row, there - 1u) * v_bytes + ((chunk ^ value_turn<D>(row)) * 16u));
+        }
+    };
+    fetch_keys(begin, sh.k[0]);
+    fetch_values(begin, sh.v[0]);
+
+    const Rows rows(a, it, kv_head, mine);
+    Frag qf[DW / 16];
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (uint64_t)(it.first + rows.pos) * a.q_stride + (uint64_t)rows.head * D + column;
+#pragma unroll
+    for (int i = 0; i < DW / 16; ++i) {
+        qf[i].u = *reinterpret_cast<const uint4*>(q + i * 16 + half * 8u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[i].w[j] ^= a.flip;
+    }
+
+    // Where a lane's operands lie in buffer 0. A chunk's number is exchanged in its low four bits (three for heads of 64),
+    // so the addresses repeat after kKeyTurns key reads and kValueTurns values' blocks of 32.
+    constexpr int kKeyTurns = D >= 128 ? 8 : 4, kValueTurns = D >= 128 ? 4 : 2;
+    uint32_t key_at[kKeyTurns], value_at[kValueTurns];
+#pragma unroll
+    for (int i = 0; i < kKeyTurns; ++i) key_at[i] = lds_at(sh.k[0]) + (col * D + column) * 2u + (((2u * i) ^ half ^ key_turn<D>(col)) * 16u);
+#pragma unroll
+    for (int i = 0; i < kValueTurns; ++i)
+        value_at[i] = lds_at(sh.v[0]) + ((4u * half + ((lane >> 2) & 3u)) * D + column + (lane & 1u) * 4u) * 2u +
+                      ((4u * i ^ ((lane >> 4) & 1u) * 2u ^ ((lane & 3u) >> 1) ^ value_turn<D>(lane >> 2)) * 16u);
+    uint32_t buf_at = 0u;  // of the tile in hand
+    auto key_read = [&](int n) {
+        const int i = n / kBlocks;
+        Frag x;
+        x.x = *(const __attribute__((address_space(3))) u32x4*)(key_at[i % kKeyTurns] + buf_at +
+                                                                 (uint32_t)(n % kBlocks * 32 * D * 2 + i / kKeyTurns * kKeyTurns * 32));
+        return x;
+    };
+    auto value_read = [&](int n) {
+        const int i = n / (2 * kBlocks);
+        Frag x;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                value_at[i % kValueTurns] + buf_at + (uint32_t)((16 * (n % (2 * kBlocks)) + 8 * e) * D * 2 + i / kValueTurns * kValueTurns * 64)));
+        return x;
+    };
+
+    f32x16 o[DW / 32], s[kBlocks];
+    Softmax sm;
+    Frag x[2][C], p[2 * kBlocks];
+    constexpr int kKeyReads = DW / 16 * kBlocks, kValueReads = DW / 32 * 2 * kBlocks;
+    static_assert(kKeyReads / C % 2 == 0 && kValueReads % C == 0);
+    // The sched_barriers keep the compiler from asking for all operands of a step at once, which spills.
+    auto scores = [&] {
 #pragma unroll
         for (int n = 0; n < C; ++n) x[0][n] = key_read(n);
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-            for (int t = 0; t < RT; ++t) s[t][b] = zeros();
+        for (int b = 0; b < kBlocks; ++b) s[b] = zeros();
 #pragma unroll
         for (int c = 0; c < kKeyReads / C; ++c) {
+            if (c + 1 < kKeyReads / C) {
 #pragma unroll
-            for (int n = 0; n < C; ++n) x[(c + 1) & 1][n] = c + 1 < kKeyReads / C ? key_read((c + 1) * C + n) : value_read(n);
+                for (int n = 0; n < C; ++n) x[(c + 1) & 1][n] = key_read((c + 1) * C + n);
+            }
 #pragma unroll
-            for (int n = 0; n < C; ++n)
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    s[t][(c * C + n) % kBlocks] =
-                        __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, qf[t][(c * C + n) / kBlocks].b, s[t][(c * C + n) % kBlocks], 0, 0, 0);
+            for (int n = 0; n < C; ++n) {
+                f32x16& to = s[(c * C + n) % kBlocks];
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, qf[(c * C + n) / kBlocks].b, to, 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        static_assert(kKeyReads / C % 2 == 0);
-        if constexpr (PARTS > 1) {  // the two halves' products add up
-            static_assert(PARTS == 2 && RT == 1 && kBlocks == 1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sh.scores[wave][e][lane] = make_float4(s[0][0][4 * e], s[0][0][4 * e + 1], s[0][0][4 * e + 2], s[0][0][4 * e + 3]);
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float4 y = sh.scores[wave ^ 1u][e][lane];
-                s[0][0][4 * e] += y.x, s[0][0][4 * e + 1] += y.y, s[0][0][4 * e + 2] += y.z, s[0][0][4 * e + 3] += y.w;
-            }
-        }
-        Frag p[RT][2 * kBlocks];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            if (!rows[t].all(a, base, SK)) {
-                asm volatile("");  // a branch, not selects: few blocks are not seen whole
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const uint32_t key = base + 32u * b + element(r, half);
-                        if (key < rows[t].lo || key > rows[t].pos) s[t][b][r] = kNegInf;
-                    }
-            }
-            float alpha;
-            if (sm[t].weights(s[t], a.scale_log2e, alpha)) {
-#pragma unroll
-                for (int i = 0; i < DW / 32; ++i) o[t][i] *= alpha;
-            }
+    };
+    auto weigh = [&](uint32_t base, f32x16 (&t)[kBlocks]) {
+        if (!rows.all(a, base, KT)) {
+            asm volatile("");  // a branch, not selects: few blocks are not seen whole
+            const uint32_t from = rows.lo - base - 4u * half, to = rows.pos - base - 4u * half;  // of the lane's first key
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[t][2 * b + (j >> 2)].w[j & 3] = pack_bf16(s[t][b][2 * j], s[t][b][2 * j + 1]);
+                for (int r = 0; r < 16; ++r) {
+                    const int key = 32 * b + (int)element(r, 0u);
+                    if (key < (int)from || key > (int)to) t[b][r] = kNegInf;
+                }
         }
+        float alpha;
+        if (sm.weights(t, a.scale_log2e, alpha)) {
+#pragma unroll
+            for (int i = 0; i < DW / 32; ++i) o[i] *= alpha;
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[2 * b + (j >> 2)].w[j & 3] = pack_bf16(t[b][2 * j], t[b][2 * j + 1]);
         __builtin_amdgcn_sched_barrier(0);
+    };
+    auto first_values = [&] {
+#pragma unroll
+        for (int n = 0; n < C; ++n) x[0][n] = value_read(n);
+    };
+    auto sums = [&] {
 #pragma unroll
         for (int c = 0; c < kValueReads / C; ++c) {
             if (c + 1 < kValueReads / C) {
@@ -567,52 +585,64 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
                 for (int n = 0; n < C; ++n) x[(c + 1) & 1][n] = value_read((c + 1) * C + n);
             }
 #pragma unroll
-            for (int n = 0; n < C; ++n)
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    f32x16& to = o[t][(c * C + n) / (2 * kBlocks)];
-                    to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, p[t][(c * C + n) % (2 * kBlocks)].b, to, 0, 0, 0);
-                }
+            for (int n = 0; n < C; ++n) {
+                f32x16& to = o[(c * C + n) / (2 * kBlocks)];
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c & 1][n].b, p[(c * C + n) % (2 * kBlocks)].b, to, 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int i = 0; i < DW / 32; ++i) o[t][i] = zeros();
-    }
-    fetch(begin, 0u);
-    for (uint32_t base = begin, buf = 0; base < end; base += KT, buf ^= 1u) {
+    auto landed = [&] {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile is there
-        __syncthreads();                     // the others' too, and nobody reads the other buffer any more
-        if (base + KT < end) fetch(base + KT, buf ^ 1u);
-#pragma unroll 1
-        for (uint32_t at = 0; at < KT; at += SK) {
-            bool some = false;
+        __syncthreads();                     // the others' too, and nobody reads what is fetched next any more
+    };
 #pragma unroll
-            for (int t = 0; t < RT; ++t) some = some || rows[t].some(a, base + at, SK);
-            if (PARTS > 1 || (some && mine < all)) step(base + at, sh.k[buf] + at * D, sh.v[buf] + at * D);
-        }
-    }
+    for (int i = 0; i < DW / 32; ++i) o[i] = zeros();
+
+    for (uint32_t base = begin, buf = 0; base < end; base += KT, buf ^= 1u) {
+        landed();
+        if (base + KT < end) fetch_keys(base + KT, sh.k[buf ^ 1u]), fetch_values(base + KT, sh.v[buf ^ 1u]);
+        if (PARTS == 1 && (mine >= all || !rows.some(a, base, KT))) continue;
+        buf_at = buf * (KT * D * 2u);
+        // The waves of a SIMD are at different places of their steps; the one that multiplies goes first. Pairs keep step by
+        // their barrier, and there it costs 3 %.
+        if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(1);
+        scores();
+        if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(0);
+        if constexpr (PARTS > 1) {  // the pair's products are each over half of the columns and meet in LDS
+            static_assert(PARTS == 2 && kBlocks == 1);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const float by = 1.0f / halves_sum(sm[t].l);
-        uint16_t* to = static_cast<uint16_t*>(a.out) + (uint64_t)(it.first + rows[t].pos) * a.out_stride + (uint64_t)rows[t].head * D + column + half * 4u;
-        bool odd = false;
+            for (int e = 0; e < 4; ++e) sh.scores[wave][e][lane] = make_float4(s[0][4 * e], s[0][4 * e + 1], s[0][4 * e + 2], s[0][4 * e + 3]);
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < DW / 32; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const f32x16 x = o[t][i];
-                float y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = x[r + e] * by, odd = odd || not_finite(y[e]);
-                if (rows[t].exists) *reinterpret_cast<uint2*>(to + i * 32 + 2 * r) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+            for (int e = 0; e < 4; ++e) {
+                const float4 y = sh.scores[wave ^ 1u][e][lane];
+                s[0][4 * e] += y.x, s[0][4 * e + 1] += y.y, s[0][4 * e + 2] += y.z, s[0][4 * e + 3] += y.w;
             }
-        const unsigned long long both = __ballot(odd && rows[t].exists);
-        for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
-            redo_row<D, DW, uint16_t>(a, it, kv_head, mine + t * 32u + (uint32_t)__ffs(left) - 1u, column);
+        }
+        first_values();
+        weigh(base, s);
+        if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(1);
+        sums();
+        if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(0);
     }
+
+    const float by = 1.0f / halves_sum(sm.l);
+    uint16_t* to = static_cast<uint16_t*>(a.out) + (uint64_t)(it.first + rows.pos) * a.out_stride + (uint64_t)rows.head * D + column + half * 4u;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < DW / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x16 y = o[i];
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = y[r + e] * by, odd = odd || not_finite(z[e]);
+            if (rows.exists) *reinterpret_cast<uint2*>(to + i * 32 + 2 * r) = make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]));
+        }
+    const unsigned long long both = __ballot(odd && rows.exists);
+    for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
+        redo_row<D, DW, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
 }
 
 // As many workgroups as tiles of `rows` rows that the sequences can have (all but one row of each one's last may be
@@ -626,9 +656,9 @@ void launch_few(const PromptArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_few<D, F32>), dim3(items_of(a, kRows)), dim3(kThreads), 0, st, a);
 }
 
-template <int D, int W, int RT, int KT, int SK, int PARTS, int WAVES>
+template <int D, int W, int KT, int PARTS, int C, int WAVES>
 void launch_many(const PromptArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_many<D, W, RT, KT, SK, PARTS, WAVES>), dim3(items_of(a, 32u * RT * W / PARTS)), dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL((k_many<D, W, KT, PARTS, C, WAVES>), dim3(items_of(a, 32u * W / PARTS)), dim3(64 * W), 0, st, a);
 }
 
 template <int D>
@@ -636,10 +666,10 @@ void launch_dim(const PromptArgs& a, int dtype, uint32_t cus, hipStream_t st) {
     if (dtype == TURBO_HIDDEN_F32) return launch_few<D, true>(a, st);
     if constexpr (D <= 128)
         if (items_of(a, 128u) < cus) return launch_few<D, false>(a, st);
-    if constexpr (D == 64) return launch_many<D, 4, 1, 64, 64, 1, 3>(a, st);
-    if constexpr (D == 128) return launch_many<D, 4, 1, 64, 64, 1, 2>(a, st);
-    if constexpr (D == 256) return launch_many<D, 4, 1, 32, 32, 1, 2>(a, st);
-    if constexpr (D == 512) return launch_many<D, 8, 1, 32, 32, 2, 2>(a, st);
+    if constexpr (D == 64) return launch_many<D, 4, 64, 1, 4, 3>(a, st);
+    if constexpr (D == 128) return launch_many<D, 4, 64, 1, 4, 2>(a, st);
+    if constexpr (D == 256) return launch_many<D, 4, 32, 1, 2, 2>(a, st);
+    if constexpr (D == 512) return launch_many<D, 8, 32, 2, 2, 2>(a, st);
 }
 
 }  // namespace
