@@ -97,8 +97,13 @@ Divider divider(uint32_t d) {  // ceil(2^(31 + L) / d) with 2^(L - 1) < d <= 2^L
 // where two left fewer than 16 records to each. With a border of 8 records 16 sequences of 2,000 measured
 // 17 -> 19 us and 7 x 8 drafts 18 -> 19, though 3 x 10 drafts behind 4,000 31 -> 27; with one of 32, 32 sequences
 // behind 8,000 30 -> 36 us, though 300 prompt tokens 40 -> 34.
+// Trees, whose sequences have many rows each, weigh whole rounds of workgroups: 768 workgroups on 512 places take as long
+// as 1,024 (24 trees of 64 nodes behind 8,192, heads of 256: 508 us; in two splits TREE_SHARED). Figures in microseconds:
+// 8 to begin and end, 3.2 (two tiles) or 2 (one) for a record to each of four waves, 4 for the join and its bytes at
+// 4 TB/s. A window's records are counted once, not for the prefix and the own tokens each (7 trees of 17 nodes with a
+// window of 1,024: TREE_WINDOW us).
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
-                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus) {
+                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
     auto records = [&](uint64_t keys, uint64_t spread) {
         if (window) keys = std::min<uint64_t>(keys, (uint64_t)window + spread);
@@ -107,6 +112,8 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
     const uint64_t pr = prefix_len ? records(prefix_len, prefix_len / 4u) : 0u, orr = own_most ? records(own_most, q_len) : 0u;
     AttnPlan p{};
     p.rows = (uint64_t)batch * q_len * q_heads;
+    double best = 0.0;
+    AttnPlan chosen{};
     for (uint32_t most = most_tiles(head_dim, dtype == TURBO_HIDDEN_F32);; most /= 2u) {
         p.own_tile_rows = 16u * tiles_for(own_rows, most);
         const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
@@ -114,7 +121,8 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         uint64_t pt = (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows;
         const bool shared = pr && 2u * batch * ot > 3u * pt;
         if (!shared) p.prefix_tile_rows = p.own_tile_rows, pt = 0u;
-        const uint64_t alone = shared ? orr : pr + orr;  // records of a workgroup's sequence
+        uint64_t alone = shared ? orr : pr + orr;  // records of a workgroup's sequence
+        if (tree && !shared && window) alone = std::min(alone, records((uint64_t)prefix_len + own_most, q_len) + 1u);
         const uint64_t work = kv_heads * (pt * pr + batch * ot * alone);
         const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(4u, (work + groups - 1u) / groups);
         p.prefix_tiles = (uint32_t)pt;
@@ -125,6 +133,23 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         if (!shared && !alone) p.own_splits = 1u;
         p.prefix_items = kv_heads * pt * p.prefix_splits;
         p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
+        if (tree && !shared) {
+            const uint64_t tiles = (uint64_t)batch * kv_heads * ot, most_splits = std::min<uint64_t>(64u, (alone + 3u) / 4u);
+            for (uint64_t s = 1u; s <= std::max<uint64_t>(1u, most_splits); ++s) {
+                const double rounds = (double)((tiles * s + groups - 1u) / groups), each = (double)(((alone + s - 1u) / s + 3u) / 4u);
+                const double join = s > 1u ? 4.0 + (double)p.rows * s * head_dim * 8.0 / 4e6 : 0.0;
+                const double cost = rounds * (8.0 + each * (p.own_tile_rows == 32u ? 3.2 : 2.0)) + join;
+                if (best == 0.0 || cost < best) {
+                    best = cost;
+                    chosen = p;
+                    chosen.own_splits = (uint32_t)s;
+                    chosen.items = tiles * s;
+                }
+            }
+            if (most > 1u) continue;
+            p = chosen;
+            break;
+        }
         if (most == 1u || per >= 16u) break;
     }
     p.parts = p.prefix_splits + p.own_splits;

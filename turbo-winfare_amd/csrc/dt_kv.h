@@ -138,7 +138,7 @@ struct AttnPlan {
     uint64_t stats_bytes, bytes;
 };
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
-                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus);
+                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree);
 // tree_attention.hip: the workgroups' kernel of a call with masks; the plan and the join are attention.hip's.
 void launch_tree_attend(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);
 void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);

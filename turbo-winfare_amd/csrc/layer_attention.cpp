@@ -2,6 +2,7 @@
 // key/value cache, the heads' norms and rotation, and attention over a shared prefix.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -74,7 +75,7 @@ RotaryBox* rbox(void* p) {
 }
 
 // The sizes of an attention call, checked, and how it is split.
-tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in) {
+tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, bool tree) {
     dtype_size(in.dtype);
     if (in.batch < 0 || in.batch > (1 << 20)) fail("batch must be in 0..1048576");
     if (in.q_len < 1 || in.q_len > (1 << 20)) fail("q_len must be in 1..1048576");
@@ -86,7 +87,7 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in) 
     const tdt::AttnPlan p =
         tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype,
                             in.prefix_len, (uint32_t)(room == 0u ? 0u : beyond == 0u ? 1u : beyond < room ? beyond : room),
-                            in.window, c.cus);
+                            in.window, c.cus, tree);
     if (p.items > (1u << 24) - 1u || p.rows * (c.head_dim / 4u) > 0xFFFFFF00ull) fail("batch * q_len * q_heads is too large for one call");
     return p;
 }
@@ -372,7 +373,8 @@ TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInp
     ATT_TRY
     CacheBox* c = cbox(handle);
     if (!in || !bytes) fail("in or bytes is NULL");
-    *bytes = (size_t)attention_plan(*c, *in).bytes;
+    *bytes = (size_t)attention_plan(*c, *in, false).bytes;
+    if (in->q_len <= (int)kTreeNodes) *bytes = std::max(*bytes, (size_t)attention_plan(*c, *in, true).bytes);
     return 1;
     ATT_CATCH(0)
 }
@@ -380,7 +382,7 @@ TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInp
 static void attend(void* handle, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream) {
     CacheBox* c = cbox(handle);
     if (!in) fail("in is NULL");
-    const tdt::AttnPlan plan = attention_plan(*c, *in);
+    const tdt::AttnPlan plan = attention_plan(*c, *in, masks != nullptr);
     if (!std::isfinite(in->scale)) fail("scale must be finite");
     if (in->batch == 0) return;
     const size_t size = dtype_size(in->dtype), packed = (size_t)in->q_heads * c->head_dim;
