@@ -645,6 +645,252 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
         redo_row<D, DW, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
 }
 
+// Many rows of FP32. The matrix unit multiplies 16-bit numbers at 16 times its rate of FP32 ones, so every number enters as
+// a sum of such: queries and keys as two of fp16 after a power of two of the row or key (22 bits, and 2^-40 of the largest;
+// the product of the two small parts, 2^-22, is left out), weights and values, which need no power there, as three of BF16
+// (24 bits; of the nine products those of 2^-24 are left out). A tile's numbers are split once, on their way to LDS, by
+// the whole workgroup.
+// Heads above 128 are divided among PARTS waves, 128 columns each, whose score products meet in LDS; where the tile's keys
+// and values do not fit there together (heads of 512), the values take the keys' place.
+template <int D, int W, int PARTS>
+struct Many32 {
+    static constexpr bool kOnePlace = D > 256;
+    static constexpr int kKeyWords = 2 * kKeys * D, kValueWords = 3 * kKeys * D;
+    // fp16 keys: the number rounded, and what is left of it; BF16 values in three parts
+    uint16_t k[kOnePlace ? kValueWords : kKeyWords], v[kOnePlace ? 8 : kValueWords];
+    float4 scores[PARTS > 1 ? W : 1][PARTS > 1 ? 4 : 1][64];
+    int power[kKeys];  // of the keys
+};
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+// Two numbers rounded to fp16 in the first word, what is left of them in the second.
+__device__ inline void split_fp16(float a, float b, uint32_t& high, uint32_t& low) {
+    const half2v h = {(_Float16)a, (_Float16)b};
+    const half2v l = {(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])};
+    high = __builtin_bit_cast(uint32_t, h), low = __builtin_bit_cast(uint32_t, l);
+}
+__device__ inline void split_bf16(float a, float b, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        w[n] = pack_bf16(a, b);
+        a -= __uint_as_float(w[n] << 16), b -= __uint_as_float(w[n] & 0xFFFF0000u);
+    }
+}
+// The power of two that takes a number's largest magnitude to 2^14 .. 2^15
+__device__ inline int power_to_fp16(float top) { return top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0; }
+
+template <int D, int W, int PARTS>
+__global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
+    constexpr uint32_t R = 32 * W / PARTS, kPerKey = 64 * W / kKeys;  // rows, threads that share a key
+    constexpr int DW = D / PARTS, kPieces = D / 4 / kPerKey;          // columns of a wave, four numbers each of a thread
+    typedef Many32<D, W, PARTS> Tile;
+    __shared__ __attribute__((aligned(1024))) Tile sh;
+    uint16_t* const values = Tile::kOnePlace ? sh.k : sh.v;
+    const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t kv_head = blockIdx.x % a.kv_heads;
+    const Item it = locate(a, blockIdx.x / a.kv_heads, R);
+    if (!it.exists) return;
+    const uint32_t all = it.len * a.group, row0 = it.tile * R, mine = row0 + wave / PARTS * 32u, column = wave % PARTS * DW, last = it.len - 1u;
+    const uint32_t begin = Rows::from(a, row0 / a.group) / kKeys * kKeys, end = min(row0 + R - 1u, all - 1u) / a.group + 1u;
+    const uint32_t my_key = threadIdx.x / kPerKey, my_col = threadIdx.x % kPerKey * 4u;
+    const float* k = static_cast<const float*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D + my_col;
+    const float* v = static_cast<const float*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D + my_col;
+    float4 kn[kPieces], vn[kPieces];  // of the next tile
+    auto fetch_keys = [&](uint32_t base) {
+        const uint64_t row = min(base + my_key, last);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) kn[i] = *reinterpret_cast<const float4*>(k + row * a.k_stride + i * (int)kPerKey * 4);
+    };
+    auto fetch_values = [&](uint32_t base) {
+        const uint64_t row = min(base + my_key, last);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) vn[i] = *reinterpret_cast<const float4*>(v + row * a.v_stride + i * (int)kPerKey * 4);
+    };
+    fetch_keys(begin);
+    fetch_values(begin);
+
+    const Rows rows(a, it, kv_head, mine);
+    Frag qh[DW / 16], ql[DW / 16];
+    int q_power;
+    {
+        const float* q = static_cast<const float*>(a.q) + (uint64_t)(it.first + rows.pos) * a.q_stride + (uint64_t)rows.head * D + half * 8u;
+        float top = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < D / 16; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(q + i * 16), y = *reinterpret_cast<const float4*>(q + i * 16 + 4);
+            top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                                   fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
+        }
+        q_power = power_to_fp16(halves_max(top));
+        const float sign = a.flip ? -1.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(q + column + i * 16), y = *reinterpret_cast<const float4*>(q + column + i * 16 + 4);
+            const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_fp16(sign * ldexpf(z[2 * j], q_power), sign * ldexpf(z[2 * j + 1], q_power), qh[i].w[j], ql[i].w[j]);
+        }
+    }
+
+    // places in LDS, as in k_many
+    constexpr int kKeyTurns = D >= 128 ? 8 : 4, kValueTurns = D >= 128 ? 4 : 2;
+    uint32_t key_at[kKeyTurns], value_at[kValueTurns];
+#pragma unroll
+    for (int i = 0; i < kKeyTurns; ++i) key_at[i] = lds_at(sh.k) + (col * D + column) * 2u + (((2u * i) ^ half ^ key_turn<D>(col)) * 16u);
+#pragma unroll
+    for (int i = 0; i < kValueTurns; ++i)
+        value_at[i] = lds_at(values) + ((4u * half + ((lane >> 2) & 3u)) * D + column + (lane & 1u) * 4u) * 2u +
+                      ((4u * i ^ ((lane >> 4) & 1u) * 2u ^ ((lane & 3u) >> 1) ^ value_turn<D>(lane >> 2)) * 16u);
+    auto key_read = [&](int part, int i) {
+        Frag x;
+        x.x = *(const __attribute__((address_space(3))) u32x4*)(key_at[i % kKeyTurns] + (uint32_t)(part * kKeys * D * 2 + i / kKeyTurns * kKeyTurns * 32));
+        return x;
+    };
+    auto value_read = [&](int part, int i, int j) {
+        Frag x;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                value_at[i % kValueTurns] + (uint32_t)((part * kKeys + 16 * j + 8 * e) * D * 2 + i / kValueTurns * kValueTurns * 64)));
+        return x;
+    };
+    auto split_keys = [&] {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) top = fmaxf(top, fmaxf(fmaxf(fabsf(kn[i].x), fabsf(kn[i].y)), fmaxf(fabsf(kn[i].z), fabsf(kn[i].w))));
+#pragma unroll
+        for (uint32_t d = 1; d < kPerKey; d *= 2u) top = fmaxf(top, __shfl_xor(top, (int)d));
+        const int power = power_to_fp16(top);
+        if (my_col == 0u) sh.power[my_key] = -power;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const uint32_t chunk = (i * kPerKey * 4u + my_col) >> 3;
+            uint2 h, l;
+            split_fp16(ldexpf(kn[i].x, power), ldexpf(kn[i].y, power), h.x, l.x);
+            split_fp16(ldexpf(kn[i].z, power), ldexpf(kn[i].w, power), h.y, l.y);
+            uint16_t* to = sh.k + my_key * D + (my_col & 4u) + (chunk ^ key_turn<D>(my_key)) * 8u;
+            *reinterpret_cast<uint2*>(to) = h;
+            *reinterpret_cast<uint2*>(to + kKeys * D) = l;
+        }
+    };
+    auto split_values = [&] {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const uint32_t chunk = (i * kPerKey * 4u + my_col) >> 3;
+            uint32_t x[3], y[3];
+            split_bf16(vn[i].x, vn[i].y, x);
+            split_bf16(vn[i].z, vn[i].w, y);
+            uint16_t* to = values + my_key * D + (my_col & 4u) + (chunk ^ value_turn<D>(my_key)) * 8u;
+#pragma unroll
+            for (int n = 0; n < 3; ++n) *reinterpret_cast<uint2*>(to + n * kKeys * D) = make_uint2(x[n], y[n]);
+        }
+    };
+
+    f32x16 o[DW / 32];
+    Softmax sm;
+#pragma unroll
+    for (int i = 0; i < DW / 32; ++i) o[i] = zeros();
+    for (uint32_t base = begin; base < end; base += kKeys) {
+        __syncthreads();  // nobody reads the tile before any more
+        split_keys();
+        if constexpr (!Tile::kOnePlace) split_values();
+        __syncthreads();
+        if (base + kKeys < end) {
+            fetch_keys(base + kKeys);
+            if constexpr (!Tile::kOnePlace) fetch_values(base + kKeys);
+        }
+        if (PARTS == 1 && (mine >= all || !rows.some(a, base, kKeys))) continue;
+        f32x16 s[1] = {zeros()}, t = zeros();
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) {
+            const Frag h = key_read(0, i), l = key_read(1, i);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, h.x), __builtin_bit_cast(half8v, qh[i].x), s[0], 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, h.x), __builtin_bit_cast(half8v, ql[i].x), t, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, l.x), __builtin_bit_cast(half8v, qh[i].x), t, 0, 0, 0);
+            if (i % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        s[0] += t;
+        if constexpr (PARTS > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sh.scores[wave][e][lane] = make_float4(s[0][4 * e], s[0][4 * e + 1], s[0][4 * e + 2], s[0][4 * e + 3]);
+            __syncthreads();
+            s[0] = zeros();
+#pragma unroll
+            for (uint32_t n = 0; n < PARTS; ++n)  // in the same order for every wave of the row: so are their weights
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 y = sh.scores[wave / PARTS * PARTS + n][e][lane];
+                    s[0][4 * e] += y.x, s[0][4 * e + 1] += y.y, s[0][4 * e + 2] += y.z, s[0][4 * e + 3] += y.w;
+                }
+            if constexpr (Tile::kOnePlace) {
+                split_values();
+                __syncthreads();
+                if (base + kKeys < end) fetch_values(base + kKeys);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int4 e = *reinterpret_cast<const int4*>(&sh.power[element(r, half)]);
+            s[0][r] = ldexpf(s[0][r], e.x - q_power), s[0][r + 1] = ldexpf(s[0][r + 1], e.y - q_power);
+            s[0][r + 2] = ldexpf(s[0][r + 2], e.z - q_power), s[0][r + 3] = ldexpf(s[0][r + 3], e.w - q_power);
+        }
+        if (!rows.all(a, base, kKeys)) {
+            asm volatile("");
+            const int from = (int)(rows.lo - base - 4u * half), to = (int)(rows.pos - base - 4u * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((int)element(r, 0u) < from || (int)element(r, 0u) > to) s[0][r] = kNegInf;
+        }
+        float alpha;
+        if (sm.weights(s, a.scale_log2e, alpha)) {
+#pragma unroll
+            for (int i = 0; i < DW / 32; ++i) o[i] *= alpha;
+        }
+        Frag p[3][2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w[3];
+            split_bf16(s[0][2 * j], s[0][2 * j + 1], w);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) p[n][j >> 2].w[j & 3] = w[n];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < DW / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const Frag h = value_read(0, i, j), m = value_read(1, i, j), l = value_read(2, i, j);
+                f32x16& to = o[i];
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(l.b, p[0][j].b, to, 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.b, p[2][j].b, to, 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m.b, p[1][j].b, to, 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m.b, p[0][j].b, to, 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.b, p[1][j].b, to, 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(h.b, p[0][j].b, to, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+
+    const float by = 1.0f / halves_sum(sm.l);
+    float* to = static_cast<float*>(a.out) + (uint64_t)(it.first + rows.pos) * a.out_stride + (uint64_t)rows.head * D + column + half * 4u;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < DW / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x16 y = o[i];
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = y[r + e] * by, odd = odd || not_finite(z[e]);
+            if (rows.exists) *reinterpret_cast<float4*>(to + i * 32 + 2 * r) = make_float4(z[0], z[1], z[2], z[3]);
+        }
+    const unsigned long long both = __ballot(odd && rows.exists);
+    for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
+        redo_row<D, DW, float>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
+}
+
 // As many workgroups as tiles of `rows` rows that the sequences can have (all but one row of each one's last may be
 // missing) over all key/value heads.
 uint32_t items_of(const PromptArgs& a, uint32_t rows) {
@@ -663,7 +909,13 @@ void launch_many(const PromptArgs& a, hipStream_t st) {
 
 template <int D>
 void launch_dim(const PromptArgs& a, int dtype, uint32_t cus, hipStream_t st) {
-    if (dtype == TURBO_HIDDEN_F32) return launch_few<D, true>(a, st);
+    if (dtype == TURBO_HIDDEN_F32) {
+        constexpr int kParts = D <= 128 ? 1 : D / 128, kManyWaves = kParts == 1 ? 4 : 8;
+        const uint32_t items = items_of(a, 32u * kManyWaves / kParts);
+        if (items < cus / 2u) return launch_few<D, true>(a, st);
+        hipLaunchKernelGGL((k_many32<D, kManyWaves, kParts>), dim3(items), dim3(64 * kManyWaves), 0, st, a);
+        return;
+    }
     if constexpr (D <= 128)
         if (items_of(a, 128u) < cus) return launch_few<D, false>(a, st);
     if constexpr (D == 64) return launch_many<D, 4, 64, 1, 4, 3>(a, st);
