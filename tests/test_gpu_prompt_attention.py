@@ -83,11 +83,26 @@ def test_many_rows(d, hq, hk, window):
     check(q, k, v, call(q, k, v, lengths, BF16, window=window), lengths, BF16, window)
 
 
-@pytest.mark.parametrize("d", [64, 256])
-def test_many_sequences(d):
-    lengths = [(7 * i) % 23 for i in range(200)]
-    q, k, v = inputs(lengths, 4, 2, d, BF16, 4)
-    check(q, k, v, call(q, k, v, lengths, BF16), lengths, BF16)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d,n", [(64, 65), (256, 200), (512, 129), (64, 5000)])
+def test_many_sequences(d, n, dtype):
+    lengths = [(7 * i) % 23 + (150 if i % 97 == 3 else 0) for i in range(n)]
+    q, k, v = inputs(lengths, 4, 2, d, dtype, 4, spare=2)
+    out = call(q, k, v, lengths, dtype)
+    last = slice(sum(lengths[:-100]), None)  # the sequences at both ends, all of up to 200
+    if n > 1000:
+        check(q, k, v, out, lengths[:100], dtype)
+        check(q[last], k[last], v[last], out[last], lengths[-100:], dtype)
+    else:
+        check(q, k, v, out, lengths, dtype)
+    assert bool((out[sum(lengths):] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d,n", [(64, 2500), (128, 1800), (256, 1100), (256, 2300), (512, 700)])
+def test_one_long_sequence(d, n, dtype):
+    q, k, v = inputs([n], 8, 4, d, dtype, 14)
+    check(q, k, v, call(q, k, v, [n], dtype), [n], dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -2,13 +2,13 @@
 //
 // With s_j = scale q . k_j over the keys j that a query at position i sees (j <= i, and i - j < window):
 //   out = sum_j 2^(c s_j - m) v_j / sum_j 2^(c s_j - m),  c = scale log2(e), m a running maximum of the c s_j,
-// one pass over the keys, sums and statistics in FP32. A workgroup takes 32 query rows of one head; its four waves
-// take the blocks of 32 keys in turn, each with its own maximum and sums, and join at the end.
-//   S^T = K Q^T, keys as the first operand: a lane holds 16 scores of one row.
-//   O^T += V^T P^T: those 16 keys are the lane's part of the second operand as they are, if the first operand takes
-//     the keys in the same order.
-#include <type_traits>
-
+// one pass over the keys, statistics and sums in FP32. Rows are (token, head) pairs: the heads that share keys lie side by
+// side, so a tile of rows reads its keys once for all of them. A wave has 32 rows and takes 32 or 64 keys at a time:
+//   S^T = K Q^T, keys as the first operand: a lane holds 16 scores of one row for every 32 keys.
+//   O^T += V^T P^T: those 16 keys are the lane's part of the second operand as they are, if the first operand takes the
+//     keys in the same order; values are transposed on their way out of LDS.
+// The maximum, and with it the sums, is left alone while weights stay below 2^8. Weights are rounded to BF16 for BF16 inputs
+// (2^-8 of each at most, as the result itself), the sum of weights is that of the unrounded ones.
 #include "dt_internal.h"
 #include "dt_mfma.h"
 #include "dt_step.h"
@@ -63,56 +63,55 @@ struct Item {
     bool exists;
 };
 
-// Tile number `id` of all sequences' tiles of `rows` rows (a token's heads that share keys have one each): the last tiles, which have most keys, come first, and
-// among equal ones the sequences in order. Every wave finds it for itself: the number of tiles at a level or above
-// falls with the level, so the level is found by halving.
+// Tile number `id` of all sequences' tiles of `rows` rows (a token has one for each of its heads that share keys). Every
+// wave finds it for itself.
+// Up to 64 sequences: the last tiles, which have most keys, come first, and among equal ones the sequences in order. The
+// number of tiles at a level or above falls with the level, so the level is found by halving.
+// More sequences, whose tiles fill the card in any order: sequence b's tiles begin at number (its first row) / rows + b, which
+// leaves room for them all, and a number belongs to the last sequence that begins at or before it.
 __device__ inline Item locate(const PromptArgs& a, uint32_t id, uint32_t rows) {
     const uint32_t lane = threadIdx.x & 63u;
-    auto bounds = [&](uint32_t b, uint32_t& first, uint32_t& len) {
-        first = min(a.starts[b], a.tokens);
-        len = max(min(a.starts[b + 1u], a.tokens), first) - first;
-    };
-    uint32_t first0 = 0, len0 = 0;
-    if (lane < a.batch) bounds(lane, first0, len0);
-    auto tiles_of = [&](uint32_t b) {
-        uint32_t first = first0, len = len0;
-        if (b >= 64u) bounds(b, first, len);
-        return (len * a.group + rows - 1u) / rows;
-    };
-    auto at_least = [&](uint32_t level) {  // tiles of all sequences from this level on
-        uint32_t n = 0;
-        for (uint32_t b = lane; b < a.batch; b += 64u) {
-            const uint32_t t = tiles_of(b);
-            n += t > level ? t - level : 0u;
-        }
-        return (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_reduce(n, [](uint32_t x, uint32_t y) { return x + y; }));
-    };
+    auto start_of = [&](uint32_t b) { return min(a.starts[b], a.tokens); };
+    auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
     Item it{};
-    uint32_t lo = 0u, hi = (a.tokens * a.group + rows - 1u) / rows;  // at_least(lo) > id >= at_least(hi)
-    if (at_least(0u) <= id) return it;
-    while (hi - lo > 1u) {
-        const uint32_t mid = (lo + hi) / 2u;
-        if (at_least(mid) > id) lo = mid;
-        else hi = mid;
-    }
-    uint32_t rank = id - at_least(lo + 1u);
-    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64u) {
-        const uint32_t b = b0 + lane;
-        const unsigned long long have = __ballot(b < a.batch && tiles_of(b) > lo);
-        const uint32_t n = (uint32_t)__popcll(have);
-        if (rank >= n) {
-            rank -= n;
-            continue;
+    uint32_t found;
+    if (a.batch <= 64u) {
+        const uint32_t first = lane < a.batch ? start_of(lane) : 0u, len = lane < a.batch ? max(start_of(lane + 1u), first) - first : 0u;
+        const uint32_t tiles = (len * a.group + rows - 1u) / rows;
+        auto at_least = [&](uint32_t level) {  // tiles of all sequences from this level on
+            return uniform(wave_reduce(tiles > level ? tiles - level : 0u, [](uint32_t x, uint32_t y) { return x + y; }));
+        };
+        uint32_t lo = 0u, hi = (a.tokens * a.group + rows - 1u) / rows;  // at_least(lo) > id >= at_least(hi)
+        if (at_least(0u) <= id) return it;
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (at_least(mid) > id) lo = mid;
+            else hi = mid;
         }
-        const unsigned long long mine = __ballot(((have >> lane) & 1ull) && (uint32_t)__popcll(have & ((1ull << lane) - 1ull)) == rank);
-        const uint32_t found = b0 + (uint32_t)__ffsll(mine) - 1u;
-        bounds(found, it.first, it.len);
-        it.first = (uint32_t)__builtin_amdgcn_readfirstlane((int)it.first);
-        it.len = (uint32_t)__builtin_amdgcn_readfirstlane((int)it.len);
+        const uint32_t rank = id - at_least(lo + 1u);  // by all lanes: a reduction
+        const unsigned long long have = __ballot(tiles > lo);
+        const unsigned long long mine = __ballot(tiles > lo && (uint32_t)__popcll(have & ((1ull << lane) - 1ull)) == rank);
+        if (mine == 0ull) return it;
+        found = (uint32_t)__ffsll(mine) - 1u;
         it.tile = lo;
-        it.exists = true;
-        break;
+    } else {
+        uint32_t lo = 0u, n = a.batch, begins = 0u;  // the sequence is one of n from lo on
+        while (true) {
+            const uint32_t step = (n + 63u) / 64u, b = lo + lane * step;
+            const uint32_t at = lane * step < n ? start_of(b) * a.group / rows + b : 0xFFFFFFFFu;
+            const uint32_t before = (uint32_t)__popcll(__ballot(at <= id));
+            if (before == 0u) return it;
+            lo += (before - 1u) * step;
+            n = min(step, n - (before - 1u) * step);
+            begins = uniform(__shfl(at, (int)before - 1));
+            if (n == 1u) break;
+        }
+        found = lo;
+        it.tile = id - begins;
     }
+    it.first = uniform(start_of(found));
+    it.len = max(uniform(start_of(found + 1u)), it.first) - it.first;
+    it.exists = it.tile < (it.len * a.group + rows - 1u) / rows;
     return it;
 }
 
@@ -222,23 +221,22 @@ __device__ inline void redo_row(const PromptArgs& a, const Item& it, uint32_t kv
     }
 }
 
-// Few rows: a workgroup takes 32 of them. Its four waves take the blocks of 32 keys in turn, each with its own maximum
-// and sums, and join at the end.
-template <int D, bool F32>
+// Few rows of FP32: a workgroup takes 32 of them. Its four waves take the blocks of 32 keys in turn, each with its own
+// maximum and sums, and join at the end. The matrix unit takes FP32 numbers as they are, at a sixteenth of its rate of
+// 16-bit ones.
+template <int D>
 struct Few {
     union {
-        float4 q[F32 ? D / 8 : 1][64];                 // FP32 queries as second operands
-        uint4 v[F32 ? 1 : kWaves][kKeys * D / 8];      // a wave's block of BF16 values, [key][D]
+        float4 q[D / 8][64];  // the queries as second operands
         float sums[kWaves][kRows][68];
     };
     float m[kWaves][kRows], l[kWaves][kRows];
     uint32_t odd;  // rows whose result is not finite
 };
 
-template <int D, bool F32>
-__global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const PromptArgs a) {
-    typedef typename std::conditional<F32, float, uint16_t>::type E;
-    __shared__ Few<D, F32> sh;
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void k_few32(const PromptArgs a) {
+    __shared__ Few<D> sh;
     const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
@@ -247,107 +245,50 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const Prompt
     const uint32_t last = it.len - 1u;
     const Rows rows(a, it, kv_head, it.tile * kRows);
     const uint32_t begin = Rows::from(a, rows.first), end = rows.last + 1u;
-    const E* q = static_cast<const E*>(a.q) + (uint64_t)(it.first + rows.pos) * a.q_stride + (uint64_t)rows.head * D;
-    const E* k = static_cast<const E*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
-    const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D;
-
-    Frag qf[F32 ? 1 : D / 16];
-    if constexpr (!F32) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            qf[i].u = *reinterpret_cast<const uint4*>(q + i * 16 + half * 8u);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) qf[i].w[j] ^= a.flip;
-        }
+    const float* q = static_cast<const float*>(a.q) + (uint64_t)(it.first + rows.pos) * a.q_stride + (uint64_t)rows.head * D;
+    const float* k = static_cast<const float*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
+    const float* v = static_cast<const float*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D;
+    for (int i = wave; i < D / 8; i += kWaves) {
+        uint4 x = *reinterpret_cast<const uint4*>(q + i * 8 + half * 4u);
+        x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
+        sh.q[i][lane] = __builtin_bit_cast(float4, x);
     }
+    __syncthreads();
     f32x16 o[D / 32];
     Softmax sm;
-    {
-        if constexpr (F32) {
-            for (int i = wave; i < D / 8; i += kWaves) {
-                uint4 x = *reinterpret_cast<const uint4*>(q + i * 8 + half * 4u);
-                x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
-                sh.q[i][lane] = __builtin_bit_cast(float4, x);
-            }
-            __syncthreads();
-        }
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = zeros();
-        sm = Softmax();
-        for (uint32_t base = begin / kKeys * kKeys + wave * kKeys; base < end; base += kWaves * kKeys) {
-            // ---- scores
-            const E* krow = k + (uint64_t)min(base + col, last) * a.k_stride;
-            f32x16 s[1] = {zeros()};
-            if constexpr (F32) {
+    for (int i = 0; i < D / 32; ++i) o[i] = zeros();
+    for (uint32_t base = begin / kKeys * kKeys + wave * kKeys; base < end; base += kWaves * kKeys) {
+        // ---- scores
+        const float* krow = k + (uint64_t)min(base + col, last) * a.k_stride;
+        f32x16 s[1] = {zeros()};
 #pragma unroll 8
-                for (int i = 0; i < D / 8; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(krow + i * 8 + half * 4u), y = sh.q[i][lane];
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s[0], 0, 0, 0);
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s[0], 0, 0, 0);
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s[0], 0, 0, 0);
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s[0], 0, 0, 0);
-                }
-            } else {
-                constexpr int kLoads = kKeys * D / 512;  // the values' block on its way to LDS meanwhile
-                uint4 held[kLoads];
+        for (int i = 0; i < D / 8; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(krow + i * 8 + half * 4u), y = sh.q[i][lane];
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s[0], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s[0], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s[0], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s[0], 0, 0, 0);
+        }
+        if (!rows.all(a, base, kKeys)) {
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const uint32_t at = i * 512u + lane * 8u, row = at / D;
-                    held[i] = *reinterpret_cast<const uint4*>(v + (uint64_t)min(base + row, last) * a.v_stride + at % D);
-                }
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    Frag x;
-                    x.u = *reinterpret_cast<const uint4*>(krow + i * 16 + half * 8u);
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, qf[i].b, s[0], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) sh.v[wave][i * 64u + lane] = held[i];
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t key = base + element(r, half);
+                if (key < rows.lo || key > rows.pos) s[0][r] = kNegInf;
             }
-            if (!rows.all(a, base, kKeys)) {
+        }
+        // ---- weights
+        float alpha;
+        if (sm.weights(s, a.scale_log2e, alpha)) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const uint32_t key = base + element(r, half);
-                    if (key < rows.lo || key > rows.pos) s[0][r] = kNegInf;
-                }
-            }
-            // ---- weights
-            float alpha;
-            if (sm.weights(s, a.scale_log2e, alpha)) {
+            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+        }
+        // ---- weighted values
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
-            }
-            // ---- weighted values
-            if constexpr (F32) {
+        for (int r = 0; r < 16; ++r) {
+            const float* vrow = v + (uint64_t)min(base + element(r, half), last) * a.v_stride + col;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const E* vrow = v + (uint64_t)min(base + element(r, half), last) * a.v_stride + col;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i)
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[i * 32], s[0][r], o[i], 0, 0, 0);
-                }
-            } else {
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-                Frag p[2];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) p[j >> 2].w[j & 3] = pack_bf16(s[0][2 * j], s[0][2 * j + 1]);
-                // keys 4 half .. and 8 + 4 half .. of 16, columns col of 32: 16 lanes read four keys of 16 columns and
-                // get a column each
-                const uint16_t* vs = reinterpret_cast<const uint16_t*>(sh.v[wave]) + (4u * half + ((lane & 15u) >> 2)) * D + (lane & 16u) + (lane & 3u) * 4u;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        Frag x;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            x.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) short4v*)(vs + (16 * j + 8 * e) * D + i * 32));
-                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.b, p[j].b, o[i], 0, 0, 0);
-                    }
-            }
+            for (int i = 0; i < D / 32; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[i * 32], s[0][r], o[i], 0, 0, 0);
         }
     }
 
@@ -369,7 +310,7 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const Prompt
     const float by = 1.0f / total;
     bool odd = false;
     const uint32_t out_row = it.tile * kRows + row, token = out_row / a.group;
-    E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token) * a.out_stride +
+    float* to = static_cast<float*>(a.out) + (uint64_t)(it.first + token) * a.out_stride +
             (uint64_t)(kv_head * a.group + out_row - token * a.group) * D + c8;
 #pragma unroll
     for (int n = 0; n < D / 64; ++n) {
@@ -393,18 +334,14 @@ __global__ __launch_bounds__(kThreads, D <= 256 ? 2 : 1) void k_few(const Prompt
             odd = odd || not_finite(x[i]);
         }
         if (token < it.len) {
-            if constexpr (F32) {
-                *reinterpret_cast<float4*>(to + n * 64) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(to + n * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
-                *reinterpret_cast<uint4*>(to + n * 64) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-            }
+            *reinterpret_cast<float4*>(to + n * 64) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(to + n * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
     }
     if (odd && token < it.len) atomicOr(&sh.odd, 1u << row);
     __syncthreads();  // what was written is written over, in order
     for (uint32_t left = sh.odd, n = 0; left; left &= left - 1u, ++n)
-        if (n % kWaves == wave) redo_row<D, D, E>(a, it, kv_head, it.tile * kRows + (uint32_t)__ffs(left) - 1u, 0u);
+        if (n % kWaves == wave) redo_row<D, D, float>(a, it, kv_head, it.tile * kRows + (uint32_t)__ffs(left) - 1u, 0u);
 }
 
 // Many rows: every wave has 32 RT rows of its own, and tiles of KT keys and values go from memory to LDS, without
@@ -429,10 +366,20 @@ struct TileSource {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(words) : "memory");
     }
 };
-template <int D, int KT, int W, int PARTS>
+template <int D, int KT, int W, int PARTS, int TEAMS>
 struct Many {
-    uint16_t k[2][KT * D], v[2][KT * D];
-    float4 scores[PARTS > 1 ? W : 1][PARTS > 1 ? 4 : 1][64];
+    static constexpr int kBuffers = W > 1 ? 2 : 1;
+    union {
+        struct {
+            uint16_t k[kBuffers][KT * D], v[kBuffers][KT * D];
+        } tile[TEAMS];
+        // the sums that a team makes for another one, which joins and writes those columns
+        float4 sums[TEAMS > 1 ? W : 1][TEAMS > 1 ? TEAMS * (TEAMS - 1) : 1][TEAMS > 1 ? D / 8 / TEAMS : 1][64];
+    };
+    union {
+        float2 stats[TEAMS][TEAMS > 1 ? W : 1][64];  // (m, l) of every row
+        float4 scores[PARTS > 1 ? W : 1][PARTS > 1 ? 4 : 1][64];
+    };
 };
 template <int D>
 __device__ inline uint32_t key_turn(uint32_t row) { return D >= 128 ? row & 15u : (row >> 1) & 7u; }
@@ -446,14 +393,17 @@ __device__ inline uint32_t lds_at(T* p) { return (uint32_t)(uintptr_t)(__attribu
 
 // W waves in pairs (PARTS 2) or alone, of which each has DW columns of the queries, keys, values and sums of 32 rows:
 // the registers of two waves per SIMD hold 256. WAVES waves per SIMD; C operands are read from LDS while the C products
-// before them run.
-template <int D, int W, int KT, int PARTS, int C, int WAVES>
-__global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
+// before them run. TEAMS of W waves take a workgroup's tiles of keys in turn for the same rows, with maxima and sums of
+// their own, and join at the end. A team of one wave has one tile's place and waits for no other until then.
+template <int D, int W, int KT, int PARTS, int C, int WAVES, int TEAMS>
+__global__ __launch_bounds__(64 * W * TEAMS, WAVES) void k_many(const PromptArgs a) {
     constexpr int DW = D / PARTS, kBlocks = KT / 32, kLoads = KT * D / 512 / W;  // kLoads: a wave's loads of 1 KB
     constexpr uint32_t kChunks = D / 8, kLoadRows = 64 / kChunks, kStep = W * kLoadRows, R = 32 * W / PARTS;
-    __shared__ __attribute__((aligned(1024))) Many<D, KT, W, PARTS> sh;
+    __shared__ __attribute__((aligned(1024))) Many<D, KT, W, PARTS, TEAMS> sh;
     const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / (64u * W)) : 0u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - team * W;
+    auto& mem = sh.tile[team];
     const uint32_t kv_head = blockIdx.x % a.kv_heads;
     const Item it = locate(a, blockIdx.x / a.kv_heads, R);
     if (!it.exists) return;
@@ -484,8 +434,8 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
             from.load(to + (wave + W * n) * 512u, min(row, there - 1u) * v_bytes + ((chunk ^ value_turn<D>(row)) * 16u));
         }
     };
-    fetch_keys(begin, sh.k[0]);
-    fetch_values(begin, sh.v[0]);
+    const uint32_t my_begin = begin + team * KT;  // a team's tiles
+    if (my_begin < end) fetch_keys(my_begin, mem.k[0]), fetch_values(my_begin, mem.v[0]);
 
     const Rows rows(a, it, kv_head, mine);
     Frag qf[DW / 16];
@@ -502,10 +452,10 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
     constexpr int kKeyTurns = D >= 128 ? 8 : 4, kValueTurns = D >= 128 ? 4 : 2;
     uint32_t key_at[kKeyTurns], value_at[kValueTurns];
 #pragma unroll
-    for (int i = 0; i < kKeyTurns; ++i) key_at[i] = lds_at(sh.k[0]) + (col * D + column) * 2u + (((2u * i) ^ half ^ key_turn<D>(col)) * 16u);
+    for (int i = 0; i < kKeyTurns; ++i) key_at[i] = lds_at(mem.k[0]) + (col * D + column) * 2u + (((2u * i) ^ half ^ key_turn<D>(col)) * 16u);
 #pragma unroll
     for (int i = 0; i < kValueTurns; ++i)
-        value_at[i] = lds_at(sh.v[0]) + ((4u * half + ((lane >> 2) & 3u)) * D + column + (lane & 1u) * 4u) * 2u +
+        value_at[i] = lds_at(mem.v[0]) + ((4u * half + ((lane >> 2) & 3u)) * D + column + (lane & 1u) * 4u) * 2u +
                       ((4u * i ^ ((lane >> 4) & 1u) * 2u ^ ((lane & 3u) >> 1) ^ value_turn<D>(lane >> 2)) * 16u);
     uint32_t buf_at = 0u;  // of the tile in hand
     auto key_read = [&](int n) {
@@ -593,17 +543,23 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
         }
     };
     auto landed = [&] {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile is there
-        __syncthreads();                     // the others' too, and nobody reads what is fetched next any more
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile is there
+        if constexpr (W > 1) __syncthreads();             // the others' too, and nobody reads what is fetched next any more
     };
 #pragma unroll
     for (int i = 0; i < DW / 32; ++i) o[i] = zeros();
 
-    for (uint32_t base = begin, buf = 0; base < end; base += KT, buf ^= 1u) {
+    for (uint32_t at = begin, buf = 0; at < end; at += KT * TEAMS, buf ^= 1u) {
+        const uint32_t base = at + team * KT, next = base + KT * TEAMS;
         landed();
-        if (base + KT < end) fetch_keys(base + KT, sh.k[buf ^ 1u]), fetch_values(base + KT, sh.v[buf ^ 1u]);
-        if (PARTS == 1 && (mine >= all || !rows.some(a, base, KT))) continue;
-        buf_at = buf * (KT * D * 2u);
+        if constexpr (W > 1) {
+            if (next < end) fetch_keys(next, mem.k[buf ^ 1u]), fetch_values(next, mem.v[buf ^ 1u]);
+            buf_at = buf * (KT * D * 2u);
+        }
+        if (PARTS == 1 && (mine >= all || (TEAMS > 1 && base >= end) || !rows.some(a, base, KT))) {
+            if (W == 1 && next < end) fetch_keys(next, mem.k[0]), fetch_values(next, mem.v[0]);
+            continue;
+        }
         // The waves of a SIMD are at different places of their steps; the one that multiplies goes first. Pairs keep step by
         // their barrier, and there it costs 3 %.
         if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(1);
@@ -625,24 +581,79 @@ __global__ __launch_bounds__(64 * W, WAVES) void k_many(const PromptArgs a) {
         if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(1);
         sums();
         if constexpr (PARTS == 1) __builtin_amdgcn_s_setprio(0);
+        if constexpr (W == 1)
+            if (next < end) fetch_keys(next, mem.k[0]), fetch_values(next, mem.v[0]);  // the tile has been read
     }
 
-    const float by = 1.0f / halves_sum(sm.l);
-    uint16_t* to = static_cast<uint16_t*>(a.out) + (uint64_t)(it.first + rows.pos) * a.out_stride + (uint64_t)rows.head * D + column + half * 4u;
+    // Unit n of a lane's sums, o[n / 4][n % 4 * 4 ..], are columns 8 n + 4 half .. of its row.
+    constexpr int kUnits = DW / 8 / TEAMS;  // of a team
+    float l = halves_sum(sm.l);
+    if constexpr (TEAMS > 1) {
+        static_assert(PARTS == 1);
+        __syncthreads();  // the tiles' places are free
+        sh.stats[team][wave][lane] = make_float2(sm.m, l);
+        auto place = [](int from, int to) { return from * (TEAMS - 1) + (to < from ? to : to - 1); };
+#pragma unroll
+        for (int n = 0; n < DW / 8; ++n)
+            if (n / kUnits != (int)team)
+                sh.sums[wave][place((int)team, n / kUnits)][n % kUnits][lane] =
+                    make_float4(o[n / 4][n % 4 * 4], o[n / 4][n % 4 * 4 + 1], o[n / 4][n % 4 * 4 + 2], o[n / 4][n % 4 * 4 + 3]);
+        __syncthreads();
+        float top = kNegInf, factor[TEAMS];
+#pragma unroll
+        for (int n = 0; n < TEAMS; ++n) top = fmaxf(top, sh.stats[n][wave][lane].x);
+        l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < TEAMS; ++n) {
+            const float2 x = sh.stats[n][wave][lane];
+            factor[n] = __builtin_amdgcn_exp2f(x.x - (top == kNegInf ? 0.0f : top));
+            l = fmaf(x.y, factor[n], l);
+        }
+#pragma unroll
+        for (int u = 0; u < TEAMS; ++u) {
+            if (u != (int)team) continue;
+#pragma unroll
+            for (int n = u * kUnits; n < (u + 1) * kUnits; ++n) {
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int from = 0; from < TEAMS; ++from) {
+                    float4 y;
+                    if (from == u) y = make_float4(o[n / 4][n % 4 * 4], o[n / 4][n % 4 * 4 + 1], o[n / 4][n % 4 * 4 + 2], o[n / 4][n % 4 * 4 + 3]);
+                    else y = sh.sums[wave][place(from, u)][n % kUnits][lane];
+                    x.x = fmaf(y.x, factor[from], x.x), x.y = fmaf(y.y, factor[from], x.y);
+                    x.z = fmaf(y.z, factor[from], x.z), x.w = fmaf(y.w, factor[from], x.w);
+                }
+                const int m = n - u * kUnits;  // to the front, where every team's are written from
+                o[m / 4][m % 4 * 4] = x.x, o[m / 4][m % 4 * 4 + 1] = x.y, o[m / 4][m % 4 * 4 + 2] = x.z, o[m / 4][m % 4 * 4 + 3] = x.w;
+            }
+        }
+    }
+    const float by = 1.0f / l;
+    uint16_t* to = static_cast<uint16_t*>(a.out) + (uint64_t)(it.first + rows.pos) * a.out_stride + (uint64_t)rows.head * D + column + team * (kUnits * 8u) + half * 4u;
     bool odd = false;
 #pragma unroll
-    for (int i = 0; i < DW / 32; ++i)
+    for (int n = 0; n < kUnits; ++n) {
+        const f32x16 y = o[n / 4];
+        float z[4];
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const f32x16 y = o[i];
-            float z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = y[r + e] * by, odd = odd || not_finite(z[e]);
-            if (rows.exists) *reinterpret_cast<uint2*>(to + i * 32 + 2 * r) = make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]));
-        }
+        for (int e = 0; e < 4; ++e) z[e] = y[n % 4 * 4 + e] * by, odd = odd || not_finite(z[e]);
+        if (rows.exists) *reinterpret_cast<uint2*>(to + n * 8) = make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]));
+    }
     const unsigned long long both = __ballot(odd && rows.exists);
-    for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
-        redo_row<D, DW, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
+    uint32_t left = (uint32_t)both | (uint32_t)(both >> 32);
+    if constexpr (TEAMS > 1) {  // all teams' columns of a row are one team's, after all have written theirs
+        __syncthreads();
+        uint32_t* rows_of = reinterpret_cast<uint32_t*>(&sh.stats[0][wave][0]);
+        if (team == 0u && lane == 0u) *rows_of = 0u;
+        __syncthreads();
+        if (lane == 0u && left) atomicOr(rows_of, left);
+        __syncthreads();
+        left = *rows_of;
+        for (uint32_t n = 0; left; left &= left - 1u, ++n)
+            if (n % TEAMS == team) redo_row<D, D, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, 0u);
+    } else {
+        for (; left; left &= left - 1u) redo_row<D, DW, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
+    }
 }
 
 // Many rows of FP32. The matrix unit multiplies 16-bit numbers at 16 times its rate of FP32 ones, so every number enters as
@@ -891,37 +902,51 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
         redo_row<D, DW, float>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
 }
 
-// As many workgroups as tiles of `rows` rows that the sequences can have (all but one row of each one's last may be
-// missing) over all key/value heads.
+// As many workgroups as locate() may give numbers to, over all key/value heads.
 uint32_t items_of(const PromptArgs& a, uint32_t rows) {
-    return grid_blocks(((uint64_t)a.tokens * a.group + (uint64_t)a.batch * (rows - 1u)) / rows * a.kv_heads);
+    const uint64_t all = (uint64_t)a.tokens * a.group;
+    const uint64_t tiles = a.batch <= 64u ? (all + (uint64_t)a.batch * (rows - 1u)) / rows : all / rows + a.batch;
+    return grid_blocks(tiles * a.kv_heads);
 }
 
-template <int D, bool F32>
+template <int D>
 void launch_few(const PromptArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_few<D, F32>), dim3(items_of(a, kRows)), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((k_few32<D>), dim3(items_of(a, kRows)), dim3(kThreads), 0, st, a);
 }
 
-template <int D, int W, int KT, int PARTS, int C, int WAVES>
+template <int D, int W, int KT, int PARTS, int C, int WAVES, int TEAMS>
 void launch_many(const PromptArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_many<D, W, KT, PARTS, C, WAVES>), dim3(items_of(a, 32u * W / PARTS)), dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL((k_many<D, W, KT, PARTS, C, WAVES, TEAMS>), dim3(items_of(a, 32u * W / PARTS)), dim3(64 * W * TEAMS), 0, st, a);
 }
 
+// Which form, by the tiles of 128 rows that the sequences may have (measured in us, heads of 256 unless said):
+// - Few tiles leave compute units without work: 32 rows to a workgroup while those fit the card at once (one of them to a
+//   compute unit with heads of 256, two with 128, four with 64): 1 x 512 tokens 27.7 -> 17.7, 1 x 256 with heads of 128
+//   11.5 -> 7.8; past that 4 x 256 would take 22.6 in place of 19.0.
+// - At most two tiles to a compute unit whose sequences are long: two teams, 1 x 2,048 88 -> 67, 1 x 2,048 with heads of 64
+//   39.5 -> 36; 4 x 512 with heads of 64 would take 18.4 in place of 14.0, more tiles more (4 x 1,000: 58 in place of 54).
+// - Heads of 512 take pairs at every size.
+// - FP32: 32 rows to a workgroup and FP32 products below a tile to each compute unit, 1 x 500 84 -> 45, 4 x 256 53 -> 42;
+//   from there on 16-bit parts, 4 x 512 119 -> 88. Heads of 512 take the parts at every size (1 x 64: 57 -> 42).
 template <int D>
 void launch_dim(const PromptArgs& a, int dtype, uint32_t cus, hipStream_t st) {
     if (dtype == TURBO_HIDDEN_F32) {
         constexpr int kParts = D <= 128 ? 1 : D / 128, kManyWaves = kParts == 1 ? 4 : 8;
         const uint32_t items = items_of(a, 32u * kManyWaves / kParts);
-        if (items < cus / 2u) return launch_few<D, true>(a, st);
+        if constexpr (D <= 256)
+            if (items < cus) return launch_few<D>(a, st);
         hipLaunchKernelGGL((k_many32<D, kManyWaves, kParts>), dim3(items), dim3(64 * kManyWaves), 0, st, a);
         return;
     }
-    if constexpr (D <= 128)
-        if (items_of(a, 128u) < cus) return launch_few<D, false>(a, st);
-    if constexpr (D == 64) return launch_many<D, 4, 64, 1, 4, 3>(a, st);
-    if constexpr (D == 128) return launch_many<D, 4, 64, 1, 4, 2>(a, st);
-    if constexpr (D == 256) return launch_many<D, 4, 32, 1, 2, 2>(a, st);
-    if constexpr (D == 512) return launch_many<D, 8, 32, 2, 2, 2>(a, st);
+    if constexpr (D == 512) {
+        launch_many<D, 8, 32, 2, 2, 2, 1>(a, st);
+    } else {
+        const uint32_t tiles = items_of(a, 128u);
+        if ((uint64_t)tiles * D <= cus * 64u) return launch_many<D, 1, 32, 1, 2, (D <= 128 ? 2 : 1), 4>(a, st);
+        constexpr int kTile = D <= 128 ? 64 : 32, kAhead = D <= 128 ? 4 : 2;
+        if (tiles <= 2u * cus && (uint64_t)a.tokens >= 1000ull * a.batch) return launch_many<D, 4, kTile, 1, kAhead, 2, 2>(a, st);
+        launch_many<D, 4, kTile, 1, kAhead, (D == 64 ? 3 : 2), 1>(a, st);
+    }
 }
 
 }  // namespace
