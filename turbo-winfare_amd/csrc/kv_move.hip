@@ -1,9 +1,9 @@
 // Tokens of the quantised cache moved from slot to slot, codes, scales and biases as they are.
 //
-// A workgroup takes one row of moves, one key/value head and the key or the value codes. It reads everything that
-// the row moves into LDS before it writes anything, so a row may move tokens onto slots that it reads. A token's
-// codes share no byte with another token's, so rows need no order among themselves. The bytes are few; what bounds a
-// call is the chain of slots, codes, LDS and stores.
+// A workgroup takes one row of moves, one key/value head and the key or the value codes. Everything that the row moves
+// is read, into LDS, before anything is written, so a row may move tokens onto slots that it reads. A token's codes
+// share no byte with another token's, so rows need no order among themselves. The bytes are few; what bounds a call
+// is the chain of slots, codes and stores.
 #include "dt_internal.h"
 #include "dt_step.h"
 
@@ -50,30 +50,32 @@ __global__ __launch_bounds__(kThreads) void k_kv_move(const KvMoveArgs a) {
         return part + kv_value_byte(bits, t, bits == 8u ? p : (p >> 4) * 32u + (p & 15u));
     };
     auto scale_at = [&](uint32_t t, uint32_t g) { return 2u * part + kv_scale_byte(groups, values ? 1u : 0u, t, g); };
-    auto all_pieces = [&](auto&& code, auto&& scale) {
-        const uint32_t per = pieces + groups;
-        for (uint32_t i = threadIdx.x; i < n * per; i += kThreads) {
-            const uint32_t m = i / per, p = i - m * per;
-            if (p < pieces) code(m, p, lds + m * words + p * size);
-            else scale(m, p - pieces, reinterpret_cast<uint32_t*>(lds + m * words + bytes) + p - pieces);
-        }
-    };
-    auto copy = [&](uint8_t* to, const uint8_t* from) {
-        if (size == 1u) *to = *from;
-        else if (size == 8u) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
-        else
-            *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from),
-            *reinterpret_cast<uint2*>(to + 8) = *reinterpret_cast<const uint2*>(from + 8);
-    };
-    all_pieces([&](uint32_t m, uint32_t p, uint8_t* at) { copy(at, a.kv.base + source[m] + piece_at(source_at[m], p)); },
-               [&](uint32_t m, uint32_t g, uint32_t* at) {
-                   *at = *reinterpret_cast<const uint32_t*>(a.kv.base + source[m] + scale_at(source_at[m], g));
-               });
-    __syncthreads();
-    all_pieces([&](uint32_t m, uint32_t p, uint8_t* at) { copy(a.kv.base + target[m] + piece_at(target_at[m], p), at); },
-               [&](uint32_t m, uint32_t g, uint32_t* at) {
-                   *reinterpret_cast<uint32_t*>(a.kv.base + target[m] + scale_at(target_at[m], g)) = *at;
-               });
+    // A thread takes the same pieces of every token, kAhead tokens' loads side by side. Those of other threads never meet
+    // its own, so it waits for nobody.
+    constexpr uint32_t kAhead = 8u;
+    for (uint32_t p = threadIdx.x; p < pieces + groups; p += kThreads) {
+        uint8_t* const at = lds + (p < pieces ? p * size : bytes + (p - pieces) * 4u);
+        auto move_piece = [&](auto unit) {
+            typedef decltype(unit) Unit;
+            auto place = [&](uint64_t record, uint32_t t) {
+                return reinterpret_cast<Unit*>(a.kv.base + record + (p < pieces ? piece_at(t, p) : scale_at(t, p - pieces)));
+            };
+            for (uint32_t m = 0; m < n; m += kAhead) {
+                Unit x[kAhead];
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i)
+                    if (m + i < n) x[i] = *place(source[m + i], source_at[m + i]);
+#pragma unroll
+                for (uint32_t i = 0; i < kAhead; ++i)
+                    if (m + i < n) *reinterpret_cast<Unit*>(at + (m + i) * words) = x[i];
+            }
+            for (uint32_t m = 0; m < n; ++m) *place(target[m], target_at[m]) = *reinterpret_cast<const Unit*>(at + m * words);
+        };
+        if (p >= pieces) move_piece(uint32_t{});
+        else if (values) move_piece(uint8_t{});
+        else if (bits == 4u) move_piece(uint2{});
+        else move_piece(uint4{});
+    }
 }
 
 }  // namespace
