@@ -1,5 +1,6 @@
 // Attention of a batch over the quantised cache: how a call is split, and what joins the partial results.
 #include <algorithm>
+#include <cmath>
 #include <stdexcept>
 
 #include "dt_attend.h"
@@ -97,11 +98,11 @@ Divider divider(uint32_t d) {  // ceil(2^(31 + L) / d) with 2^(L - 1) < d <= 2^L
 // where two left fewer than 16 records to each. With a border of 8 records 16 sequences of 2,000 measured
 // 17 -> 19 us and 7 x 8 drafts 18 -> 19, though 3 x 10 drafts behind 4,000 31 -> 27; with one of 32, 32 sequences
 // behind 8,000 30 -> 36 us, though 300 prompt tokens 40 -> 34.
-// Trees, whose sequences have many rows each, weigh whole rounds of workgroups: 768 workgroups on 512 places take as long
-// as 1,024 (24 trees of 64 nodes behind 8,192, heads of 256: 508 us; in two splits TREE_SHARED). Figures in microseconds:
-// 8 to begin and end, 3.2 (two tiles) or 2 (one) for a record to each of four waves, 4 for the join and its bytes at
-// 4 TB/s. A window's records are counted once, not for the prefix and the own tokens each (7 trees of 17 nodes with a
-// window of 1,024: TREE_WINDOW us).
+// Trees, whose sequences have many rows each, weigh tiles of 32 and 16 rows and numbers of splits against each other. Figures
+// in microseconds: 8 to begin and end, 3.2 (32 rows) or 2 (16) for a record to each of four waves, 4 for the join and its
+// bytes at 4 TB/s. With few records to a wave the chain of a record's loads and products counts, and so do whole rounds of
+// workgroups; with many the vector unit is full, and a round that is not takes less. A window's records are counted once,
+// not for the prefix and the own tokens each. 7 trees of 17 nodes with a window of 1,024: 32.3 -> 22.3.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -136,7 +137,8 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         if (tree && !shared) {
             const uint64_t tiles = (uint64_t)batch * kv_heads * ot, most_splits = std::min<uint64_t>(64u, (alone + 3u) / 4u);
             for (uint64_t s = 1u; s <= std::max<uint64_t>(1u, most_splits); ++s) {
-                const double rounds = (double)((tiles * s + groups - 1u) / groups), each = (double)(((alone + s - 1u) / s + 3u) / 4u);
+                const double each = (double)(((alone + s - 1u) / s + 3u) / 4u), full = (double)(tiles * s) / (double)groups;
+                const double rounds = each < 16.0 ? std::ceil(full) : std::max(1.0, full);
                 const double join = s > 1u ? 4.0 + (double)p.rows * s * head_dim * 8.0 / 4e6 : 0.0;
                 const double cost = rounds * (8.0 + each * (p.own_tile_rows == 32u ? 3.2 : 2.0)) + join;
                 if (best == 0.0 || cost < best) {

@@ -245,9 +245,11 @@ struct Shared {
     float m[kWaves][16 * MT], l[kWaves][16 * MT], factor[16 * MT];
     int lo[16 * MT], hi[16 * MT];           // what the rows see, read where a record is not seen whole
     float qsum[16 * MT][NG + 1];  // of a row's groups
-    // of drafted trees: where a row's tree begins and the nodes that it sees
-    int tree[TREE ? 16 * MT : 1];
-    unsigned long long nodes[TREE ? 16 * MT : 1];
+    // of drafted trees: where a row's tree begins and the nodes that it sees; then where the sequence's begins and the nodes
+    // that some row sees. Read where a record is not seen whole: registers for them spill (524 -> 570 us of 24 trees of 64
+    // nodes behind 8,192).
+    int tree[TREE ? 16 * MT + 1 : 1];
+    unsigned long long nodes[TREE ? 16 * MT + 1 : 1];
 };
 
 template <int NG, uint32_t BITS, bool F32, int MT, bool TREE>
@@ -272,8 +274,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     Row row[MT];
     bool live[MT];
     int lo_min = 0x7FFFFFFF, lo_max = 0, hi_min = 0x7FFFFFFF, hi_max = 0;  // hi_min: of tokens that are all seen
-    unsigned long long nodes = 0ull;  // of a sequence's tree that some row sees, and where it begins
-    int tree = 0x7FFFFFFF;
+    [[maybe_unused]] unsigned long long nodes = 0ull;  // of a sequence's tree that some row sees
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         row[mt] = row_of<TREE>(a, it, it.row0 + mt * 16u + (lane & 15u));
@@ -291,10 +292,11 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     lo_min = uniform(wave_reduce(lo_min, least)), lo_max = uniform(wave_reduce(lo_max, most));
     hi_min = uniform(wave_reduce(hi_min, least)), hi_max = uniform(wave_reduce(hi_max, most));
     if constexpr (TREE) {
-        if (!it.shared) {
-            nodes = wave_reduce(nodes, [](unsigned long long x, unsigned long long y) { return x | y; });
-            const long long before = (long long)a.kv_len[it.seq] - (long long)a.q_len;
-            if (hi_max > 0) tree = (int)min(before, 0x7FFFFFFFll);
+        nodes = wave_reduce(nodes, [](unsigned long long x, unsigned long long y) { return x | y; });
+        if (threadIdx.x == 0u) {
+            // rows of several sequences have no tree in common; the prefix, which is all that they read, is there
+            sh.tree[16 * MT] = it.shared || hi_max == 0 ? 0x7FFFFFFF : (int)((long long)a.kv_len[it.seq] - (long long)a.q_len);
+            sh.nodes[16 * MT] = nodes;
         }
     }
     // records: of the prefix up to prefix_records, then of the sequence's own tokens
@@ -426,14 +428,14 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     bool vnan = false;
     auto prepare = [&](int base, int end) {
         end = min(end, hi_max);
-        if (base < lo_min || base + (int)kKvBlock > end || (TREE && base + (int)kKvBlock > tree)) {
+        if (base < lo_min || base + (int)kKvBlock > (TREE ? min(end, hi_min) : end)) {
             asm volatile("");  // a branch, not selects: few records are not seen whole
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const int key = base + (int)((lane * NG + i) & 31u);
                 if (key < lo_min || key >= end) sw[i] = 0u;
                 if constexpr (TREE)  // a node that is absent: its slot may hold anything
-                    if (key >= tree && key < end && !((nodes >> (key - tree)) & 1ull)) sw[i] = 0u;
+                    if (const int tree = sh.tree[16 * MT]; key >= tree && key < end && !((sh.nodes[16 * MT] >> (key - tree)) & 1ull)) sw[i] = 0u;
             }
         }
         uint32_t top = 0u;
