@@ -720,7 +720,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
         for (int i = 0; i < kPieces; ++i) vn[i] = *reinterpret_cast<const float4*>(v + row * a.v_stride + i * (int)kPerKey * 4);
     };
     fetch_keys(begin);
-    fetch_values(begin);
+    if constexpr (!Tile::kOnePlace) fetch_values(begin);
 
     const Rows rows(a, it, kv_head, mine);
     Frag qh[DW / 16], ql[DW / 16];
@@ -767,6 +767,17 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
                 value_at[i % kValueTurns] + (uint32_t)((part * kKeys + 16 * j + 8 * e) * D * 2 + i / kValueTurns * kValueTurns * 64)));
         return x;
     };
+    // where a thread's pieces go: an eighth or sixteenth of the row apart, so the exchanged chunks repeat after kTurns
+    constexpr int kApart = (int)kPerKey / 2, kTurns = (D >= 128 ? 16 : 8) / kApart;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) u32x2* Place;
+    uint32_t key_to[kTurns], value_to[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const uint32_t chunk = i * kApart + (my_col >> 3), in = (my_key * D + (my_col & 4u)) * 2u;
+        key_to[i] = lds_at(sh.k) + in + (chunk ^ key_turn<D>(my_key)) * 16u;
+        value_to[i] = lds_at(values) + in + (chunk ^ value_turn<D>(my_key)) * 16u;
+    }
     auto split_keys = [&] {
         float top = 0.0f;
 #pragma unroll
@@ -777,25 +788,23 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
         if (my_col == 0u) sh.power[my_key] = -power;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const uint32_t chunk = (i * kPerKey * 4u + my_col) >> 3;
             uint2 h, l;
             split_fp16(ldexpf(kn[i].x, power), ldexpf(kn[i].y, power), h.x, l.x);
             split_fp16(ldexpf(kn[i].z, power), ldexpf(kn[i].w, power), h.y, l.y);
-            uint16_t* to = sh.k + my_key * D + (my_col & 4u) + (chunk ^ key_turn<D>(my_key)) * 8u;
-            *reinterpret_cast<uint2*>(to) = h;
-            *reinterpret_cast<uint2*>(to + kKeys * D) = l;
+            const uint32_t to = key_to[i % kTurns] + (uint32_t)(i / kTurns * kTurns * kApart * 16);
+            *(Place)(to) = u32x2{h.x, h.y};
+            *(Place)(to + (uint32_t)(kKeys * D * 2)) = u32x2{l.x, l.y};
         }
     };
     auto split_values = [&] {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const uint32_t chunk = (i * kPerKey * 4u + my_col) >> 3;
             uint32_t x[3], y[3];
             split_bf16(vn[i].x, vn[i].y, x);
             split_bf16(vn[i].z, vn[i].w, y);
-            uint16_t* to = values + my_key * D + (my_col & 4u) + (chunk ^ value_turn<D>(my_key)) * 8u;
+            const uint32_t to = value_to[i % kTurns] + (uint32_t)(i / kTurns * kTurns * kApart * 16);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) *reinterpret_cast<uint2*>(to + n * kKeys * D) = make_uint2(x[n], y[n]);
+            for (int n = 0; n < 3; ++n) *(Place)(to + (uint32_t)(n * kKeys * D * 2)) = u32x2{x[n], y[n]};
         }
     };
 
@@ -804,41 +813,54 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
 #pragma unroll
     for (int i = 0; i < DW / 32; ++i) o[i] = zeros();
     for (uint32_t base = begin; base < end; base += kKeys) {
+        if constexpr (D == 512) {
+            // from one place each, made anew here: kept over the loop they spill
+            asm volatile("" : "+v"(key_at[0]), "+v"(value_at[0]));
+#pragma unroll
+            for (int i = 1; i < kKeyTurns; ++i) key_at[i] = key_at[0] ^ (i * 32u);
+#pragma unroll
+            for (int i = 1; i < kValueTurns; ++i) value_at[i] = value_at[0] ^ (i * 64u);
+        }
         __syncthreads();  // nobody reads the tile before any more
         split_keys();
         if constexpr (!Tile::kOnePlace) split_values();
         __syncthreads();
-        if (base + kKeys < end) {
+        if (!Tile::kOnePlace && base + kKeys < end) {
             fetch_keys(base + kKeys);
-            if constexpr (!Tile::kOnePlace) fetch_values(base + kKeys);
+            fetch_values(base + kKeys);
         }
         if (PARTS == 1 && (mine >= all || !rows.some(a, base, kKeys))) continue;
-        f32x16 s[1] = {zeros()}, t = zeros();
+        f32x16 s[1] = {zeros()};
 #pragma unroll
         for (int i = 0; i < DW / 16; ++i) {
             const Frag h = key_read(0, i), l = key_read(1, i);
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, h.x), __builtin_bit_cast(half8v, qh[i].x), s[0], 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, h.x), __builtin_bit_cast(half8v, ql[i].x), t, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, l.x), __builtin_bit_cast(half8v, qh[i].x), t, 0, 0, 0);
+            const half8v kh = __builtin_bit_cast(half8v, h.x), kl = __builtin_bit_cast(half8v, l.x);
+            const half8v xh = __builtin_bit_cast(half8v, qh[i].x), xl = __builtin_bit_cast(half8v, ql[i].x);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, xh, s[0], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, xl, s[0], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, xh, s[0], 0, 0, 0);
             if (i % 2) __builtin_amdgcn_sched_barrier(0);
         }
-        s[0] += t;
         if constexpr (PARTS > 1) {
+            // in one place the values follow the keys, asked for here: the registers hold no more beside the queries
+            if constexpr (Tile::kOnePlace) fetch_values(base);
 #pragma unroll
             for (int e = 0; e < 4; ++e) sh.scores[wave][e][lane] = make_float4(s[0][4 * e], s[0][4 * e + 1], s[0][4 * e + 2], s[0][4 * e + 3]);
             __syncthreads();
             s[0] = zeros();
 #pragma unroll
-            for (uint32_t n = 0; n < PARTS; ++n)  // in the same order for every wave of the row: so are their weights
+            for (uint32_t n = 0; n < PARTS; ++n) {  // in the same order for every wave of the row: so are their weights
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float4 y = sh.scores[wave / PARTS * PARTS + n][e][lane];
                     s[0][4 * e] += y.x, s[0][4 * e + 1] += y.y, s[0][4 * e + 2] += y.z, s[0][4 * e + 3] += y.w;
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if constexpr (Tile::kOnePlace) {
                 split_values();
                 __syncthreads();
-                if (base + kKeys < end) fetch_values(base + kKeys);
+                if (base + kKeys < end) fetch_keys(base + kKeys);
             }
         }
 #pragma unroll
