@@ -83,6 +83,17 @@ def test_packed(batch, longest, page, prefix, in_place):
     compare(pool, new, max_tokens=sum(new) + 5, in_place=in_place)
 
 
+@pytest.mark.parametrize("batch", [2047, 2048, 2049, 8192])
+def test_the_largest_batches(batch):
+    rng = random.Random(batch)
+    past = [rng.randint(0, 90) for _ in range(batch)]
+    new = [rng.choice([0, 1, 2, rng.randint(0, 70)]) for _ in range(batch)]
+    pool = Pool(past, 32, 0, 6, 3 * batch)
+    compare(pool, new, max_tokens=sum(new) + 3, in_place=bool(batch % 2))
+    rows = [min(n, 4) for n in new]
+    compare(pool, rows, row_tokens=4, parents=random_trees(rng, batch, 4, 0.05))
+
+
 @pytest.mark.parametrize("batch,rows", [(1, 1), (5, 1), (40, 7), (9, 64), (600, 3), (2, 5000)])
 def test_rows(batch, rows):
     rng = random.Random(batch)

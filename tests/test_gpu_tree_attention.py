@@ -207,6 +207,19 @@ def test_a_sibling_of_nan():
         assert bool(out.isfinite().all())
 
 
+def test_the_workspace_holds_either_call():
+    """What turbo_attention_workspace gives serves a tree and a run of the same sizes; a byte less than a call needs is refused."""
+    c = Case([900, 1000], 8, 4, 1, 128, seed=5)
+    for window in (0, 200):
+        c.run(window=window)
+        c.check(window)
+        c.cache.attend(c.inp)
+        if window == 0:  # the few records of a window are one part, which needs no scratch
+            c.inp.workspace_bytes = 16
+            with pytest.raises(T.TurboError, match="workspace holds"):
+                c.cache.attend_tree(c.inp, c.d_masks)
+
+
 def test_nodes_past_the_table_give_nan():
     c = Case([60, 20], 8, 2, 1, 64, page=32)
     c.tables = c.tables[:, :2].contiguous()  # room for 64 tokens: sequence 0 has 68

@@ -158,5 +158,9 @@ def test_binding_refuses_arrays_of_another_kind():
         T.make_prompt_inputs(2, 6, q=q, k=q, v=q, out=q, q_heads=2, kv_heads=2, head_dim=64, starts=i32(2), scale=1.0)
     with pytest.raises(ValueError, match="element size"):
         T.make_prompt_inputs(1, 6, dtype=BF16, q=q, k=q, v=q, out=q, q_heads=2, kv_heads=2, head_dim=64, starts=i32(2), scale=1.0)
+    with pytest.raises(ValueError, match="fewer"):
+        T.make_prompt_inputs(1, 7, q=q, k=q, v=q, out=q, q_heads=2, kv_heads=2, head_dim=64, starts=i32(2), scale=1.0)
+    with pytest.raises(ValueError, match="fewer"):
+        T.make_prompt_inputs(1, 6, q=q, k=q, v=q, out=q, q_heads=4, kv_heads=2, head_dim=64, starts=i32(2), scale=1.0)
     with pytest.raises(ValueError, match="tokens"):
         T.make_tree_accept(2, 4, parents=i32(8), new_len=i32(2), tokens=i32(7), chosen=i32(8), kept=i32(2), next=i32(2))

@@ -74,7 +74,7 @@ RotaryBox* rbox(void* p) {
     return r;
 }
 
-// The sizes of an attention call, checked, and how it is split.
+// The sizes of an attention call, checked, and how it is split (which may be into more workgroups than a grid holds).
 tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, bool tree) {
     dtype_size(in.dtype);
     if (in.batch < 0 || in.batch > (1 << 20)) fail("batch must be in 0..1048576");
@@ -88,8 +88,13 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, 
         tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype,
                             in.prefix_len, (uint32_t)(room == 0u ? 0u : beyond == 0u ? 1u : beyond < room ? beyond : room),
                             in.window, c.cus, tree);
-    if (p.items > (1u << 24) - 1u || p.rows * (c.head_dim / 4u) > 0xFFFFFF00ull) fail("batch * q_len * q_heads is too large for one call");
     return p;
+}
+
+bool fits(const CacheBox& c, const tdt::AttnPlan& p) { return p.items <= (1u << 24) - 1u && p.rows * (c.head_dim / 4u) <= 0xFFFFFF00ull; }
+
+void check_plan(const CacheBox& c, const tdt::AttnPlan& p) {
+    if (!fits(c, p)) fail("batch * q_len * q_heads is too large for one call");
 }
 
 }  // namespace
@@ -373,8 +378,14 @@ TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInp
     ATT_TRY
     CacheBox* c = cbox(handle);
     if (!in || !bytes) fail("in or bytes is NULL");
-    *bytes = (size_t)attention_plan(*c, *in, false).bytes;
-    if (in->q_len <= (int)kTreeNodes) *bytes = std::max(*bytes, (size_t)attention_plan(*c, *in, true).bytes);
+    const tdt::AttnPlan plan = attention_plan(*c, *in, false);
+    check_plan(*c, plan);
+    size_t most = (size_t)plan.bytes;
+    if (in->q_len <= (int)kTreeNodes) {  // a tree's call of these sizes may be split another way
+        const tdt::AttnPlan tree = attention_plan(*c, *in, true);
+        if (fits(*c, tree)) most = std::max(most, (size_t)tree.bytes);
+    }
+    *bytes = most;
     return 1;
     ATT_CATCH(0)
 }
@@ -383,6 +394,7 @@ static void attend(void* handle, const TurboAttentionInputs* in, const uint64_t*
     CacheBox* c = cbox(handle);
     if (!in) fail("in is NULL");
     const tdt::AttnPlan plan = attention_plan(*c, *in, masks != nullptr);
+    check_plan(*c, plan);
     if (!std::isfinite(in->scale)) fail("scale must be finite");
     if (in->batch == 0) return;
     const size_t size = dtype_size(in->dtype), packed = (size_t)in->q_heads * c->head_dim;

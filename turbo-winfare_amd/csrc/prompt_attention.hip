@@ -924,11 +924,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
         redo_row<D, DW, float>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
 }
 
-// As many workgroups as locate() may give numbers to, over all key/value heads.
+// As many workgroups of up to 512 threads as locate() may give numbers to, over all key/value heads.
 uint32_t items_of(const PromptArgs& a, uint32_t rows) {
     const uint64_t all = (uint64_t)a.tokens * a.group;
     const uint64_t tiles = a.batch <= 64u ? (all + (uint64_t)a.batch * (rows - 1u)) / rows : all / rows + a.batch;
-    return grid_blocks(tiles * a.kv_heads);
+    return grid_blocks(tiles * a.kv_heads * 2u) / 2u;  // its limit is that of 256 threads
 }
 
 template <int D>

@@ -712,8 +712,10 @@ def _count(name: str, t, n: int) -> int | None:
     return at
 
 
-def _device(*ts) -> int:
-    """The HIP device of the first tensor that has one (0 for raw addresses)."""
+def _device(device: int | None, *ts) -> int:
+    """`device` where it is given, else the HIP device of the first tensor that has one (0 for raw addresses)."""
+    if device is not None:
+        return device
     for t in ts:
         d = getattr(getattr(t, "device", None), "index", None)
         if d is not None:
@@ -847,7 +849,7 @@ class Rotary:
 
 def make_batch_plan(batch: int, *, page_tokens: int, past_len, new_len, max_tokens: int, pages, held, free_pages, free_count,
                     prefix_len: int = 0, row_tokens: int = 0, parents=None, held_out=None, free_count_out=None, starts=None,
-                    kv_len=None, positions=None, slots=None, masks=None, totals=None) -> TurboBatchPlan:
+                    kv_len=None, positions=None, slots=None, masks=None, totals=None, device: int | None = None) -> TurboBatchPlan:
     """Device ids throughout; pages: [batch][page_stride]. held_out and free_count_out: held and free_count, updated in
     place, unless given. The tensors must outlive the struct."""
     held_out = held if held_out is None else held_out
@@ -861,7 +863,7 @@ def make_batch_plan(batch: int, *, page_tokens: int, past_len, new_len, max_toke
                           _count("free_count_out", free_count_out, 1), _count("starts", starts, batch + 1),
                           _count("kv_len", kv_len, batch), _count("positions", positions, max_tokens),
                           _count("slots", slots, max_tokens), _masks(masks, batch * row_tokens), _count("totals", totals, 4),
-                          _device(past_len, pages, held))
+                          _device(device, past_len, pages, held))
 
 
 def batch_plan(inp: TurboBatchPlan, stream=None) -> None:
@@ -870,26 +872,26 @@ def batch_plan(inp: TurboBatchPlan, stream=None) -> None:
 
 
 def pages_release(batch: int, *, page_tokens: int, keep_len, pages, held, free_pages, free_count, prefix_len: int = 0,
-                  stream=None) -> None:
+                  stream=None, device: int | None = None) -> None:
     """turbo_pages_release: every sequence keeps the pages of its first keep_len tokens; held, free_pages and
     free_count are updated."""
     if len(pages.shape) != 2 or pages.shape[0] < batch:
         raise ValueError("pages is [batch][page_stride]")
     inp = TurboPagesRelease(batch, page_tokens, prefix_len, _count("keep_len", keep_len, batch), _ids(pages), int(pages.shape[1]),
                             _count("held", held, batch), _ids(free_pages), _count("free_count", free_count, 1),
-                            int(free_pages.numel()), _device(keep_len, pages, held))
+                            int(free_pages.numel()), _device(device, keep_len, pages, held))
     _ok(load().turbo_pages_release(C.byref(inp), stream))
 
 
 def make_tree_accept(batch: int, row_tokens: int, *, parents, new_len, tokens, chosen, kept, next, past_len=None, slots=None,
-                     length=None, path=None, source=None, target=None) -> TurboTreeAccept:
+                     length=None, path=None, source=None, target=None, device: int | None = None) -> TurboTreeAccept:
     """Device ids: parents, tokens, chosen, slots, path, source and target [batch][row_tokens], the others [batch]."""
     n = batch * row_tokens
     return TurboTreeAccept(batch, row_tokens, _count("parents", parents, n), _count("new_len", new_len, batch),
                            _count("tokens", tokens, n), _count("chosen", chosen, n), _count("past_len", past_len, batch),
                            _count("slots", slots, n), _count("kept", kept, batch), _count("next", next, batch),
                            _count("length", length, batch), _count("path", path, n), _count("source", source, n),
-                           _count("target", target, n), _device(parents, tokens, chosen))
+                           _count("target", target, n), _device(device, parents, tokens, chosen))
 
 
 def tree_accept(inp: TurboTreeAccept, stream=None) -> None:
@@ -898,12 +900,15 @@ def tree_accept(inp: TurboTreeAccept, stream=None) -> None:
 
 
 def make_prompt_inputs(batch: int, tokens: int, *, dtype: int = TURBO_HIDDEN_F32, q, k, v, out, q_heads: int, kv_heads: int,
-                       head_dim: int, starts, window: int = 0, scale: float) -> TurboPromptInputs:
+                       head_dim: int, starts, window: int = 0, scale: float, device: int | None = None) -> TurboPromptInputs:
     """q, k, v, out: torch CUDA tensors [tokens][heads][head_dim] (slices of wider rows too) or raw addresses (packed);
     starts: [batch + 1] device ids."""
+    for name, t, heads in (("q", q, q_heads), ("k", k, kv_heads), ("v", v, kv_heads), ("out", out, q_heads)):
+        if hasattr(t, "numel") and t.numel() < tokens * heads * head_dim:
+            raise ValueError(f"{name} holds fewer than tokens * heads * head_dim values")
     return TurboPromptInputs(batch, tokens, q_heads, kv_heads, head_dim, dtype, _ptr(q), _ptr(k), _ptr(v), _ptr(out),
                              _stride(q, dtype), _stride(k, dtype), _stride(v, dtype), _stride(out, dtype),
-                             _count("starts", starts, batch + 1), window, scale, _device(q, k, v))
+                             _count("starts", starts, batch + 1), window, scale, _device(device, q, k, v))
 
 
 def prompt_attention(inp: TurboPromptInputs, stream=None) -> None:
