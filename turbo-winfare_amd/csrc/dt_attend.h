@@ -246,8 +246,7 @@ struct Shared {
     int lo[16 * MT], hi[16 * MT];           // what the rows see, read where a record is not seen whole
     float qsum[16 * MT][NG + 1];  // of a row's groups
     // of drafted trees: where a row's tree begins and the nodes that it sees; then where the sequence's begins and the nodes
-    // that some row sees. Read where a record is not seen whole: registers for them spill (524 -> 570 us of 24 trees of 64
-    // nodes behind 8,192).
+    // that some row sees. Read from here, as lo and hi are, where a record is not seen whole: the loop has no registers left.
     int tree[TREE ? 16 * MT + 1 : 1];
     unsigned long long nodes[TREE ? 16 * MT + 1 : 1];
 };

@@ -344,14 +344,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_few32(const PromptArgs a) {
         if (n % kWaves == wave) redo_row<D, D, float>(a, it, kv_head, it.tile * kRows + (uint32_t)__ffs(left) - 1u, 0u);
 }
 
-// Many rows: every wave has 32 RT rows of its own, and tiles of KT keys and values go from memory to LDS, without
-// passing registers, for all of them, one tile ahead. A row of a tile is D values, whose 16-byte chunks are exchanged
-// (chunk c lies at c ^ f(row)) so that neither the key reads, 16 bytes of 32 rows, nor the transposing value reads, 64
-// bytes of 8 rows, meet in a bank.
 // Memory that a wave's buffer-to-LDS loads read, 16 bytes to a lane at its byte offset, 1 KB side by side in LDS. They are
 // written as assembly because the compiler takes every later LDS read for one of theirs and waits for them there, before
-// the tile in hand is begun (2,096 us for 16,384 tokens with heads of 128). The wait is the caller's, before the barrier in
-// front of the tile. A load has no result register; its address register is read at issue.
+// the tile in hand is begun (4 x 1,000 tokens with heads of 256: 60 us, 55 as assembly). The wait is the caller's, before
+// the barrier in front of the tile. A load has no result register; its address register is read at issue.
 struct TileSource {
     u32x4 words;
     __device__ inline TileSource(const void* p, uint32_t bytes) {
@@ -363,9 +359,13 @@ struct TileSource {
         const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)lds);
         // five wait states between a scalar register that the vector unit wrote and its use by a buffer load, one behind
         // M0, which nothing else here uses
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(words) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(words) : "memory", "m0");
     }
 };
+// Many rows: every wave has 32 rows of its own, and tiles of KT keys and values go from memory to LDS, without passing
+// registers, for all of them, one tile ahead. A row of a tile is D values, whose 16-byte chunks are exchanged (chunk c lies
+// at c ^ f(row)) so that neither the key reads, 16 bytes of 32 rows, nor the transposing value reads, 64 bytes of 8 rows,
+// meet in a bank.
 template <int D, int KT, int W, int PARTS, int TEAMS>
 struct Many {
     static constexpr int kBuffers = W > 1 ? 2 : 1;
@@ -936,6 +936,11 @@ void launch_few(const PromptArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_few32<D>), dim3(items_of(a, kRows)), dim3(kThreads), 0, st, a);
 }
 
+template <int D, int W, int PARTS>
+void launch_many32(const PromptArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_many32<D, W, PARTS>), dim3(items_of(a, 32u * W / PARTS)), dim3(64 * W), 0, st, a);
+}
+
 template <int D, int W, int KT, int PARTS, int C, int WAVES, int TEAMS>
 void launch_many(const PromptArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_many<D, W, KT, PARTS, C, WAVES, TEAMS>), dim3(items_of(a, 32u * W / PARTS)), dim3(64 * W * TEAMS), 0, st, a);
@@ -949,16 +954,19 @@ void launch_many(const PromptArgs& a, hipStream_t st) {
 //   39.5 -> 36; 4 x 512 with heads of 64 would take 18.4 in place of 14.0, more tiles more (4 x 1,000: 58 in place of 54).
 // - Heads of 512 take pairs at every size.
 // - FP32: 32 rows to a workgroup and FP32 products below a tile to each compute unit, 1 x 500 84 -> 45, 4 x 256 53 -> 42;
-//   from there on 16-bit parts, 4 x 512 119 -> 88. Heads of 512 take the parts at every size (1 x 64: 57 -> 42).
+//   from there on 16-bit parts, 4 x 512 119 -> 88. Heads of 512 take the parts at every size (1 x 64: 57 -> 42), four waves
+//   of 32 rows below a tile to each compute unit, 1 x 512 137 -> 107, and eight of 64 from there on (1 x 1,024: the same).
 template <int D>
 void launch_dim(const PromptArgs& a, int dtype, uint32_t cus, hipStream_t st) {
     if (dtype == TURBO_HIDDEN_F32) {
         constexpr int kParts = D <= 128 ? 1 : D / 128, kManyWaves = kParts == 1 ? 4 : 8;
         const uint32_t items = items_of(a, 32u * kManyWaves / kParts);
-        if constexpr (D <= 256)
-            if (items < cus) return launch_few<D>(a, st);
-        hipLaunchKernelGGL((k_many32<D, kManyWaves, kParts>), dim3(items), dim3(64 * kManyWaves), 0, st, a);
-        return;
+        if (items < cus) {
+            if constexpr (D <= 256) launch_few<D>(a, st);
+            else launch_many32<D, 4, kParts>(a, st);
+            return;
+        }
+        return launch_many32<D, kManyWaves, kParts>(a, st);
     }
     if constexpr (D == 512) {
         launch_many<D, 8, 32, 2, 2, 2, 1>(a, st);
