@@ -59,13 +59,13 @@ class Case:
             out.append((out[p] if p >= 0 else 0) | 1 << t)
         return out
 
-    def run(self, *, window=0, scale=None, masks=None, workspace=None, stream=None, sync=True):
+    def run(self, *, window=0, scale=None, masks=None, workspace=None, stream=None, sync=True, longest=None):
         b = len(self.before)
         self.scale = self.d**-0.5 if scale is None else scale
         self.out = torch.full(self.q.shape, 7.0, dtype=self.q.dtype, device="cuda")
         words = self.masks if masks is None else masks
         self.d_masks = torch.tensor([[m - 2**64 if m >= 2**63 else m for m in row] for row in words], dtype=torch.int64, device="cuda")
-        longest = max([n or 0 for n in self.before]) + self.nodes
+        longest = longest or max([n or 0 for n in self.before]) + self.nodes
         self.inp = self.cache.make_attention_inputs(b, dtype=self.dtype, q=self.q, out=self.out, q_heads=self.hq, q_len=self.nodes,
                                                     kv_len=self.kv_len, max_kv_len=longest, pages=self.tables,
                                                     prefix_len=self.prefix, prefix_pages=self.prefix_pages, window=window, scale=self.scale)
@@ -94,7 +94,8 @@ class Case:
             seen[j, at[-window:] if window else at] = True
         return seen.cuda()
 
-    def check(self, window=0, masks=None):
+    def check(self, window=0, masks=None, rounding=0.0):
+        """rounding: of a key and a value, relative to it."""
         t = self.nodes
         for i, n in enumerate(self.before):
             out = self.out[i * t:(i + 1) * t]
@@ -106,8 +107,8 @@ class Case:
             # a score is off by roundings of 2^-22 (both parts of an FP32 query; a BF16 one is exact) and d + 64 of 2^-24 of
             # what enters it, and a weight by as much relative to itself; a weight times a scale keeps 22 bits, for BF16
             # 11 (2^-11 of each at most); sums of n tokens, n of 2^-24; the result is rounded once
-            spread = 2 * (2.0**-21 + (self.d + 64) * 2.0**-24) * abs(self.scale) * size[..., None]
-            weight = spread + (n + t + 64) * 2.0**-24 + 2.0**-20 + (2.0**-11 if self.dtype == BF16 else 0)
+            spread = 2 * (rounding + 2.0**-21 + (self.d + 64) * 2.0**-24) * abs(self.scale) * size[..., None]
+            weight = spread + rounding + (n + t + 64) * 2.0**-24 + 2.0**-20 + (2.0**-11 if self.dtype == BF16 else 0)
             bound = 1.01 * mean * weight + want.abs() * (2.0**-8 if self.dtype == BF16 else 2.0**-23)
             far = (out.double() - want).abs()
             assert bool((far <= bound).all()), (i, (far / bound).max().item())
@@ -249,6 +250,132 @@ def test_graph_streams_and_two_workspaces():
         c.cache.attend_tree(c.inp, c.d_masks, st.cuda_stream)
     torch.cuda.synchronize()
     assert torch.equal(a.out, want[0]) and torch.equal(b.out, want[1])
+
+
+# ---- trees of many rows, whose records are widened once for 128 of them --------------------------------
+
+# A key and a value are rounded to fp16 there: half a step, 2^-11 of it; and, where it is small against the largest of its
+# head, 2^-22 of that (4 bits: 2^-18), which is below 2^-14 of the size that Case.stored() gives, half a group's range.
+ROUNDING = 2.0**-11 + 2.0**-14
+
+
+class Many(Case):
+    """Takes that form by the longest sequence that the call announces: its table has the columns, of no page."""
+
+    def __init__(self, before, nodes, hq, hk, d, announced=40000, **rest):
+        super().__init__(before, nodes, hq, hk, d, **rest)
+        more = -(-announced // self.page) - self.width
+        if more > 0:
+            fill = torch.full((len(before), more), self.bad_page, dtype=self.tables.dtype, device="cuda")
+            self.tables = torch.cat([self.tables, fill], dim=1).contiguous()
+        self.announced = announced
+
+    def run(self, **rest):
+        return super().run(longest=self.announced, **rest)
+
+
+MANY = [([0, 31, None, 500, 1999], 64, 32, 4), ([700, 33, 32, 1, 64], 40, 24, 4), ([300] * 9, 64, 16, 4), ([2500], 64, 128, 8)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("before,nodes,hq,hk", MANY)
+def test_many_rows(before, nodes, hq, hk, d, bits):
+    c = Many(before, nodes, hq, hk, d, bits=bits, seed=d)
+    c.run()
+    c.check(rounding=ROUNDING)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("prefix", [1, 32, 100, 999])
+def test_many_rows_behind_a_prefix(prefix, d):
+    """Some trees begin inside the shared tokens, one behind none of its own."""
+    c = Many([prefix, prefix + 45, max(0, prefix - 70), None, prefix + 800], 64, 32, 4, d, prefix=prefix, seed=prefix)
+    c.run()
+    c.check(rounding=ROUNDING)
+
+
+def test_many_rows_masks_that_leave_nothing():
+    masks = [[0] * 64, [0 if t % 3 else 1 << t for t in range(64)], [2**64 - 1] * 64]
+    c = Many([900, 100, 40], 64, 64, 4, 128, masks=masks)
+    out = c.run().clone()
+    c.check(rounding=ROUNDING)
+    assert bool((out[:64] == 0).all()) and bool((out[65:67] == 0).all())
+    assert torch.equal(c.run(), out)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_rows_large_values_without_weight(d, bits):
+    """Values 2^60 times the others under keys that no row gives weight, between the others and before them all, cost the
+    others nothing; nor do keys 2^20 times smaller. (The third sequence's last token is taken twice, 2^120: the cache holds
+    2^103 and more as NaN, which all its rows see.)"""
+    c = Many([600, 200, 64], 64, 32, 4, d, bits=bits, seed=1)
+    c.q = c.q.abs() + 0.5
+    for i, n in enumerate(c.before):
+        k, v = c.held[i]
+        for at in (0, 1, 63, n // 2, n - 1):
+            k[at], v[at] = -100, v[at] * 2.0**60
+        k[n // 3] *= 2.0**-20
+        slots = S.ids([S.words(c.tables)[i][j // c.page] * c.page + j % c.page for j in range(n)])
+        c.cache.write(k[:n].contiguous(), v[:n].contiguous(), slots, n, dtype=BF16)
+    out = c.run()
+    assert bool((out[:128].abs() < 100).all()) and bool(out[128:].isnan().all())
+    c.before = c.before[:2]
+    seen = c.seen
+
+    def others(i, window, masks):  # those tokens have no weight: the bound is that of the others
+        s, n = seen(i, window, masks), c.before[i]
+        s[:, [0, 1, 63, n // 2, n - 1]] = False
+        return s
+
+    c.seen = others
+    c.check(rounding=ROUNDING)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_many_rows_nan(which):
+    """NaN in a token before one tree: all its rows see it, the other sequences' none."""
+    c = Many([400, 300], 64, 64, 4, 128)
+    k, v = (x[77:78].clone() for x in c.held[0])
+    (k if which == "k" else v)[0, 1, 3] = math.nan
+    c.cache.write(k.contiguous(), v.contiguous(), S.ids([S.words(c.tables)[0][77 // c.page] * c.page + 77 % c.page]), 1, dtype=BF16)
+    out = c.run()
+    heads = slice(16, 32)  # of that key/value head
+    assert bool(out[:64, heads, 0:64].isnan().all())
+    out = out.clone()
+    out[:64, heads] = 0
+    assert bool(out.isfinite().all())
+
+
+def test_many_rows_bad_pages_and_tables():
+    c = Many([400, 300, 200], 64, 64, 4, 128)
+    t = c.tables.clone()
+    c.tables[0, 3] = -5  # no page of the cache
+    out = c.run().clone()
+    assert bool(out[:64].isnan().all()) and bool(out[64:].isfinite().all())
+    c.tables = t
+    c.kv_len = S.ids([c.announced + 500, 0, 264])  # past the table; padded
+    out = c.run()
+    assert bool(out[:64].isnan().all()) and bool((out[64:128] == 0).all()) and bool(out[128:].isfinite().all())
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_many_rows_graphs_and_streams(d):
+    a, b = Many([900, 30], 64, 64, 4, d, seed=1), Many([400, 1500], 64, 64, 4, d, seed=2)
+    want = [c.run().clone() for c in (a, b)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st = torch.cuda.current_stream().cuda_stream
+        for c in (a, b):
+            c.cache.attend_tree(c.inp, c.d_masks, st)
+    for _ in range(3):
+        for c in (a, b):
+            c.out.zero_()
+            c.workspace.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a.out, want[0]) and torch.equal(b.out, want[1])
 
 
 # ---- a step from lengths to kept tokens --------------------------------------------------------------

@@ -103,6 +103,10 @@ Divider divider(uint32_t d) {  // ceil(2^(31 + L) / d) with 2^(L - 1) < d <= 2^L
 // bytes at 4 TB/s. With few records to a wave the chain of a record's loads and products counts, and so do whole rounds of
 // workgroups; with many the vector unit is full, and a round that is not takes less. A window's records are counted once,
 // not for the prefix and the own tokens each. 7 trees of 17 nodes with a window of 1,024: 32.3 -> 22.3.
+// Trees of many rows in BF16 without a window may take workgroups of 128 rows that widen a record once for all of them
+// (tree_attention.hip). Figures: a record of each of n workgroups on a compute unit, measured in rounds of as many as it holds;
+// 16 to begin and end, the tree's own records among it; the partial results, written and read at 4 TB/s. With heads of 256
+// the other kind's figures, which are those of short chains, are a third below what many records take.
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -154,7 +158,29 @@ AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32
         }
         if (most == 1u || per >= 16u) break;
     }
-    p.parts = p.prefix_splits + p.own_splits;
+    if (tree && best > 0.0 && !window && dtype == TURBO_HIDDEN_BF16 && head_dim <= 256u) {
+        const uint64_t tiles = (own_rows + 127u) / 128u, at_once = wide_groups(head_dim), all = pr + orr;
+        auto record = [&](uint64_t n) {  // of each of n workgroups
+            if (n == 0u) return 0.0;
+            return head_dim == 64u ? 1.1 + 0.32 * (double)n : head_dim == 128u ? 0.95 + 0.67 * (double)n : 1.65 + 0.65 * (double)n;
+        };
+        double least = head_dim == 256u ? 1.35 * best : best;
+        for (uint64_t s = 1u; s <= std::min<uint64_t>(64u, all / 8u); ++s) {
+            const uint64_t on_one = (batch * kv_heads * tiles * s + cus - 1u) / cus;
+            const double records = (double)((all + s - 1u) / s), rounds = (double)(on_one / at_once);
+            const double cost = 16.0 + records * (rounds * record(at_once) + record(on_one % at_once)) + (double)p.rows * (s + 1u) * head_dim * 8.0 / 4e6;
+            if (cost >= least) continue;
+            least = cost;
+            p.wide_tiles = (uint32_t)tiles, p.wide_splits = (uint32_t)s;
+        }
+        if (p.wide_splits) {
+            p.own_tile_rows = p.prefix_tile_rows = 32u;
+            p.own_tiles = (uint32_t)((own_rows + 31u) / 32u), p.own_splits = 1u;
+            p.wide_items = (uint64_t)batch * kv_heads * p.wide_tiles * p.wide_splits;
+            p.items = p.wide_items + (uint64_t)batch * kv_heads * p.own_tiles;
+        }
+    }
+    p.parts = p.prefix_splits + p.wide_splits + p.own_splits;
     if (p.parts > 1u) {
         p.stats_bytes = (p.rows * p.parts * sizeof(float2) + 15u) / 16u * 16u;
         p.bytes = p.stats_bytes + p.rows * p.parts * head_dim * sizeof(float);
@@ -166,6 +192,7 @@ void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int 
     a.prefix_tiles = plan.prefix_tiles, a.prefix_splits = plan.prefix_splits;
     a.own_tiles = plan.own_tiles, a.own_splits = plan.own_splits;
     a.prefix_items = (uint32_t)plan.prefix_items, a.items = (uint32_t)plan.items;
+    a.wide_tiles = plan.wide_tiles, a.wide_splits = plan.wide_splits, a.wide_items = (uint32_t)plan.wide_items;
     a.parts = plan.parts;
     a.by_rows = divider(a.q_len * a.group), a.by_group = divider(a.group);
     if (a.masks) launch_tree_attend(a, plan, head_dim, dtype, st);

@@ -160,6 +160,7 @@ struct Item {
     uint32_t seq;                  // otherwise: the sequence
     uint32_t split, splits, part;
     int begin, end;                // positions of the keys
+    int first;                     // of a tree: records before this one are other workgroups'
     const uint32_t* pages;         // of the sequence's own tokens
 };
 
@@ -305,7 +306,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     };
     int s0 = 0, s1 = 0;  // this split's records
     if (hi_max > 0) {
-        const int b0 = record_of(lo_min), b1 = record_of(hi_max - 1) + 1;
+        const int b1 = record_of(hi_max - 1) + 1, b0 = TREE ? min(b1, max(it.first, record_of(lo_min))) : record_of(lo_min);
         const int per = (b1 - b0 + (int)it.splits - 1) / (int)it.splits;
         s0 = min(b1, b0 + (int)it.split * per), s1 = min(b1, s0 + per);
     }
@@ -787,6 +788,7 @@ __global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const Attn
         Shared<NG, F32, MTO, TREE> o;
     } sh;
     Item it;
+    it.first = 0;
     uint32_t id = blockIdx.x;
     it.shared = id < a.prefix_items;
     if (it.shared) {

@@ -124,6 +124,8 @@ struct AttnArgs {
                                              // sequences take it with their own keys)
     uint32_t own_tiles, own_splits;          // of one sequence's own keys
     uint32_t prefix_items, items;            // workgroups
+    uint32_t wide_tiles, wide_splits;        // of trees: tiles of 128 rows and splits of the records before the tree (0: none)
+    uint32_t wide_items;                     // their workgroups, the first ones
     const uint64_t* masks;                   // [batch][q_len] the nodes that a row of a drafted tree sees, or null
     Divider by_rows, by_group;               // by q_len * group, by group
     uint32_t parts;                          // partial results per row (1: written to out directly)
@@ -133,10 +135,13 @@ struct AttnArgs {
 struct AttnPlan {
     uint32_t prefix_tile_rows, own_tile_rows;  // rows to a workgroup: 16 or 32
     uint32_t prefix_tiles, prefix_splits, own_tiles, own_splits;
-    uint64_t prefix_items, items, rows;
+    uint32_t wide_tiles, wide_splits;
+    uint64_t wide_items, prefix_items, items, rows;
     uint32_t parts;
     uint64_t stats_bytes, bytes;
 };
+// Workgroups of 128 rows of a tree that a compute unit holds at once, by their registers.
+constexpr uint32_t wide_groups(uint32_t head_dim) { return head_dim == 64u ? 4u : head_dim == 128u ? 3u : 2u; }
 AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
                         uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree);
 // tree_attention.hip: the workgroups' kernel of a call with masks; the plan and the join are attention.hip's.
