@@ -487,7 +487,9 @@ TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs*
  * sequence (turbo_batch_plan makes them of the nodes' parents; bits from q_len on are ignored). A query sees the
  * kv_len[b] - q_len tokens before the tree and the nodes of its mask, in this order the last `window` of them
  * where window is not 0. A mask of 0 marks an absent node, which gives zeros; nodes that a query does not see
- * have no part in its result, whatever their slots hold. Everything else, the workspace too, is as there.
+ * have no part in its result, whatever their slots hold. Everything else, the workspace too, is as there, but that
+ * for BF16 queries of many rows the keys and values before the tree may be rounded to fp16, 2^-11 of each and 2^-18 of
+ * the largest of its head, and the smallest weighted values to 2^-20 of the largest.
  */
 TURBO_DT_API int turbo_tree_attention(void* cache, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream);
 
