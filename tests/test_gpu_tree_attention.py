@@ -333,6 +333,13 @@ def test_many_rows_large_values_without_weight(d, bits):
     c.check(rounding=ROUNDING)
 
 
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 0.7])
+def test_many_rows_scales(scale):
+    c = Many([500, 90], 64, 64, 4, 128)
+    c.run(scale=scale)
+    c.check(rounding=ROUNDING)
+
+
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_many_rows_nan(which):
     """NaN in a token before one tree: all its rows see it, the other sequences' none."""

@@ -16,14 +16,17 @@ struct TileSource {
     u32x4 words;
     __device__ inline TileSource(const void* p, uint32_t bytes) {
         const uint64_t at = reinterpret_cast<uint64_t>(p);
-        words = u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
-                      (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufDword3};
+        auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+        words = u32x4{scalar((uint32_t)at), scalar((uint32_t)(at >> 32)) & 0xFFFFu, scalar(bytes), (uint32_t)kBufDword3};
     }
     __device__ inline void load(void* lds, uint32_t offset) const {
-        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+        const uint32_t place = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+        const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
         // five wait states between a scalar register that the vector unit wrote and its use by a buffer load, one behind
         // M0, which nothing else here uses
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(words) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     ::"s"(to), "v"(offset), "s"(words)
+                     : "memory", "m0");
     }
 };
 

@@ -29,8 +29,8 @@ __device__ inline int whole_records(const AttnArgs& a, uint32_t seq) {
 // LDS of a workgroup: a record's operands, and two more records as they come from memory.
 template <int NG, uint32_t BITS>
 struct Wide {
-    static constexpr int kUnits = NG >= 2 ? NG / 2 : 1;                                // of 16 codes to a lane that a wave widens, of keys and of values
-    static constexpr int kLoads = BITS == 8u ? kUnits : kUnits > 1 ? kUnits / 2 : 1;  // of 1 KB
+    // units of 16 codes to a lane that a wave widens, of keys and of values, and loads of 1 KB for them
+    static constexpr int kUnits = NG >= 2 ? NG / 2 : 1, kLoads = BITS == 8u ? kUnits : kUnits > 1 ? kUnits / 2 : 1;
     uint4 k[NG * 4][64], v[NG * 4][64];         // keys [group][16 tokens][chunk of 32], values [16 values]
     int k_power[2][kKvBlock], v_power[2][kKvBlock];
     uint32_t words[kWaves][2 * NG * kKvBlock];  // a wave's: scale and bias of [keys, values][group][token] in fp16
@@ -105,7 +105,8 @@ __device__ inline void wide(const AttnArgs& a, const Item& it, int records, Wide
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t w = q[mt][n][c].u[i];
-                    v[2 * i] = ldexpf(__uint_as_float(w << 16), shift) * sign, v[2 * i + 1] = ldexpf(__uint_as_float(w & 0xFFFF0000u), shift) * sign;
+                    v[2 * i] = ldexpf(__uint_as_float(w << 16), shift) * sign;
+                    v[2 * i + 1] = ldexpf(__uint_as_float(w & 0xFFFF0000u), shift) * sign;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {  // in the order of the codes
@@ -171,7 +172,7 @@ __device__ inline void wide(const AttnArgs& a, const Item& it, int records, Wide
             const uint4 x = from[j][lane];
             to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
         } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(&from[KU > 1 ? j >> 1 : 0][lane]) + ((unit0 + j) & 1u) * 8u);
+            const uint2 x = reinterpret_cast<const uint2*>(&from[KU > 1 ? j >> 1 : 0][lane])[(unit0 + j) & 1u];
             to[0] = x.x, to[1] = x.y;
         }
     };
@@ -319,9 +320,10 @@ __device__ inline void wide(const AttnArgs& a, const Item& it, int records, Wide
             if (r < prefix_records && (r + 1) * (int)kKvBlock > prefix_len) {
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) asm volatile("" : "+v"(s[mt][0]), "+v"(s[mt][1]));  // a branch, not selects
+                const int behind = prefix_len - r * (int)kKvBlock - (int)(this_lane() >> 4) * 4;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (r * (int)kKvBlock + (j >> 2) * 16 + (int)(this_lane() >> 4) * 4 + (j & 3) >= prefix_len) s[0][j >> 2][j & 3] = s[1][j >> 2][j & 3] = kNegInf;
+                    if ((j >> 2) * 16 + (j & 3) >= behind) s[0][j >> 2][j & 3] = s[1][j >> 2][j & 3] = kNegInf;
             }
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
