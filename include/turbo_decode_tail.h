@@ -550,7 +550,7 @@ typedef struct {
     /* results, each may be NULL */
     uint32_t* starts;               /* [batch + 1] first entry of every sequence */
     uint32_t* kv_len;               /* [batch] past + new; for rows past + row_tokens, as the attention counts its
-                                       queries (0 for a sequence that adds nothing) */
+                                       queries (0 for a sequence that adds nothing); may be past_len itself */
     uint32_t* positions;            /* [max_tokens] */
     uint32_t* slots;                /* [max_tokens] */
     uint64_t* masks;                /* [batch][row_tokens], with parents */

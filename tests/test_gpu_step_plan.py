@@ -83,6 +83,25 @@ def test_packed(batch, longest, page, prefix, in_place):
     compare(pool, new, max_tokens=sum(new) + 5, in_place=in_place)
 
 
+@pytest.mark.parametrize("batch,longest", [(5, 20), (60, 700), (2100, 40)])
+def test_lengths_in_the_place_of_the_past(batch, longest):
+    """kv_len may be past_len itself: the lengths after the step, and the same slots, whatever runs first."""
+    rng = random.Random(batch)
+    past = [rng.randint(0, 300) for _ in range(batch)]
+    new = [rng.randint(0, longest) for _ in range(batch)]
+    pool = Pool(past, 32, 0, (300 + longest) // 32 + 2, sum(new) // 32 + 2 * batch)
+    n, tables = sum(new), [list(t) for t in pool.tables]
+    want = S.plan(pool.past, new, pool.held, tables, pool.free, 32, 0, pool.width, 0, n, None)
+    pool.device(len(pool.free) + 1)
+    slots, held, count = empty(n), empty(batch), empty(1)
+    T.batch_plan(T.make_batch_plan(batch, page_tokens=32, past_len=pool.d_past, new_len=(d_new := S.ids(new)), max_tokens=n,
+                                   pages=pool.d_pages, held=pool.d_held, free_pages=pool.d_free, free_count=pool.d_count,
+                                   held_out=held, free_count_out=count, kv_len=pool.d_past, slots=slots))
+    torch.cuda.synchronize()
+    assert S.words(slots) == want["slots"] and S.words(pool.d_past) == want["kv_len"] and S.words(held) == want["held"]
+    del d_new
+
+
 @pytest.mark.parametrize("batch", [2047, 2048, 2049, 8192])
 def test_the_largest_batches(batch):
     rng = random.Random(batch)

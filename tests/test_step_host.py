@@ -47,6 +47,14 @@ def test_plan_refuses(field, value, word):
     refused(T.load().turbo_batch_plan, inp, word)
 
 
+@pytest.mark.parametrize("result,taken", [("slots", "past_len"), ("kv_len", "new_len"), ("held_out", "past_len"), ("starts", "pages"),
+                                          ("free_count_out", "held"), ("totals", "free_count"), ("kv_len", "slots"), ("positions", "slots")])
+def test_plan_refuses_results_in_the_place_of_others(result, taken):
+    inp = plan()
+    setattr(inp, result, getattr(inp, taken))
+    refused(T.load().turbo_batch_plan, inp, "of the plan")
+
+
 @pytest.mark.parametrize("rows,word", [(0, "row_tokens"), (65, "row_tokens")])
 def test_plan_refuses_trees_that_masks_do_not_hold(rows, word):
     inp = plan()

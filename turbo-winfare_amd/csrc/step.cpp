@@ -77,6 +77,18 @@ TURBO_DT_API int turbo_batch_plan(const TurboBatchPlan* in, void* hip_stream) {
     for (const void* p : {static_cast<const void*>(in->parents), static_cast<const void*>(in->starts), static_cast<const void*>(in->kv_len),
                           static_cast<const void*>(in->positions), static_cast<const void*>(in->slots), static_cast<const void*>(in->totals)})
         if (reinterpret_cast<uintptr_t>(p) % 4u != 0u) fail("an array of the plan is not 4-byte aligned");
+    // what some workgroups read while others write results; held, free_count and past_len may be updated in place
+    const void* inputs[] = {in->past_len, in->new_len, in->held, in->free_pages, in->free_count, in->parents, in->pages};
+    const void* results[] = {in->held_out, in->free_count_out, in->kv_len, in->starts, in->positions, in->slots, in->totals, in->masks};
+    for (const void*& r : results) {
+        if (!r) continue;
+        for (const void* p : inputs)
+            if (p == r && !(r == in->held_out && p == in->held) && !(r == in->free_count_out && p == in->free_count) &&
+                !(r == in->kv_len && p == in->past_len))
+                fail("a result of the plan is one of its inputs");
+        for (const void*& other : results)
+            if (&other != &r && other == r) fail("two results of the plan are one array");
+    }
     check_device(in->device);
     a.batch = (uint32_t)in->batch;
     a.prefix_len = in->prefix_len;

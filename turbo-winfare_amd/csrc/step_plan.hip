@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void k_accept(const AcceptArgs a) {
 void launch_plan(PlanArgs a, hipStream_t st) {
     const uint32_t lds = (2u * (a.batch + 1u) + (a.batch <= kCopied ? 2u * a.batch : 0u)) * 4u;
     const uint32_t tokens = a.parents ? (a.batch + kWaves - 1u) / kWaves : grid_blocks(((uint64_t)a.max_tokens + kTokensPerBlock - 1u) / kTokensPerBlock);
-    const bool apart = a.held_out != a.held && a.free_out != a.free_count;
+    const bool apart = a.held_out != a.held && a.free_out != a.free_count && a.kv_len != a.past;
     uint32_t blocks = 1u;
     a.tokens = 1u, a.pages_from = 0u, a.state = 1;
     if (tokens > 1u) {
