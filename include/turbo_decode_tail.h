@@ -477,7 +477,8 @@ typedef struct {
     size_t workspace_bytes;
 } TurboAttentionInputs;
 
-/* The scratch a call with these sizes needs (0: none); pointers are not looked at. */
+/* The scratch a call with these sizes needs (0: none); pointers are not looked at. With a q_len of at most 64 it serves
+ * turbo_tree_attention too, whose partial results may be more (of many rows 512 MB at most). */
 TURBO_DT_API int turbo_attention_workspace(void* cache, const TurboAttentionInputs* in, size_t* bytes);
 TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs* in, void* hip_stream);
 
