@@ -234,7 +234,9 @@ __device__ inline Frag operand(uint4 v) {
 
 template <int NG, bool F32, int MT, bool TREE>
 struct Shared {
-    static constexpr uint32_t kRow = 68;  // floats of a row of 64, padded
+    // One tile of up to 256 columns is joined at once, others a group of 64 columns at a time; padded rows
+    static constexpr bool kAtOnce = MT == 1 && NG <= 4;
+    static constexpr uint32_t kRow = kAtOnce ? NG * 64 + 4 : 68;
     union {
         struct {
             uint4 q[MT][NG][F32 ? 4 : 2][64];            // the queries as second operands: [.., chunk of 32 (and low parts)][lane]
@@ -315,42 +317,57 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     // all four waves, which divide the tiles among them and then a tile's groups; a negative scale is
     // theirs, so that larger scores are larger weights
     const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
-    constexpr int kSharers = (int)kWaves / MT;
+    constexpr int kSharers = (int)kWaves / MT, kOwn = (NG + kSharers - 1) / kSharers;  // of a tile; groups of a wave
+    {
+        const uint32_t mt = wave % MT, share = wave / MT;
+        float x[kOwn][2][8], top = 0.0f, bad = 0.0f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        if (mt != (int)wave % MT) continue;
-        const uint64_t at = row[mt].token * a.q_stride + (uint64_t)row[mt].head * D + g * 16u;
-        float x[NG][2][8], top = 0.0f, bad = 0.0f;
+        for (int i = 0; i < MT; ++i) {
+            if ((uint32_t)i != mt) continue;
+            const uint64_t at = row[i].token * a.q_stride + (uint64_t)row[i].head * D + g * 16u;
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+            for (int j = 0; j < kOwn; ++j) {
+                if (share + j * kSharers >= (uint32_t)NG) continue;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                load_q8<F32>(a.q, at + n * 64u + c * 8u, x[n][c]);
+                for (int c = 0; c < 2; ++c) {
+                    load_q8<F32>(a.q, at + (share + j * kSharers) * 64u + c * 8u, x[j][c]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[n][c][i])), bad = fmaf(x[n][c][i], 0.0f, bad);
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][c][e])), bad = fmaf(x[j][c][e], 0.0f, bad);
+                }
             }
+        }
         top = rows_max(top);
         bad = rows_sum(bad);  // NaN where a value is infinite or NaN: so is the row then, whatever its scores' signs
+        if constexpr (kSharers > 1 && NG > 1) {  // over the tile's waves
+            if (g == 0u) sh.m[wave][lane] = top, sh.l[wave][lane] = bad;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t w = 0; w < (uint32_t)kSharers; ++w) {
+                top = fmaxf(top, sh.m[w * MT + mt][lane & 15u]);
+                bad += sh.l[w * MT + mt][lane & 15u];
+            }
+        }
         const int shift = top > 0.0f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
         const float factor = sign == 0.0f ? 1.0f : fminf(ldexpf(fabsf(a.scale_log2e), a.scale_power - shift), 0x1.fffffep127f);
-        if (g == 0u && (int)wave < MT) sh.factor[mt * 16 + lane] = factor + bad;
+        if (g == 0u && share == 0u) sh.factor[mt * 16 + lane] = factor + bad;
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if (n % kSharers != (int)wave / MT) continue;
+        for (int j = 0; j < kOwn; ++j) {
+            const uint32_t n = share + j * kSharers;
+            if (n >= (uint32_t)NG) continue;
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ldexpf(x[n][c][i], shift) * sign, sum += v[i];
+                for (int i = 0; i < 8; ++i) v[i] = ldexpf(x[j][c][i], shift) * sign, sum += v[i];
                 Frag h, low;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int j = BITS == 8u ? 2 * i : i, k = j + (BITS == 8u ? 1 : 4);
-                    h.u[i] = pack_fp16(v[j], v[k]);
+                    const int y = BITS == 8u ? 2 * i : i, z = y + (BITS == 8u ? 1 : 4);
+                    h.u[i] = pack_fp16(v[y], v[z]);
                     if constexpr (F32) {
                         const Pair u = unpack_fp16(h.u[i]);
-                        low.u[i] = pack_fp16(v[j] - u.lo, v[k] - u.hi);
+                        low.u[i] = pack_fp16(v[y] - u.lo, v[z] - u.hi);
                     }
                 }
                 sh.q[mt][n][c][lane] = make_uint4(h.u[0], h.u[1], h.u[2], h.u[3]);
@@ -700,6 +717,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
         rec = next_rec;
     }
 
+    constexpr bool kAtOnce = Shared<NG, F32, MT, TREE>::kAtOnce;
     // ---- the four waves join: every wave scales its sums to the workgroup's maximum
     __syncthreads();
 #pragma unroll
@@ -737,7 +755,7 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-        if (n) __syncthreads();
+        if (n && !kAtOnce) __syncthreads();
         float centre[MT];  // of group n
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -755,26 +773,29 @@ __device__ inline void attend(const AttnArgs& a, const Item& it, Shared<NG, F32,
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = counts[mt] ? own[mt] * (ldexpf(o[mt][n * 4 + d][e], (int)u[mt] - kUnit) + centre[mt]) : 0.0f;
-                *reinterpret_cast<float4*>(&sh.sums[wave][mt * 16 + (lane & 15u)][d * 16 + g * 4]) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(&sh.sums[wave][mt * 16 + (lane & 15u)][(kAtOnce ? n * 64 : 0) + d * 16 + g * 4]) = make_float4(v[0], v[1], v[2], v[3]);
             }
+        if (kAtOnce && n < NG - 1) continue;
         __syncthreads();
+#pragma unroll
+        for (int n2 = kAtOnce ? 0 : n; n2 <= n; ++n2)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t r = mt * 16u + out_row;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (uint32_t w = 0; w < kWaves; ++w) {
-                const float4 x = *reinterpret_cast<const float4*>(&sh.sums[w][r][col]);
+                const float4 x = *reinterpret_cast<const float4*>(&sh.sums[w][r][(kAtOnce ? n2 * 64 : 0) + col]);
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
             }
             if (!to[mt].exists) continue;
             if (a.parts > 1u) {
                 if (total[mt] != 0.0f)
                     *reinterpret_cast<float4*>(a.sums + (((uint64_t)to[mt].token * a.q_heads + to[mt].head) * a.parts + it.part) * D +
-                                               n * 64u + col) = v;
+                                               n2 * 64u + col) = v;
             } else {
                 const float r1 = total[mt] != 0.0f ? 1.0f / total[mt] : 0.0f;
-                store_out<F32>(a.out, to[mt].token * a.out_stride + (uint64_t)to[mt].head * D + n * 64u + col,
+                store_out<F32>(a.out, to[mt].token * a.out_stride + (uint64_t)to[mt].head * D + n2 * 64u + col,
                                make_float4(v.x * r1, v.y * r1, v.z * r1, v.w * r1));
             }
         }
