@@ -842,11 +842,6 @@ __global__ __launch_bounds__(kThreads, NG <= 4 ? 2 : 1) void k_attend(const Attn
     }
 }
 
-// 16-row tiles of a workgroup at most: what the registers of two waves per SIMD hold without spills (heads of 256:
-// all 256). One in place of two: 94 -> 117 us (2 x 512 prompt tokens behind 2,000), 100 -> 121 us (128 sequences
-// behind 16,000, heads of 128), but 40 -> 34 us (300 prompt tokens with heads of 128, whose workgroups then fill the
-// card).
-constexpr int most_tiles(uint32_t head_dim, bool f32) { return head_dim <= (f32 ? 128u : 256u) ? 2 : 1; }
 template <int NG, uint32_t BITS, bool F32, bool TREE, int MTP, int MTO>
 void launch_tiles(const AttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_attend<NG, BITS, F32, MTP, MTO, TREE>), dim3(a.items), dim3(kThreads), 0, st, a);

@@ -19,9 +19,9 @@
 #include <stdint.h>
 #include <stdexcept>
 
-namespace tdt {
+#include "dt_plan.h"
 
-constexpr uint32_t kKvBlock = 32;  // tokens per record
+namespace tdt {
 
 struct KvView {
     uint8_t* base;
@@ -132,18 +132,6 @@ struct AttnArgs {
     float2* stats;                           // [rows][parts] (running maximum, sum)
     float* sums;                             // [rows][parts][head_dim]
 };
-struct AttnPlan {
-    uint32_t prefix_tile_rows, own_tile_rows;  // rows to a workgroup: 16 or 32
-    uint32_t prefix_tiles, prefix_splits, own_tiles, own_splits;
-    uint32_t wide_tiles, wide_splits;
-    uint64_t wide_items, prefix_items, items, rows;
-    uint32_t parts;
-    uint64_t stats_bytes, bytes;
-};
-// Workgroups of 128 rows of a tree that a compute unit holds at once, by their registers.
-constexpr uint32_t wide_groups(uint32_t head_dim) { return head_dim == 64u ? 4u : head_dim == 128u ? 3u : 2u; }
-AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, int dtype,
-                        uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree);
 // tree_attention.hip: the workgroups' kernel of a call with masks; the plan and the join are attention.hip's.
 void launch_tree_attend(const AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);
 void launch_attention(AttnArgs& a, const AttnPlan& plan, uint32_t head_dim, int dtype, hipStream_t st);

@@ -85,7 +85,7 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, 
     if (in.prefix_len + room > 0x7FFFFF00u) fail("prefix_len + page_stride * page_tokens must be at most 2^31 - 256");
     const uint64_t beyond = in.max_kv_len > in.prefix_len ? in.max_kv_len - in.prefix_len : 0u;
     const tdt::AttnPlan p =
-        tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype,
+        tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype == TURBO_HIDDEN_F32,
                             in.prefix_len, (uint32_t)(room == 0u ? 0u : beyond == 0u ? 1u : beyond < room ? beyond : room),
                             in.window, c.cus, tree);
     return p;
