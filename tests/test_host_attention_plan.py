@@ -1,0 +1,104 @@
+"""How attention calls are split, from the library's own host code compiled here (csrc/dt_plan.h), for a card of 256
+compute units: the partial results that the join reads are those that the kernels of the form that was chosen write."""
+import itertools
+import random
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+FIELDS = ("prefix_tile_rows", "own_tile_rows", "prefix_tiles", "prefix_splits", "own_tiles", "own_splits", "wide_tiles",
+          "wide_splits", "wide_items", "prefix_items", "items", "rows", "parts", "stats_bytes", "bytes")
+PROGRAM = """
+#include <cstdio>
+#include "dt_plan.h"
+int main() {
+    unsigned v[10];
+    auto next = [&] {
+        for (unsigned& x : v)
+            if (std::scanf("%%u", &x) != 1) return false;
+        return true;
+    };
+    while (next()) {
+        const tdt::AttnPlan p = tdt::plan_attention(v[0], v[1], v[2], v[3], v[4], v[5] == 0u, v[6], v[7], v[8], 256u, v[9] != 0u);
+        const unsigned long long out[] = {%s};
+        for (unsigned long long x : out) std::printf("%%llu ", x);
+        std::puts("");
+    }
+}
+""" % ", ".join("p." + f for f in FIELDS)
+F32, BF16 = 0, 1
+
+
+@pytest.fixture(scope="module")
+def plans(tmp_path_factory):
+    """Plans of shapes (batch, q_len, q_heads, kv_heads, head_dim, dtype, prefix, own tokens, window, tree)."""
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++20", "-O2", f"-I{ROOT / 'turbo-winfare_amd' / 'csrc'}", str(d / "plan.cpp"),
+                    "-o", str(d / "plan")], check=True)
+
+    def run(shapes):
+        text = "\n".join(" ".join(str(int(x)) for x in s) for s in shapes)
+        out = subprocess.run([str(d / "plan")], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
+        assert len(out) == len(shapes)
+        return [dict(zip(FIELDS, map(int, line.split()))) for line in out]
+
+    return run
+
+
+def parts_written(shape, p):
+    """Numbers of the partial results of a row that the kernels write, by the workgroups that a call has."""
+    batch, q_len, q_heads, kv_heads = shape[:4]
+    rows = q_len * (q_heads // kv_heads)
+    assert p["own_tiles"] * p["own_tile_rows"] >= rows
+    if p["wide_splits"]:  # 128 rows of a sequence, then its other records in one part
+        assert p["wide_tiles"] * 128 >= rows and p["wide_items"] == batch * kv_heads * p["wide_tiles"] * p["wide_splits"]
+        assert p["items"] == p["wide_items"] + batch * kv_heads * p["own_tiles"]
+        return list(range(p["wide_splits"])) + [p["wide_splits"]]
+    assert p["wide_tiles"] == p["wide_items"] == 0
+    if p["prefix_splits"]:
+        assert p["prefix_tiles"] * p["prefix_tile_rows"] >= batch * rows
+    assert p["prefix_items"] == kv_heads * p["prefix_tiles"] * p["prefix_splits"]
+    assert p["items"] == p["prefix_items"] + batch * kv_heads * p["own_tiles"] * p["own_splits"]
+    return list(range(p["prefix_splits"])) + [p["prefix_splits"] + s for s in range(p["own_splits"])]
+
+
+def hold(plans, shapes):
+    got = plans(shapes)
+    for shape, p in zip(shapes, got):
+        assert parts_written(shape, p) == list(range(p["parts"])), (shape, p)
+        assert p["rows"] == shape[0] * shape[1] * shape[2]
+        values = p["rows"] * p["parts"] if p["parts"] > 1 else 0
+        assert p["stats_bytes"] >= 8 * values and p["bytes"] == p["stats_bytes"] + 4 * values * shape[4], (shape, p)
+    return got
+
+
+# Trees whose tiles of 32 rows take the prefix with their own tokens, while tiles of 16 rows take it apart.
+TWO_KINDS = [(18, 10, 64, 32, 64, 1536, 40), (34, 21, 16, 16, 64, 1600, 21), (49, 7, 96, 32, 64, 256, 7), (57, 21, 9, 9, 64, 1000, 600),
+             (66, 21, 8, 8, 64, 336, 600)]
+
+
+def test_trees_that_one_tile_takes_apart_and_another_does_not(plans):
+    hold(plans, [(b, t, hq, hk, d, BF16, prefix, own, 0, True) for b, t, hq, hk, d, prefix, own in TWO_KINDS])
+
+
+def test_every_part_is_written_by_somebody(plans):
+    heads = [(4, 4), (8, 1), (16, 8), (9, 9), (64, 32), (24, 8)]
+    shapes = [(b, t, hq, hk, d, dtype, prefix, own, window, tree)
+              for b, t, (hq, hk), d, dtype, prefix, own, window, tree in itertools.product(
+                  (1, 2, 18, 57), (1, 7, 17, 21, 64), heads, (64, 256, 512), (F32, BF16), (0, 100, 1536), (0, 40, 2000), (0, 300),
+                  (False, True))]
+    hold(plans, shapes)
+
+
+def test_every_part_of_random_trees_is_written_by_somebody(plans):
+    rng = random.Random(1)
+    shapes = []
+    for _ in range(150000):
+        hk = rng.choice([1, 2, 3, 4, 8, 9, 16, 32])
+        shapes.append((rng.randint(1, 80), rng.randint(1, 64), hk * rng.choice([1, 1, 2, 3, 4, 8]), hk, rng.choice([64, 128, 256]), BF16,
+                       rng.randint(0, 3000), rng.randint(0, 1500), 0, True))
+    got = hold(plans, shapes)
+    assert sum(p["wide_splits"] > 0 for p in got) > 1000 and sum(p["prefix_splits"] > 0 for p in got) > 1000

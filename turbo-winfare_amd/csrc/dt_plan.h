@@ -55,7 +55,9 @@ inline uint32_t tiles_for(uint64_t rows, uint32_t most) {
 // (tree_attention.hip). Figures: a record of each of n workgroups on a compute unit, measured in rounds of as many as it holds;
 // 16 to begin and end, the tree's own records among it; the partial results, written and read at 4 TB/s. With heads of 256
 // the other kind's figures, which are those of short chains, are a quarter below what many records take. Of 40 mixed shapes
-// four take 11 to 33 % less time than in the other kind, one 7 % more.
+// four take 11 to 33 % less time than in the other kind, one 7 % more. Where tiles of 16 rows take the prefix apart, that is
+// what runs, whatever tiles of 32 rows would have cost: 18 trees of 10 nodes, 64 / 32 heads of 64 behind 1,536, 40 us in place
+// of 80; 57 of 21 behind 1,000, 44 in place of 72.
 inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, bool f32,
                                uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
@@ -107,7 +109,7 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
         }
         if (most == 1u || per >= 16u) break;
     }
-    if (tree && best > 0.0 && !window && !f32 && head_dim <= 256u) {
+    if (tree && !p.prefix_splits && !window && !f32 && head_dim <= 256u) {
         const uint64_t tiles = (own_rows + 127u) / 128u, at_once = wide_groups(head_dim), all = pr + orr;
         auto record = [&](uint64_t n) {  // of each of n workgroups
             if (n == 0u) return 0.0;
