@@ -3,8 +3,9 @@ their scratch must hold, against the formula in 64 bits."""
 import pytest
 
 torch = pytest.importorskip("torch")
+import step_util as S
 import turbo_decode_tail as T
-from test_gpu_tree_attention import ROUNDING, Case
+from test_gpu_tree_attention import ROUNDING, Case, Many
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +29,43 @@ def test_the_join_reads_what_the_call_wrote(batch, nodes, hq, hk, prefix, own):
     c.check(rounding=ROUNDING)
     for byte in (255, 0, 64):
         assert torch.equal(again_over(c, byte), want), byte
+
+
+@pytest.mark.parametrize("power", [20, 28, 34, 60])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_values_that_lose_their_weight(d, bits, power):
+    """Every third record holds nothing but large values under keys that lead while no others are met, and have 2^-100 of the
+    weight of those: what they leave is below 2^-40 of the result, and the others' bits must be as without them."""
+    c = Many([640, 200, 1999], 64, 32, 4, d, bits=bits, seed=power)
+    c.q = c.q.abs() + 0.5
+    large = [torch.arange(n, device="cuda") // 32 % 3 == 0 for n in c.before]
+    large[1][:] = False
+    for i, n in enumerate(c.before):
+        k, v = (x[:n] for x in c.held[i])
+        v.copy_(v.abs() + 0.5)
+        k[large[i]] = -70.0 / (1.3 * d**0.5)
+        v[large[i]] *= 2.0**power
+        slots = S.ids([S.words(c.tables)[i][j // c.page] * c.page + j % c.page for j in range(n)])
+        c.cache.write(k.contiguous(), v.contiguous(), slots, n, dtype=T.TURBO_HIDDEN_BF16)
+    out = c.run().double()
+    small = 2.0**-18 if bits == 4 else 2.0**-22  # of a head's largest
+    for i, n in enumerate(c.before):
+        k, v = (c.stored(x)[0].double() for x in c.held[i])
+        seen = c.seen(i, 0)
+        seen[:, :n] &= ~large[i]
+        for h in range(c.hq):
+            kk, vv = k[:, h // 8], v[:, h // 8]
+            q = c.q[i * 64:(i + 1) * 64, h].double()
+            s = (q @ kk.T.contiguous() * c.scale).masked_fill_(~seen, -torch.inf)
+            w = s.softmax(dim=1)
+            want = w @ vv
+            # Of a key and a value 2^-11 and `small` of the head's largest; a weight is off by as much, relative to itself, as
+            # twice a score, and by 2^-11 when it is rounded. A weighted value that is small keeps 2^-20 of the row's largest.
+            wrong = (q.abs() @ (2.0**-11 * kk.abs() + small * kk.abs().amax(dim=1, keepdim=True)).T.contiguous() * c.scale).masked_fill_(~seen, 0.0)
+            weight = 2 * wrong.amax(dim=1, keepdim=True) + 2.0**-11 + 2.0**-16
+            top = vv.masked_fill(~seen.any(dim=0)[:, None], 0.0).abs().amax(dim=1)
+            rest = (w * top).amax(dim=1, keepdim=True) * 2.0**-20 * (n + 64) + small * (w @ top)[:, None]
+            bound = 1.01 * ((w @ vv.abs()) * (weight + 2.0**-11) + rest) + want.abs() * 2.0**-8
+            far = (out[i * 64:(i + 1) * 64, h] - want).abs()
+            assert bool((far <= bound).all()), (i, h, (far / bound).max().item())

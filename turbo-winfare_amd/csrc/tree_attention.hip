@@ -122,7 +122,8 @@ __device__ inline void wide(const AttnArgs& a, const Item& it, int records, Wide
 
     float4v o[2][NG * 4];
     float m[2], l[2];
-    int unit[2] = {-1000, -1000};  // a row's sums are in units of 2^(unit - kUnit)
+    constexpr int kNoUnit = -1000;  // below all that a record needs
+    int unit[2] = {kNoUnit, kNoUnit};  // a row's sums are in units of 2^(unit - kUnit)
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
         m[mt] = kNegInf, l[mt] = 0.0f;
@@ -338,11 +339,16 @@ __device__ inline void wide(const AttnArgs& a, const Item& it, int records, Wide
                 const float rise = top - m[mt];
                 if (__any(rise > kSlack)) {
                     asm volatile("");
-                    const float by = rise > kSlack ? rise : 0.0f, alpha = __builtin_amdgcn_exp2f(-by);
+                    const float by = rise > kSlack ? rise : 0.0f;
                     if (rise > kSlack) m[mt] = top;
-                    l[mt] *= alpha;
+                    l[mt] *= __builtin_amdgcn_exp2f(-by);
+                    // The unit falls with the sums, which then lose less than a bit: what large values under keys that led
+                    // leave behind does not take the later ones' bits.
+                    const int to = max(unit[mt] - (int)fminf(by, 4000.0f), kNoUnit);
+                    const float alpha = __builtin_amdgcn_exp2f((float)(unit[mt] - to) - by);
 #pragma unroll
                     for (int i = 0; i < NG * 4; ++i) o[mt][i] *= alpha;
+                    unit[mt] = to;
                 }
                 const float zero = m[mt] == kNegInf ? 0.0f : m[mt];
 #pragma unroll
