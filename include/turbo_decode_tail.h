@@ -471,14 +471,14 @@ typedef struct {
     uint32_t page_stride;
     uint32_t window;
     float scale;
-    /* device scratch of turbo_attention_workspace bytes, 16-byte aligned; calls that may overlap (two
+    /* device scratch of turbo_attention_workspace (turbo_tree_workspace) bytes, 16-byte aligned; calls that may overlap (two
      * streams, two graphs) have one each */
     void* workspace;
     size_t workspace_bytes;
 } TurboAttentionInputs;
 
 /* The scratch a call with these sizes needs (0: none); pointers are not looked at. With a q_len of at most 64 it serves
- * turbo_tree_attention too, whose partial results may be more (of many rows 512 MB at most). */
+ * turbo_tree_attention too, which has use for more (turbo_tree_workspace). */
 TURBO_DT_API int turbo_attention_workspace(void* cache, const TurboAttentionInputs* in, size_t* bytes);
 TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs* in, void* hip_stream);
 
@@ -488,11 +488,15 @@ TURBO_DT_API int turbo_prefix_attention(void* cache, const TurboAttentionInputs*
  * sequence (turbo_batch_plan makes them of the nodes' parents; bits from q_len on are ignored). A query sees the
  * kv_len[b] - q_len tokens before the tree and the nodes of its mask, in this order the last `window` of them
  * where window is not 0. A mask of 0 marks an absent node, which gives zeros; nodes that a query does not see
- * have no part in its result, whatever their slots hold. Everything else, the workspace too, is as there, but that
+ * have no part in its result, whatever their slots hold. Everything else is as there, but that
  * for BF16 queries of many rows the keys and values before the tree may be rounded to fp16, 2^-11 of each and 2^-18 of
  * the largest of its head, and the smallest weighted values to 2^-20 of the largest.
  */
 TURBO_DT_API int turbo_tree_attention(void* cache, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream);
+/* The scratch with which a tree's call of these sizes is fastest (of many rows 512 MB of partial results at most). The call
+ * takes less, down to this or what turbo_attention_workspace gives, whichever is smaller, and then splits the keys into
+ * fewer parts: how much there is decides the last bits of the results. */
+TURBO_DT_API int turbo_tree_workspace(void* cache, const TurboAttentionInputs* in, size_t* bytes);
 
 /*
  * Moves tokens inside the cache, codes, scales and biases bit by bit: the token at source[r * width + i] goes to

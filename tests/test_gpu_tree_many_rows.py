@@ -1,5 +1,7 @@
 """Attention of drafted trees of many rows (turbo_tree_attention's workgroups of 128 rows): what their splits, their units and
 their scratch must hold, against the formula in 64 bits."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -69,3 +71,53 @@ def test_large_values_that_lose_their_weight(d, bits, power):
             bound = 1.01 * ((w @ vv.abs()) * (weight + 2.0**-11) + rest) + want.abs() * 2.0**-8
             far = (out[i * 64:(i + 1) * 64, h] - want).abs()
             assert bool((far <= bound).all()), (i, h, (far / bound).max().item())
+
+
+def sizes(c):
+    """What the two calls of the C interface give for the case's last call."""
+    n = C.c_size_t()
+    out = []
+    for call in (c.cache.lib.turbo_attention_workspace, c.cache.lib.turbo_tree_workspace):
+        assert call(c.cache.h, C.byref(c.inp), C.byref(n)) == 1
+        out.append(n.value)
+    return out
+
+
+def test_a_run_needs_what_it_needed_before_there_were_trees():
+    """256 sequences of 64 rows, one part each: no scratch, where a tree would have use for 540 MB."""
+    cache = T.KvCache(1, 64, 8, 256)
+    inp = cache.make_attention_inputs(256, dtype=T.TURBO_HIDDEN_BF16, q=None, out=None, q_heads=16, q_len=64, kv_len=None,
+                                      max_kv_len=2000, pages=torch.zeros((256, 32), dtype=torch.int32, device="cuda"), scale=1.0)
+    n = C.c_size_t()
+    assert cache.lib.turbo_attention_workspace(cache.h, C.byref(inp), C.byref(n)) == 1 and n.value == 0
+    assert cache.lib.turbo_tree_workspace(cache.h, C.byref(inp), C.byref(n)) == 1 and n.value > 2**29
+    assert cache.attention_workspace(inp, tree=False) == 0 and cache.attention_workspace(inp) == cache.attention_workspace(inp, tree=True) == n.value
+    inp.q_len = 65
+    assert cache.lib.turbo_tree_workspace(cache.h, C.byref(inp), C.byref(n)) == 0 and "q_len" in T.last_error()
+    assert cache.attention_workspace(inp) == cache.attention_workspace(inp, tree=False)
+    cache.close()
+
+
+@pytest.mark.parametrize("shape", [([900, 1000], 8, 4, 1, 128, 0), ([300] * 9, 64, 16, 4, 64, 0), ([1600] * 34, 21, 16, 16, 64, 1600),
+                                   ([2500, 700], 64, 128, 8, 256, 0)], ids=str)
+@pytest.mark.parametrize("dtype", [T.TURBO_HIDDEN_F32, T.TURBO_HIDDEN_BF16])
+def test_a_tree_in_the_scratch_of_a_run(shape, dtype):
+    """Any size from the smaller of both on, and a byte less is refused."""
+    before, nodes, hq, hk, d, prefix = shape
+    c = Case(before, nodes, hq, hk, d, prefix=prefix, dtype=dtype, seed=9)
+    c.run()
+    c.check(rounding=ROUNDING)
+    run, tree = sizes(c)
+    for n in sorted({run, tree, (run + tree) // 2, min(run, tree)}):
+        c.workspace = torch.empty(n + 64, dtype=torch.uint8, device="cuda")
+        c.inp.workspace, c.inp.workspace_bytes = c.workspace.data_ptr(), n
+        again_over(c, 255)
+        c.check(rounding=ROUNDING)
+        assert bool((c.workspace[n:] == 255).all())
+    if min(run, tree) > 0:
+        c.inp.workspace_bytes = min(run, tree) - 1
+        with pytest.raises(T.TurboError, match="workspace holds"):
+            c.cache.attend_tree(c.inp, c.d_masks)
+        c.inp.workspace, c.inp.workspace_bytes = None, tree
+        with pytest.raises(T.TurboError, match="workspace is NULL"):
+            c.cache.attend_tree(c.inp, c.d_masks)

@@ -14,14 +14,14 @@ PROGRAM = """
 #include <cstdio>
 #include "dt_plan.h"
 int main() {
-    unsigned v[10];
+    unsigned long long v[11];
     auto next = [&] {
-        for (unsigned& x : v)
-            if (std::scanf("%%u", &x) != 1) return false;
+        for (unsigned long long& x : v)
+            if (std::scanf("%%llu", &x) != 1) return false;
         return true;
     };
     while (next()) {
-        const tdt::AttnPlan p = tdt::plan_attention(v[0], v[1], v[2], v[3], v[4], v[5] == 0u, v[6], v[7], v[8], 256u, v[9] != 0u);
+        const tdt::AttnPlan p = tdt::plan_attention(v[0], v[1], v[2], v[3], v[4], v[5] == 0u, v[6], v[7], v[8], 256u, v[9] != 0u, v[10]);
         const unsigned long long out[] = {%s};
         for (unsigned long long x : out) std::printf("%%llu ", x);
         std::puts("");
@@ -33,14 +33,15 @@ F32, BF16 = 0, 1
 
 @pytest.fixture(scope="module")
 def plans(tmp_path_factory):
-    """Plans of shapes (batch, q_len, q_heads, kv_heads, head_dim, dtype, prefix, own tokens, window, tree)."""
+    """Plans of shapes (batch, q_len, q_heads, kv_heads, head_dim, dtype, prefix, own tokens, window, tree) and, where it is
+    given, the partial results that a tree may leave, in bytes."""
     d = tmp_path_factory.mktemp("plan")
     (d / "plan.cpp").write_text(PROGRAM)
     subprocess.run(["g++", "-std=c++20", "-O2", f"-I{ROOT / 'turbo-winfare_amd' / 'csrc'}", str(d / "plan.cpp"),
                     "-o", str(d / "plan")], check=True)
 
     def run(shapes):
-        text = "\n".join(" ".join(str(int(x)) for x in s) for s in shapes)
+        text = "\n".join(" ".join(str(int(x)) for x in (*s, 2**64 - 1)[:11]) for s in shapes)
         out = subprocess.run([str(d / "plan")], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
         assert len(out) == len(shapes)
         return [dict(zip(FIELDS, map(int, line.split()))) for line in out]
@@ -102,3 +103,23 @@ def test_every_part_of_random_trees_is_written_by_somebody(plans):
                        rng.randint(0, 3000), rng.randint(0, 1500), 0, True))
     got = hold(plans, shapes)
     assert sum(p["wide_splits"] > 0 for p in got) > 1000 and sum(p["prefix_splits"] > 0 for p in got) > 1000
+
+
+def test_a_tree_takes_the_scratch_that_there_is(plans):
+    """In as many bytes as the tree's best plan needs that plan; in fewer another that fits them and is whole; a run's bytes are
+    always enough."""
+    rng = random.Random(2)
+    shapes = [(b, t, hq, hk, d, BF16, prefix, own, 0, True) for b, t, hq, hk, d, prefix, own in TWO_KINDS]
+    shapes += [(256, 64, 16, 8, 256, BF16, 0, 2000, 0, True), (64, 64, 16, 8, 256, BF16, 0, 2000, 0, True)]
+    for _ in range(20000):
+        hk = rng.choice([1, 2, 4, 8, 16])
+        shapes.append((rng.randint(1, 80), rng.randint(1, 64), hk * rng.choice([1, 2, 4]), hk, rng.choice([64, 128, 256, 512]),
+                       rng.choice([F32, BF16]), rng.choice([0, rng.randint(0, 3000)]), rng.randint(0, 3000), rng.choice([0, 0, 700]), True))
+    best = hold(plans, shapes)
+    assert plans([(*s, p["bytes"]) for s, p in zip(shapes, best)]) == best
+    runs = hold(plans, [(*s[:9], False) for s in shapes])
+    for limit in ([p["bytes"] for p in runs], [0] * len(best), [rng.randint(0, p["bytes"]) for p in best]):
+        for p, most in zip(hold(plans, [(*s, n) for s, n in zip(shapes, limit)]), limit):
+            assert p["bytes"] <= most
+    grown = [(s, r["bytes"], p["bytes"]) for s, r, p in zip(shapes, runs, best) if p["bytes"] > r["bytes"]]
+    assert grown and runs[5]["bytes"] == 0  # 256 sequences of 64 rows are one part each as a run

@@ -58,8 +58,10 @@ inline uint32_t tiles_for(uint64_t rows, uint32_t most) {
 // four take 11 to 33 % less time than in the other kind, one 7 % more. Where tiles of 16 rows take the prefix apart, that is
 // what runs, whatever tiles of 32 rows would have cost: 18 trees of 10 nodes, 64 / 32 heads of 64 behind 1,536, 40 us in place
 // of 80; 57 of 21 behind 1,000, 44 in place of 72.
+// A tree's plan leaves at most most_bytes of partial results; one part, which leaves none, always does.
 inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, bool f32,
-                               uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree) {
+                               uint32_t prefix_len, uint32_t own_most, uint32_t window, uint32_t cus, bool tree,
+                               uint64_t most_bytes = ~0ull) {
     const uint64_t group = q_heads / kv_heads, own_rows = q_len * group, all_rows = batch * own_rows;
     auto records = [&](uint64_t keys, uint64_t spread) {
         if (window) keys = std::min<uint64_t>(keys, (uint64_t)window + spread);
@@ -68,6 +70,8 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
     const uint64_t pr = prefix_len ? records(prefix_len, prefix_len / 4u) : 0u, orr = own_most ? records(own_most, q_len) : 0u;
     AttnPlan p{};
     p.rows = (uint64_t)batch * q_len * q_heads;
+    auto stats_bytes = [&](uint64_t parts) { return parts > 1u ? (p.rows * parts * 2u * sizeof(float) + 15u) / 16u * 16u : 0u; };
+    auto bytes = [&](uint64_t parts) { return parts > 1u ? stats_bytes(parts) + p.rows * parts * head_dim * sizeof(float) : 0u; };
     double best = 0.0;
     AttnPlan chosen{};
     for (uint32_t most = most_tiles(head_dim, f32);; most /= 2u) {
@@ -75,12 +79,17 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
         const uint64_t ot = (own_rows + p.own_tile_rows - 1u) / p.own_tile_rows;
         p.prefix_tile_rows = 16u * tiles_for(all_rows, most);
         uint64_t pt = (all_rows + p.prefix_tile_rows - 1u) / p.prefix_tile_rows;
-        const bool shared = pr && 2u * batch * ot > 3u * pt;
+        const uint64_t groups = head_dim <= 256u ? 2u * cus : cus;
+        auto share_of = [&](uint64_t work) { return std::max<uint64_t>(4u, (work + groups - 1u) / groups); };  // records
+        bool shared = pr && 2u * batch * ot > 3u * pt;
+        if (tree && shared) {
+            const uint64_t per = share_of(kv_heads * (pt * pr + batch * ot * orr));
+            shared = bytes((pr + per - 1u) / per + (orr + per - 1u) / per) <= most_bytes;
+        }
         if (!shared) p.prefix_tile_rows = p.own_tile_rows, pt = 0u;
         uint64_t alone = shared ? orr : pr + orr;  // records of a workgroup's sequence
         if (tree && !shared && window) alone = std::min(alone, records((uint64_t)prefix_len + own_most, q_len) + 1u);
-        const uint64_t work = kv_heads * (pt * pr + batch * ot * alone);
-        const uint64_t groups = head_dim <= 256u ? 2u * cus : cus, per = std::max<uint64_t>(4u, (work + groups - 1u) / groups);
+        const uint64_t per = share_of(kv_heads * (pt * pr + batch * ot * alone));
         p.prefix_tiles = (uint32_t)pt;
         p.prefix_splits = shared ? (uint32_t)((pr + per - 1u) / per) : 0u;
         p.own_tiles = (uint32_t)ot;
@@ -91,7 +100,7 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
         p.items = p.prefix_items + (uint64_t)batch * kv_heads * ot * p.own_splits;
         if (tree && !shared) {
             const uint64_t tiles = (uint64_t)batch * kv_heads * ot, most_splits = std::min<uint64_t>(64u, (alone + 3u) / 4u);
-            for (uint64_t s = 1u; s <= std::max<uint64_t>(1u, most_splits); ++s) {
+            for (uint64_t s = 1u; s <= std::max<uint64_t>(1u, most_splits) && bytes(s) <= most_bytes; ++s) {
                 const double each = (double)(((alone + s - 1u) / s + 3u) / 4u), full = (double)(tiles * s) / (double)groups;
                 const double rounds = each < 16.0 ? std::ceil(full) : std::max(1.0, full);
                 const double join = s > 1u ? 4.0 + (double)p.rows * s * head_dim * 8.0 / 4e6 : 0.0;
@@ -119,7 +128,7 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
         for (uint64_t s = 1u; s <= std::min<uint64_t>(64u, all / 8u); ++s) {
             const uint64_t on_one = (batch * kv_heads * tiles * s + cus - 1u) / cus;
             const double records = (double)((all + s - 1u) / s), rounds = (double)(on_one / at_once);
-            if (p.rows * (s + 1u) * head_dim > (1u << 27)) break;  // partial results of 512 MB at most
+            if (p.rows * (s + 1u) * head_dim > (1u << 27) || bytes(s + 1u) > most_bytes) break;  // partial results of 512 MB at most
             const double parts = (double)p.rows * (s + 1u) * head_dim * 8.0 / 4e6;
             const double cost = 16.0 + records * (rounds * record(at_once) + record(on_one % at_once)) + parts;
             if (cost >= least) continue;
@@ -134,10 +143,7 @@ inline AttnPlan plan_attention(uint32_t batch, uint32_t q_len, uint32_t q_heads,
         }
     }
     p.parts = p.prefix_splits + p.wide_splits + p.own_splits;
-    if (p.parts > 1u) {
-        p.stats_bytes = (p.rows * p.parts * 2u * sizeof(float) + 15u) / 16u * 16u;
-        p.bytes = p.stats_bytes + p.rows * p.parts * head_dim * sizeof(float);
-    }
+    p.stats_bytes = stats_bytes(p.parts), p.bytes = bytes(p.parts);
     return p;
 }
 

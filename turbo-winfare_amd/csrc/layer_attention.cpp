@@ -75,7 +75,7 @@ RotaryBox* rbox(void* p) {
 }
 
 // The sizes of an attention call, checked, and how it is split (which may be into more workgroups than a grid holds).
-tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, bool tree) {
+tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, bool tree, uint64_t most_bytes = ~0ull) {
     dtype_size(in.dtype);
     if (in.batch < 0 || in.batch > (1 << 20)) fail("batch must be in 0..1048576");
     if (in.q_len < 1 || in.q_len > (1 << 20)) fail("q_len must be in 1..1048576");
@@ -87,14 +87,16 @@ tdt::AttnPlan attention_plan(const CacheBox& c, const TurboAttentionInputs& in, 
     const tdt::AttnPlan p =
         tdt::plan_attention((uint32_t)in.batch, (uint32_t)in.q_len, (uint32_t)in.q_heads, c.kv.heads, c.head_dim, in.dtype == TURBO_HIDDEN_F32,
                             in.prefix_len, (uint32_t)(room == 0u ? 0u : beyond == 0u ? 1u : beyond < room ? beyond : room),
-                            in.window, c.cus, tree);
+                            in.window, c.cus, tree, most_bytes);
     return p;
 }
 
-bool fits(const CacheBox& c, const tdt::AttnPlan& p) { return p.items <= (1u << 24) - 1u && p.rows * (c.head_dim / 4u) <= 0xFFFFFF00ull; }
-
 void check_plan(const CacheBox& c, const tdt::AttnPlan& p) {
-    if (!fits(c, p)) fail("batch * q_len * q_heads is too large for one call");
+    if (p.items > (1u << 24) - 1u || p.rows * (c.head_dim / 4u) > 0xFFFFFF00ull) fail("batch * q_len * q_heads is too large for one call");
+}
+
+void check_nodes(int q_len) {
+    if (q_len < 1 || q_len > (int)tdt::kTreeNodes) fail("q_len must be in 1..64 for a tree");
 }
 
 }  // namespace
@@ -374,18 +376,26 @@ TURBO_DT_API int turbo_qk_norm_rope(void* handle, const TurboQkvInputs* in, void
 
 // ---- attention ---------------------------------------------------------------------------------------
 
-TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInputs* in, size_t* bytes) {
-    ATT_TRY
+static void workspace(void* handle, const TurboAttentionInputs* in, bool tree, size_t* bytes) {
     CacheBox* c = cbox(handle);
     if (!in || !bytes) fail("in or bytes is NULL");
-    const tdt::AttnPlan plan = attention_plan(*c, *in, false);
+    const tdt::AttnPlan plan = attention_plan(*c, *in, tree);
     check_plan(*c, plan);
-    size_t most = (size_t)plan.bytes;
-    if (in->q_len <= (int)kTreeNodes) {  // a tree's call of these sizes may be split another way
-        const tdt::AttnPlan tree = attention_plan(*c, *in, true);
-        if (fits(*c, tree)) most = std::max(most, (size_t)tree.bytes);
-    }
-    *bytes = most;
+    *bytes = (size_t)plan.bytes;
+}
+
+TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInputs* in, size_t* bytes) {
+    ATT_TRY
+    workspace(handle, in, false, bytes);
+    return 1;
+    ATT_CATCH(0)
+}
+
+TURBO_DT_API int turbo_tree_workspace(void* handle, const TurboAttentionInputs* in, size_t* bytes) {
+    ATT_TRY
+    cbox(handle);
+    if (in) check_nodes(in->q_len);
+    workspace(handle, in, true, bytes);
     return 1;
     ATT_CATCH(0)
 }
@@ -393,7 +403,10 @@ TURBO_DT_API int turbo_attention_workspace(void* handle, const TurboAttentionInp
 static void attend(void* handle, const TurboAttentionInputs* in, const uint64_t* masks, void* hip_stream) {
     CacheBox* c = cbox(handle);
     if (!in) fail("in is NULL");
-    const tdt::AttnPlan plan = attention_plan(*c, *in, masks != nullptr);
+    tdt::AttnPlan plan = attention_plan(*c, *in, masks != nullptr);
+    if (const uint64_t there = in->workspace ? in->workspace_bytes : 0u; masks && there < plan.bytes)
+        // what a run of these sizes needs is enough for a tree, in fewer parts
+        if (there >= attention_plan(*c, *in, false).bytes) plan = attention_plan(*c, *in, true, there);
     check_plan(*c, plan);
     if (!std::isfinite(in->scale)) fail("scale must be finite");
     if (in->batch == 0) return;
@@ -444,7 +457,7 @@ TURBO_DT_API int turbo_tree_attention(void* handle, const TurboAttentionInputs* 
     ATT_TRY
     cbox(handle);
     if (!in) fail("in is NULL");
-    if (in->q_len < 1 || in->q_len > (int)tdt::kTreeNodes) fail("q_len must be in 1..64 for a tree");
+    check_nodes(in->q_len);
     if (in->batch > 0 && !masks) fail("masks is NULL");
     if (reinterpret_cast<uintptr_t>(masks) % 8u != 0u) fail("masks must be 8-byte aligned");
     attend(handle, in, masks, hip_stream);

@@ -78,6 +78,7 @@ EXPORTS = (
     "turbo_attention_workspace",
     "turbo_prefix_attention",
     "turbo_tree_attention",
+    "turbo_tree_workspace",
     "turbo_kv_cache_move",
     "turbo_batch_plan",
     "turbo_pages_release",
@@ -402,6 +403,7 @@ def load(path: os.PathLike | str | None = None) -> C.CDLL:
         "turbo_qk_norm_rope": (i32, [vp, C.POINTER(TurboQkvInputs), vp]),
         "turbo_attention_workspace": (i32, [vp, C.POINTER(TurboAttentionInputs), C.POINTER(C.c_size_t)]),
         "turbo_prefix_attention": (i32, [vp, C.POINTER(TurboAttentionInputs), vp]),
+        "turbo_tree_workspace": (i32, [vp, C.POINTER(TurboAttentionInputs), C.POINTER(C.c_size_t)]),
         "turbo_tree_attention": (i32, [vp, C.POINTER(TurboAttentionInputs), vp, vp]),
         "turbo_kv_cache_move": (i32, [vp, vp, vp, i32, i32, vp]),
         "turbo_batch_plan": (i32, [C.POINTER(TurboBatchPlan), vp]),
@@ -756,10 +758,17 @@ class KvCache:
                                     int(pages.shape[1]) if pages is not None else 0, window, scale, _ptr(workspace),
                                     workspace.numel() if workspace is not None else 0)
 
-    def attention_workspace(self, inp: TurboAttentionInputs) -> int:
-        n = C.c_size_t()
-        _ok(self.lib.turbo_attention_workspace(self.h, C.byref(inp), C.byref(n)))
-        return n.value
+    def attention_workspace(self, inp: TurboAttentionInputs, tree: bool | None = None) -> int:
+        """Bytes of scratch for attend (tree False: turbo_attention_workspace) or attend_tree (True: turbo_tree_workspace);
+        without `tree` the larger of both, where there are at most 64 queries to a sequence."""
+        calls = {False: [self.lib.turbo_attention_workspace], True: [self.lib.turbo_tree_workspace]}.get(tree)
+        if calls is None:
+            calls = [self.lib.turbo_attention_workspace] + ([self.lib.turbo_tree_workspace] if inp.q_len <= 64 else [])
+        n, most = C.c_size_t(), 0
+        for call in calls:
+            _ok(call(self.h, C.byref(inp), C.byref(n)))
+            most = max(most, n.value)
+        return most
 
     def attend(self, inp: TurboAttentionInputs, stream=None) -> None:
         """turbo_prefix_attention: out = softmax(scale q k) v over the shared prefix and each sequence's own keys."""
