@@ -98,6 +98,17 @@ def test_a_run_needs_what_it_needed_before_there_were_trees():
     cache.close()
 
 
+def test_a_run_that_no_tree_could_be():
+    """As a tree these sizes are more workgroups than a grid holds; that does not refuse the run's scratch."""
+    cache = T.KvCache(1, 32, 32, 64)
+    inp = cache.make_attention_inputs(218774, dtype=T.TURBO_HIDDEN_BF16, q=None, out=None, q_heads=64, q_len=19, kv_len=None,
+                                      max_kv_len=100000, pages=torch.zeros((1, 3125), dtype=torch.int32, device="cuda"), scale=1.0)
+    with pytest.raises(T.TurboError, match="too large"):
+        cache.attention_workspace(inp, tree=True)
+    assert cache.attention_workspace(inp) == cache.attention_workspace(inp, tree=False)
+    cache.close()
+
+
 @pytest.mark.parametrize("shape", [([900, 1000], 8, 4, 1, 128, 0), ([300] * 9, 64, 16, 4, 64, 0), ([1600] * 34, 21, 16, 16, 64, 1600),
                                    ([2500, 700], 64, 128, 8, 256, 0)], ids=str)
 @pytest.mark.parametrize("dtype", [T.TURBO_HIDDEN_F32, T.TURBO_HIDDEN_BF16])

@@ -760,15 +760,16 @@ class KvCache:
 
     def attention_workspace(self, inp: TurboAttentionInputs, tree: bool | None = None) -> int:
         """Bytes of scratch for attend (tree False: turbo_attention_workspace) or attend_tree (True: turbo_tree_workspace);
-        without `tree` the larger of both, where there are at most 64 queries to a sequence."""
-        calls = {False: [self.lib.turbo_attention_workspace], True: [self.lib.turbo_tree_workspace]}.get(tree)
-        if calls is None:
-            calls = [self.lib.turbo_attention_workspace] + ([self.lib.turbo_tree_workspace] if inp.q_len <= 64 else [])
+        without `tree` the larger of both, where a tree's call of these sizes is one."""
         n, most = C.c_size_t(), 0
-        for call in calls:
-            _ok(call(self.h, C.byref(inp), C.byref(n)))
-            most = max(most, n.value)
-        return most
+        if tree or (tree is None and inp.q_len <= 64):
+            there = self.lib.turbo_tree_workspace(self.h, C.byref(inp), C.byref(n))
+            if tree:
+                _ok(there)
+                return n.value
+            most = n.value if there else 0
+        _ok(self.lib.turbo_attention_workspace(self.h, C.byref(inp), C.byref(n)))
+        return max(most, n.value)
 
     def attend(self, inp: TurboAttentionInputs, stream=None) -> None:
         """turbo_prefix_attention: out = softmax(scale q k) v over the shared prefix and each sequence's own keys."""
