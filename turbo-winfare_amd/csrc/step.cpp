@@ -220,8 +220,8 @@ TURBO_DT_API int turbo_prompt_attention(const TurboPromptInputs* in, void* hip_s
     a.kv_heads = (uint32_t)in->kv_heads;
     a.group = a.q_heads / a.kv_heads;
     a.window = in->window;
-    // of 0 the least number: every finite score then weighs 1 all the same, and a hidden one's -infinity stays
-    a.scale_log2e = std::fmax((float)std::fabs(scale), FLT_MIN);
+    // of 0 the least number there is, 2^-149: every finite score then weighs 1 to 2^-21, and a hidden one's -infinity stays
+    a.scale_log2e = std::fmax((float)std::fabs(scale), FLT_TRUE_MIN);
     a.flip = in->scale >= 0.0f ? 0u : in->dtype == TURBO_HIDDEN_BF16 ? 0x80008000u : 0x80000000u;
     DeviceGuard dg(in->device);
     launch_prompt(a, in->head_dim, in->dtype, (uint32_t)compute_units(in->device), static_cast<hipStream_t>(hip_stream));
