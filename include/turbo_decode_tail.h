@@ -614,10 +614,13 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream);
  * Query i of it sees keys 0 .. i, the last `window` of them where window is not 0:
  *   out = sum_j softmax_j(scale * q . k_j) v_j
  * query head h over key/value head h / (q_heads / kv_heads). Buffers as the layer loop's common rules have them, with
- * strides of at most 2^24 elements. Rows of no sequence are left as they were. Scores, softmax statistics and sums are
- * FP32; BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-8 of each at most), FP32 ones in FP32.
- * A score beyond FP32's range, an infinity or NaN in a query or in a key that it sees gives NaN, in a value that it
- * sees the same or an infinity. What a query does not see has no part in its result.
+ * strides of at most 2^24 elements. Rows of no sequence are left as they were. Products q . k, scores, softmax statistics and
+ * sums are FP32. BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-8 of each at most). FP32
+ * ones are multiplied in FP32 or, for calls of many rows and all with heads of 512, in 16-bit parts: of queries and keys 2^-22 of
+ * each number and 2^-39 of the largest of its head may be lost then, of weights and values 2^-24.
+ * NaN in a query or in a key that it sees gives NaN, as do an infinity in a query and a product or score that is infinite in FP32;
+ * but a key whose score is -infinity has a weight of 0 (where no other is left, NaN). NaN or an infinity in a value that it sees
+ * gives the same or NaN in its column. What a query does not see has no part in its result.
  */
 typedef struct {
     int batch;                   /* 0 .. 2^20 */
