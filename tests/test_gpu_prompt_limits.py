@@ -6,6 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import step_util as S
+import turbo_decode_tail as T
 from test_gpu_prompt_attention import BF16, F32, call, check, inputs
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +81,65 @@ def test_strong_channels_of_one_operand(lengths, hq, hk, d, power, strong):
         bound = mean * (2 * score + (n + 16) * 2.0**-24) * 1.01 + want.abs() * 2.0**-23 + 1e-30
         far = (out[rows].double() - want).abs()
         assert bool((far <= bound).all()), (n, (far / bound).max().item())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 128, 256, 512])
+@pytest.mark.parametrize("lengths,hq,hk", FORMS)
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("first,second", [(0, 77), (40, 41), (77, 60)])
+def test_columns_that_are_not_finite_by_different_keys(lengths, hq, hk, d, dtype, window, first, second):
+    """NaN in one column and an infinity in another, each met by the rows that see it, whichever of both they see."""
+    q, k, v = inputs(lengths, hq, hk, d, dtype, 24)
+    clean = v.clone()
+    n, g = lengths[0], hq // hk
+    v[first, 0, 5], v[second, 0, d - 1] = math.nan, math.inf
+    out = call(q, k, v, lengths, dtype, window=window)
+    seen = S.causal(n, window)
+    bad = torch.zeros((n, g, d), dtype=torch.bool, device="cuda")
+    bad[seen[:, first], :, 5] = True
+    bad[seen[:, second], :, d - 1] = True
+    assert torch.equal(~out[:n, :g].isfinite(), bad) and bool(out[n:].isfinite().all()) and bool(out[:n, g:].isfinite().all())
+    want, mean, size = S.softmax_rows(q[:n], k[:n], clean[:n], seen, d**-0.5)
+    bound = S.prompt_bound(want, mean, size, d**-0.5, d, n, dtype == BF16)
+    far = (out[:n].double() - want).abs()
+    far[:, :g][bad] = 0.0
+    assert bool((far <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 256, 512])
+@pytest.mark.parametrize("lengths,hq,hk", FORMS)
+def test_values_near_the_largest_number(lengths, hq, hk, d, dtype):
+    """A value that a weight above 1 would take out of FP32 before the sum is divided."""
+    q, k, v = inputs(lengths, hq, hk, d, dtype, 25, size=3.0)
+    v[20, 0, 7] = 3e38
+    check(q, k, v, call(q, k, v, lengths, dtype), lengths, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d,hq,hk", [(128, 8, 2), (256, 4, 2), (512, 4, 1)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_one_bad_token_does_not_hold_the_call(d, hq, hk, dtype, what):
+    """NaN in the first token of a long prompt, which every row of its heads sees."""
+    q, k, v = inputs([6000], hq, hk, d, dtype, 26)
+    out, st = torch.empty_like(q), S.ids([0, 6000])
+    inp = T.make_prompt_inputs(1, 6000, dtype=dtype, q=q, k=k, v=v, out=out, q_heads=hq, kv_heads=hk, head_dim=d, starts=st, scale=d**-0.5)
+
+    def ms():
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            T.prompt_attention(inp)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    before = ms()
+    (k if what == "k" else v)[0, 0, 3] = math.nan
+    after = ms()
+    print(f"{what} d {d} dtype {dtype}: {before:.3f} ms, with NaN {after:.3f}")
+    assert bool(out[:, :hq // hk, 3].isnan().all())
+    assert after < 4 * before + 1.0

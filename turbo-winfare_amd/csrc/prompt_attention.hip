@@ -175,48 +175,162 @@ struct Rows {
     __device__ inline bool all(const PromptArgs& a, uint32_t base, uint32_t n) const { return base + n <= first + 1u && base >= from(a, last); }
 };
 
-// DW columns of one row again, by one wave, where the products gave a number that is not finite. An infinite or NaN value turns
-// every row of its tile to NaN, also those that do not see it, as its weight is 0 there; here such values are added as
-// they are to the rows that see them. A lane takes a key for the scores and a column of 64 for the values.
+// A value that is infinite or NaN turns every row of its tile to NaN, also those that do not see it, as its weight is 0 there, and a
+// key that is infinite does where FP32 enters in parts. What has to be computed again for that is found at the end, among the rows
+// (bits of `left`, from row0 on) whose result is not finite. Where a row's sum of weights is NaN or 0 its scores make it so, and
+// it stays. The others stay where each column that is not finite in one of them has such a value at a key that all of them see;
+// the keys are gone through from the first on. NaN in the first token of 6,000, which every later row sees: 0.11 ms as without it,
+// 22 if all rows are computed again (heads of 128, 8 / 2 of them).
 template <int D, int DW, class E>
-__device__ inline void redo_row(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row, uint32_t column) {
-    const uint32_t lane = threadIdx.x & 63u, token = row / a.group, head = kv_head * a.group + row - token * a.group;
-    const uint32_t lo = Rows::from(a, token);
-    const E* q = static_cast<const E*>(a.q) + (uint64_t)(it.first + token) * a.q_stride + (uint64_t)head * D;
+__device__ inline bool stays(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row0, uint32_t left, uint32_t column) {
+    constexpr uint32_t kAtOnce = 8u;
+    constexpr int kCols = DW > 64 ? DW / 64 : 1;  // of a lane
+    const uint32_t lane = min(threadIdx.x & 63u, DW - 1u);
+    const uint32_t from = Rows::from(a, (row0 + 31u - (uint32_t)__clz((int)left)) / a.group), to = (row0 + (uint32_t)__ffs(left) - 1u) / a.group;
+    bool open[kCols];  // columns that are not finite, until a value is found
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) open[i] = false;
+#pragma nounroll
+    for (uint32_t rest = left; rest; rest &= rest - 1u) {
+        const uint32_t row = row0 + (uint32_t)__ffs(rest) - 1u, token = row / a.group;
+        const E* out = static_cast<const E*>(a.out) + (uint64_t)(it.first + token) * a.out_stride + (uint64_t)(kv_head * a.group + row - token * a.group) * D + column + lane;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) open[i] = open[i] || not_finite(number(out[i * 64]));
+    }
+    const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D + column + lane;
+    auto some_open = [&] {
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) some = some || open[i];
+        return __any(some);
+    };
+    bool some = some_open();
+#pragma nounroll
+    for (uint32_t base = from; some && base <= to; base += kAtOnce) {
+        E x[kAtOnce][kCols];
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j)
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) x[j][i] = v[(uint64_t)min(base + j, to) * a.v_stride + i * 64];
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j)
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) open[i] = open[i] && !not_finite(number(x[j][i]));
+        some = some_open();
+    }
+    return !some;
+}
+
+// DW columns of up to kRedo rows again (bits of `rows`, from row0 on), by one wave: number by number, from what a row sees alone;
+// infinite and NaN values are added as they are. A lane takes a key for the scores and a column of 64 for the values. The rows go
+// over the keys together, one after the other NaN amid 6,000 tokens of FP32 takes 20 ms in place of 7. A score of NaN or +infinity decides a row at once.
+constexpr uint32_t kRedo = 4;
+template <int D, int DW, class E>
+__device__ inline void redo_rows(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row0, uint32_t rows, uint32_t column) {
+    constexpr int kPiece = 16 / sizeof(E);  // numbers of 16 bytes
+    constexpr uint32_t kAtOnce = 8u;
+    constexpr int kCols = DW > 64 ? DW / 64 : 1;  // of a lane
+    const uint32_t lane = threadIdx.x & 63u, n = (uint32_t)__popc(rows);
+    uint32_t token[kRedo], head[kRedo], lo[kRedo];  // of the rows, the last one again where there are fewer
+    float m[kRedo], l[kRedo], sum[kRedo][kCols];
+#pragma unroll
+    for (uint32_t r = 0; r < kRedo; ++r) {
+        const uint32_t row = row0 + (uint32_t)__ffs(rows) - 1u;
+        if (r + 1u < n) rows &= rows - 1u;
+        token[r] = row / a.group, head[r] = kv_head * a.group + row - token[r] * a.group;
+        lo[r] = Rows::from(a, token[r]);
+        m[r] = kNegInf, l[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) sum[r][i] = 0.0f;
+    }
     const E* k = static_cast<const E*>(a.k) + (uint64_t)it.first * a.k_stride + (uint64_t)kv_head * D;
-    const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D + column;
-    float m = kNegInf, l = 0.0f, sum[DW / 64];
-#pragma unroll
-    for (int i = 0; i < DW / 64; ++i) sum[i] = 0.0f;
+    const E* v = static_cast<const E*>(a.v) + (uint64_t)it.first * a.v_stride + (uint64_t)kv_head * D + column + min(lane, DW - 1u);
+    auto query = [&](uint32_t r) { return static_cast<const E*>(a.q) + (uint64_t)(it.first + token[r]) * a.q_stride + (uint64_t)head[r] * D; };
+    union Piece {
+        uint4 u;
+        E e[kPiece];
+    };
+    const uint32_t last = token[kRedo - 1u];
 #pragma nounroll
-    for (uint32_t base = lo; base <= token; base += 64u) {
-        const E* key = k + (uint64_t)min(base + lane, token) * a.k_stride;
-        float s = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < D; ++i) s = fmaf(number(q[i]), number(key[i]), s);
-        if (a.flip) s = -s;
-        s = base + lane <= token ? s * a.scale_log2e : kNegInf;
-        const float now = fmaxf(m, wave_max(s)), zero = now == kNegInf ? 0.0f : now;
-        const float alpha = __builtin_amdgcn_exp2f(m - zero), p = __builtin_amdgcn_exp2f(s - zero);
-        m = now;
-        l = l * alpha + wave_sum(p);
+    for (uint32_t base = lo[0]; base <= last; base += 64u) {
+        const E* key = k + (uint64_t)min(base + lane, last) * a.k_stride;
+        float s[kRedo];
 #pragma unroll
-        for (int i = 0; i < DW / 64; ++i) sum[i] *= alpha;
+        for (uint32_t r = 0; r < kRedo; ++r) s[r] = 0.0f;
 #pragma nounroll
-        for (uint32_t j = 0; j < min(64u, token + 1u - base); ++j) {
-            const float w = lane_read(p, (int)j);
+        for (int i0 = 0; i0 < D; i0 += 4 * kPiece) {
+            Piece y[4];
 #pragma unroll
-            for (int i = 0; i < DW / 64; ++i) {
-                const float x = number(v[(uint64_t)(base + j) * a.v_stride + i * 64 + lane]);
-                sum[i] = not_finite(x) ? sum[i] + x : fmaf(w, x, sum[i]);
-            }
+            for (int i = 0; i < 4; ++i) y[i].u = *reinterpret_cast<const uint4*>(key + i0 + i * kPiece);
+#pragma unroll
+            for (uint32_t r = 0; r < kRedo; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    Piece x;
+                    x.u = *reinterpret_cast<const uint4*>(query(r) + i0 + i * kPiece);
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) s[r] = fmaf(number(x.e[j]), number(y[i].e[j]), s[r]);
+                }
+        }
+        bool some = false;  // of the rows goes on
+#pragma unroll
+        for (uint32_t r = 0; r < kRedo; ++r) {
+            const bool sees = base + lane >= lo[r] && base + lane <= token[r];
+            const float t = sees ? (a.flip ? -s[r] : s[r]) * a.scale_log2e : kNegInf;
+            if (__any(!(t < __builtin_inff()))) l[r] = __builtin_nanf("");
+            some = some || l[r] == l[r];
+            const float now = fmaxf(m[r], wave_max(t)), zero = now == kNegInf ? 0.0f : now;
+            const float alpha = __builtin_amdgcn_exp2f(m[r] - zero);
+            s[r] = __builtin_amdgcn_exp2f(t - zero);
+            m[r] = now;
+            l[r] = l[r] * alpha + wave_sum(s[r]);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) sum[r][i] *= alpha;
+        }
+        if (!some) break;
+        const uint32_t keys = min(64u, last + 1u - base);
+#pragma nounroll
+        for (uint32_t j0 = 0; j0 < keys; j0 += kAtOnce) {
+            E x[kAtOnce][kCols];
+#pragma unroll
+            for (uint32_t j = 0; j < kAtOnce; ++j)
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) x[j][i] = v[(uint64_t)min(base + j0 + j, last) * a.v_stride + i * 64];
+#pragma unroll
+            for (uint32_t j = 0; j < kAtOnce; ++j)
+#pragma unroll
+                for (uint32_t r = 0; r < kRedo; ++r) {
+                    const uint32_t at = base + j0 + j;
+                    if (at < lo[r] || at > token[r]) continue;
+                    const float w = lane_read(s[r], (int)(j0 + j));
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) {
+                        const float y = number(x[j][i]);
+                        sum[r][i] = not_finite(y) ? sum[r][i] + y : fmaf(w, y, sum[r][i]);
+                    }
+                }
         }
     }
-    E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token) * a.out_stride + (uint64_t)head * D + column + lane;
 #pragma unroll
-    for (int i = 0; i < DW / 64; ++i) {
-        if constexpr (sizeof(E) == 4) to[i * 64] = sum[i] / l;
-        else to[i * 64] = (uint16_t)pack_bf16(sum[i] / l, 0.0f);
+    for (uint32_t r = 0; r < kRedo; ++r) {
+        if (r >= n || lane >= (uint32_t)DW) break;
+        E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token[r]) * a.out_stride + (uint64_t)head[r] * D + column + lane;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+            if constexpr (sizeof(E) == 4) to[i * 64] = sum[r][i] / l[r];
+            else to[i * 64] = (uint16_t)pack_bf16(sum[r][i] / l[r], 0.0f);
+        }
+    }
+}
+// All the rows of `left`, or the shares of `sharers` waves that have the same rows.
+template <int D, int DW, class E>
+__device__ inline void redo(const PromptArgs& a, const Item& it, uint32_t kv_head, uint32_t row0, uint32_t left, uint32_t column, uint32_t sharers = 1u,
+                            uint32_t share = 0u) {
+#pragma nounroll
+    for (uint32_t n = 0; left; ++n) {
+        uint32_t rows = 0u;
+        for (uint32_t r = 0; r < kRedo && left; ++r) rows |= left & -left, left &= left - 1u;
+        if (n % sharers == share) redo_rows<D, DW, E>(a, it, kv_head, row0, rows, column);
     }
 }
 
@@ -337,10 +451,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_few32(const PromptArgs a) {
             *reinterpret_cast<float4*>(to + n * 64 + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
     }
-    if (odd && token < it.len) atomicOr(&sh.odd, 1u << row);
+    if (odd && token < it.len && total > 0.0f) atomicOr(&sh.odd, 1u << row);
     __syncthreads();  // what was written is written over, in order
-    for (uint32_t left = sh.odd, n = 0; left; left &= left - 1u, ++n)
-        if (n % kWaves == wave) redo_row<D, D, float>(a, it, kv_head, it.tile * kRows + (uint32_t)__ffs(left) - 1u, 0u);
+    uint32_t left = sh.odd;
+    if (left == 0u || stays<D, D, float>(a, it, kv_head, it.tile * kRows, left, 0u)) return;
+    __syncthreads();  // all have read what is written over
+    redo<D, D, float>(a, it, kv_head, it.tile * kRows, left, 0u, kWaves, wave);
 }
 
 // Many rows: every wave has 32 rows of its own, and tiles of KT keys and values go from memory to LDS, without passing
@@ -620,21 +736,12 @@ __global__ __launch_bounds__(64 * W * TEAMS, WAVES) void k_many(const PromptArgs
         for (int e = 0; e < 4; ++e) z[e] = y[n % 4 * 4 + e] * by, odd = odd || not_finite(z[e]);
         if (rows.exists) *reinterpret_cast<uint2*>(to + n * 8) = make_uint2(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]));
     }
-    const unsigned long long both = __ballot(odd && rows.exists);
-    uint32_t left = (uint32_t)both | (uint32_t)(both >> 32);
-    if constexpr (TEAMS > 1) {  // all teams' columns of a row are one team's, after all have written theirs
-        __syncthreads();
-        uint32_t* rows_of = reinterpret_cast<uint32_t*>(&sh.stats[0][wave][0]);
-        if (team == 0u && lane == 0u) *rows_of = 0u;
-        __syncthreads();
-        if (lane == 0u && left) atomicOr(rows_of, left);
-        __syncthreads();
-        left = *rows_of;
-        for (uint32_t n = 0; left; left &= left - 1u, ++n)
-            if (n % TEAMS == team) redo_row<D, D, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, 0u);
-    } else {
-        for (; left; left &= left - 1u) redo_row<D, DW, uint16_t>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
-    }
+    const unsigned long long both = __ballot(odd && rows.exists && l > 0.0f);
+    const uint32_t left = (uint32_t)both | (uint32_t)(both >> 32);
+    // a wave has its columns of a row to itself, a team's after the join too
+    constexpr int kOwn = DW / TEAMS;
+    if (__builtin_expect(left != 0u, 0) && !stays<D, kOwn, uint16_t>(a, it, kv_head, mine, left, column + team * kOwn))
+        redo<D, kOwn, uint16_t>(a, it, kv_head, mine, left, column + team * kOwn);
 }
 
 // Many rows of FP32. The matrix unit multiplies 16-bit numbers at 16 times its rate of FP32 ones, so every number enters as
@@ -652,6 +759,7 @@ struct Many32 {
     uint16_t k[kOnePlace ? kValueWords : kKeyWords], v[kOnePlace ? 8 : kValueWords];
     float4 scores[PARTS > 1 ? W : 1][PARTS > 1 ? 4 : 1][64];
     int power[kKeys];  // of the keys
+    int infinite;      // some key holds an infinity, of which the parts are not numbers
 };
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -767,6 +875,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
         for (uint32_t d = 1; d < kPerKey; d *= 2u) top = fmaxf(top, __shfl_xor(top, (int)d));
         const int power = power_to_fp16(top);
         if (my_col == 0u) sh.power[my_key] = -power;
+        if (not_finite(top)) sh.infinite = 1;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             uint2 h, l;
@@ -793,6 +902,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
     Softmax sm;
 #pragma unroll
     for (int i = 0; i < DW / 32; ++i) o[i] = zeros();
+    if (threadIdx.x == 0u) sh.infinite = 0;
     for (uint32_t base = begin; base < end; base += kKeys) {
         if constexpr (D == 512) {
             // from one place each, made anew here: kept over the loop they spill
@@ -887,7 +997,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
             }
     }
 
-    const float by = 1.0f / halves_sum(sm.l);
+    const float l = halves_sum(sm.l), by = 1.0f / l;
     float* to = static_cast<float*>(a.out) + (uint64_t)(it.first + rows.pos) * a.out_stride + (uint64_t)rows.head * D + column + half * 4u;
     bool odd = false;
 #pragma unroll
@@ -900,9 +1010,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_many32(const PromptArgs a) {
             for (int e = 0; e < 4; ++e) z[e] = y[r + e] * by, odd = odd || not_finite(z[e]);
             if (rows.exists) *reinterpret_cast<float4*>(to + i * 32 + 2 * r) = make_float4(z[0], z[1], z[2], z[3]);
         }
-    const unsigned long long both = __ballot(odd && rows.exists);
-    for (uint32_t left = (uint32_t)both | (uint32_t)(both >> 32); left; left &= left - 1u)
-        redo_row<D, DW, float>(a, it, kv_head, mine + (uint32_t)__ffs(left) - 1u, column);
+    const unsigned long long both = __ballot(odd && rows.exists && (l > 0.0f || sh.infinite));
+    uint32_t left = (uint32_t)both | (uint32_t)(both >> 32);
+    if (left && !sh.infinite && stays<D, DW, float>(a, it, kv_head, mine, left, column)) return;
+    redo<D, DW, float>(a, it, kv_head, mine, left, column);
 }
 
 // As many workgroups of up to 512 threads as locate() may give numbers to, over all key/value heads.
