@@ -46,6 +46,11 @@ inline size_t check_rows(const char* name, const void* p, size_t stride, size_t 
     return stride;
 }
 
+inline void check_words(const char* name, const void* p, uintptr_t align = 4u) {
+    if (!p) fail(std::string(name) + " is NULL");
+    if (reinterpret_cast<uintptr_t>(p) % align != 0u) fail(std::string(name) + " must be " + std::to_string(align) + "-byte aligned");
+}
+
 }  // namespace tdt
 
 #define ATT_TRY            \

@@ -218,7 +218,8 @@ TURBO_DT_API int turbo_kv_cache_move(void* handle, const uint32_t* source, const
     if (width < 1 || width > (int)tdt::kTreeNodes) fail("width must be in 1..64");
     if (rows < 0 || rows > (1 << 20)) fail("rows must be in 0..1048576");
     if (rows == 0) return 1;
-    if (!source || !target) fail("source or target is NULL");
+    check_words("source", source);
+    check_words("target", target);
     tdt::KvMoveArgs a{};
     a.kv = c->kv;
     a.source = source;

@@ -25,11 +25,6 @@ void check_batch(int batch) {
     if (batch < 0 || batch > (int)kPlanMaxBatch) fail("batch must be in 0.." + std::to_string(kPlanMaxBatch));
 }
 
-void check_words(const char* name, const void* p, uintptr_t align = 4u) {
-    if (!p) fail(std::string(name) + " is NULL");
-    if (reinterpret_cast<uintptr_t>(p) % align != 0u) fail(std::string(name) + " must be " + std::to_string(align) + "-byte aligned");
-}
-
 // The page tables and the pool, as the plan and the release take them.
 void check_pool(int batch, uint32_t page_stride, const void* pages, const void* held, const void* free_pages, uint32_t free_capacity,
                 const void* free_count, uint32_t prefix_len) {
