@@ -512,7 +512,8 @@ TURBO_DT_API int turbo_kv_cache_move(void* cache, const uint32_t* source, const 
  * What the calls above take as slots, positions, lengths, page tables and masks, made on the device from the
  * lengths of the sequences, and attention over prompts that are not in a cache yet. No counterpart in the reference
  * (one sequence, a ring of 4096). The calls have no handle: they run on the device that they name, on hip_stream,
- * allocate nothing and may be captured into a HIP graph.
+ * allocate nothing and may be captured into a HIP graph. The arrays of a call that it writes share no bytes with each other or
+ * with those that it reads, where nothing else is said.
  */
 
 /* A page that a sequence needs and the pool did not have. */
@@ -586,7 +587,8 @@ TURBO_DT_API int turbo_pages_release(const TurboPagesRelease* in, void* hip_stre
  * then, from the last kept node on, the first child whose token is the one chosen after that node (turbo_lmhead_step's
  * tokens over the nodes as rows; 0xFFFFFFFF, its mark of a degenerate row, confirms nothing). next is the choice after the last kept node:
  * node 0 of the following step. The i-th kept node's key and value belong at the slot of node i: source and target
- * say so to turbo_kv_cache_move, once for each layer's cache. Parents as in TurboBatchPlan.
+ * say so to turbo_kv_cache_move, once for each layer's cache. Parents as in TurboBatchPlan. A result may be an input itself, of
+ * the same size (length past_len, for one).
  */
 typedef struct {
     int batch;                      /* 0 .. 2^20 */

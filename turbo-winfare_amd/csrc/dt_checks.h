@@ -51,6 +51,17 @@ inline void check_words(const char* name, const void* p, uintptr_t align = 4u) {
     if (reinterpret_cast<uintptr_t>(p) % align != 0u) fail(std::string(name) + " must be " + std::to_string(align) + "-byte aligned");
 }
 
+// An array of a call, and whether two have bytes in common (an absent one has none).
+struct Span {
+    const void* p;
+    uint64_t bytes;
+    bool meets(const Span& other) const {
+        const uint64_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(other.p);
+        return p && other.p && bytes && other.bytes && a < b + other.bytes && b < a + bytes;
+    }
+    bool is(const Span& other) const { return p == other.p && bytes == other.bytes; }
+};
+
 }  // namespace tdt
 
 #define ATT_TRY            \

@@ -73,17 +73,21 @@ TURBO_DT_API int turbo_batch_plan(const TurboBatchPlan* in, void* hip_stream) {
                           static_cast<const void*>(in->positions), static_cast<const void*>(in->slots), static_cast<const void*>(in->totals)})
         if (reinterpret_cast<uintptr_t>(p) % 4u != 0u) fail("an array of the plan is not 4-byte aligned");
     // what some workgroups read while others write results; held, free_count and past_len may be updated in place
-    const void* inputs[] = {in->past_len, in->new_len, in->held, in->free_pages, in->free_count, in->parents, in->pages};
-    const void* results[] = {in->held_out, in->free_count_out, in->kv_len, in->starts, in->positions, in->slots, in->totals, in->masks};
-    for (const void*& r : results) {
-        if (!r) continue;
-        for (const void* p : inputs)
-            if (p == r && !(r == in->held_out && p == in->held) && !(r == in->free_count_out && p == in->free_count) &&
-                !(r == in->kv_len && p == in->past_len))
-                fail("a result of the plan is one of its inputs");
-        for (const void*& other : results)
-            if (&other != &r && other == r) fail("two results of the plan are one array");
+    const uint64_t each = 4u * (uint64_t)in->batch, nodes = (uint64_t)in->batch * in->row_tokens, tokens = 4u * (uint64_t)in->max_tokens;
+    const Span past{in->past_len, each}, held{in->held, each}, count{in->free_count, 4u}, pages{in->pages, each * in->page_stride};
+    const Span held_out{in->held_out, each}, count_out{in->free_count_out, 4u}, kv_len{in->kv_len, each};
+    const Span inputs[] = {past, held, count, pages, {in->new_len, each}, {in->free_pages, 4u * (uint64_t)in->free_capacity}, {in->parents, 4u * nodes}};
+    const Span results[] = {held_out, count_out, kv_len, {in->starts, each + 4u}, {in->positions, tokens}, {in->slots, tokens}, {in->totals, 16u},
+                            {in->masks, 8u * nodes}};
+    for (const Span& r : results) {
+        for (const Span& i : inputs)
+            if (r.meets(i) && !(r.is(i) && ((r.is(held_out) && i.is(held)) || (r.is(count_out) && i.is(count)) || (r.is(kv_len) && i.is(past)))))
+                fail("a result of the plan lies on one of its inputs");
+        for (const Span& other : results)
+            if (&other != &r && other.meets(r)) fail("two results of the plan lie on each other");
     }
+    for (const Span& i : inputs)
+        if (&i != &inputs[3] && pages.meets(i)) fail("the page tables lie on another input of the plan");
     check_device(in->device);
     a.batch = (uint32_t)in->batch;
     a.prefix_len = in->prefix_len;
@@ -121,6 +125,15 @@ TURBO_DT_API int turbo_pages_release(const TurboPagesRelease* in, void* hip_stre
     if (in->batch == 0) return 1;
     check_words("keep_len", in->keep_len);
     check_pool(in->batch, in->page_stride, in->pages, in->held, in->free_pages, in->free_capacity, in->free_count, in->prefix_len);
+    const uint64_t each = 4u * (uint64_t)in->batch;
+    const Span updated[] = {{in->held, each}, {in->free_pages, 4u * (uint64_t)in->free_capacity}, {in->free_count, 4u}};
+    const Span inputs[] = {{in->keep_len, each}, {in->pages, each * in->page_stride}};
+    for (const Span& u : updated) {
+        for (const Span& i : inputs)
+            if (u.meets(i)) fail("held or the pool lies on an input of the release");
+        for (const Span& other : updated)
+            if (&other != &u && other.meets(u)) fail("two updated arrays of the release lie on each other");
+    }
     check_device(in->device);
     a.batch = (uint32_t)in->batch;
     a.prefix_len = in->prefix_len;
@@ -156,6 +169,16 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream) 
     for (const void* p : {static_cast<const void*>(in->length), static_cast<const void*>(in->path), static_cast<const void*>(in->source),
                           static_cast<const void*>(in->target)})
         if (reinterpret_cast<uintptr_t>(p) % 4u != 0u) fail("an array of the tree is not 4-byte aligned");
+    // a sequence's wave has read it before it writes: a result may be updated in an input's place, of the same size
+    const uint64_t each = 4u * (uint64_t)in->batch, nodes = each * in->row_tokens;
+    const Span inputs[] = {{in->parents, nodes}, {in->new_len, each}, {in->tokens, nodes}, {in->chosen, nodes}, {in->past_len, each}, {in->slots, nodes}};
+    const Span results[] = {{in->kept, each}, {in->next, each}, {in->length, each}, {in->path, nodes}, {in->source, nodes}, {in->target, nodes}};
+    for (const Span& r : results) {
+        for (const Span& i : inputs)
+            if (r.meets(i) && !r.is(i)) fail("a result of the tree lies across one of its inputs");
+        for (const Span& other : results)
+            if (&other != &r && other.meets(r)) fail("two results of the tree lie on each other");
+    }
     check_device(in->device);
     a.batch = (uint32_t)in->batch;
     a.parents = in->parents;
