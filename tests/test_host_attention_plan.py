@@ -123,3 +123,16 @@ def test_a_tree_takes_the_scratch_that_there_is(plans):
             assert p["bytes"] <= most
     grown = [(s, r["bytes"], p["bytes"]) for s, r, p in zip(shapes, runs, best) if p["bytes"] > r["bytes"]]
     assert grown and runs[5]["bytes"] == 0  # 256 sequences of 64 rows are one part each as a run
+
+
+def test_the_tests_of_many_rows_take_that_form(plans):
+    """The cases of test_gpu_tree_attention.py (Many) and test_gpu_tree_many_rows.py that are there for the workgroups of 128 rows."""
+    pytest.importorskip("torch")
+    from test_gpu_tree_attention import MANY
+
+    dims, announced = (64, 128, 256), 40000
+    shapes = [(len(before), nodes, hq, hk, d, 0) for before, nodes, hq, hk in MANY for d in dims]
+    shapes += [(5, 64, 32, 4, d, prefix) for d in dims for prefix in (1, 32, 100, 999)]
+    shapes += [(3, 64, 32, 4, d, 0) for d in dims] + [(2, 64, 64, 4, d, 0) for d in dims] + [(3, 64, 64, 4, 128, 0)]
+    for shape, p in zip(shapes, hold(plans, [(*s[:5], BF16, s[5], announced - s[5], 0, True) for s in shapes])):
+        assert p["wide_splits"] > 0, shape
