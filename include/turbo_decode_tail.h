@@ -620,9 +620,9 @@ TURBO_DT_API int turbo_tree_accept(const TurboTreeAccept* in, void* hip_stream);
  * sums are FP32. BF16 inputs are multiplied as they are, their softmax weights rounded to BF16 (2^-8 of each at most). FP32
  * ones are multiplied in FP32 or, for calls of many rows and all with heads of 512, in 16-bit parts: of queries and keys 2^-22 of
  * each number and 2^-39 of the largest of its head may be lost then, of weights and values 2^-24.
- * NaN in a query or in a key that it sees gives NaN, as do an infinity in a query and a product or score that is infinite in FP32;
- * but a key whose score is -infinity has a weight of 0 (where no other is left, NaN). NaN or an infinity in a value that it sees
- * gives the same or NaN in its column. What a query does not see has no part in its result.
+ * NaN in a query or in a key that it sees gives NaN, as do an infinity in a query and a product or score of +infinity; a key whose
+ * score is -infinity has a weight of 0 (where no other is left, NaN). NaN or an infinity in a value that it sees gives the same or
+ * NaN in its column. What a query does not see has no part in its result. `tokens`, the rows that the buffers have, sizes the launch.
  */
 typedef struct {
     int batch;                   /* 0 .. 2^20 */
