@@ -50,6 +50,7 @@ def test_a_score_of_minus_infinity_weighs_nothing(lengths, hq, hk, d, dtype, fli
     assert bool(out[at:n, :g].isnan().all()) and bool(out[:at].isfinite().all()) and bool(out[n:].isfinite().all())
     # nothing but such keys: no weight is left
     k[:n, 0, 3] = -math.inf * flip
+    v[at, 0, 7] = math.inf
     assert bool(call(q, k, v, lengths, dtype, scale=flip * d**-0.5)[:n, :g].isnan().all())
 
 

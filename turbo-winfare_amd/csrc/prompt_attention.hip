@@ -315,6 +315,7 @@ __device__ inline void redo_rows(const PromptArgs& a, const Item& it, uint32_t k
     for (uint32_t r = 0; r < kRedo; ++r) {
         if (r >= n || lane >= (uint32_t)DW) break;
         E* to = static_cast<E*>(a.out) + (uint64_t)(it.first + token[r]) * a.out_stride + (uint64_t)head[r] * D + column + lane;
+        if (l[r] == 0.0f) l[r] = __builtin_nanf("");  // no weight is left, for an infinite value either
 #pragma unroll
         for (int i = 0; i < kCols; ++i) {
             if constexpr (sizeof(E) == 4) to[i * 64] = sum[r][i] / l[r];
